@@ -547,6 +547,96 @@ int vh_residual_add_backward(const float* dout, const void* branch, int32_t bran
                              const float* mask, void* dbranch, float* dgamma, int64_t total, int64_t channels,
                              int64_t spatial, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Operators of token lines [B, N, C]: the short causal convolution, the selective state
+ * space scan and the gated LayerNorm of rows.  No counterpart in the reference, whose only
+ * recurrence is SRNL.  Activations come with the element strides of a sequence (`_batch`)
+ * and of a token (`_token`), channels dense, so a slice of a wider projection needs no copy;
+ * outputs are dense.  `lengths` (int32 [B] or NULL) ends each sequence early (values are
+ * clamped to 0..N): outputs and gradients behind the end are zero, states are those at it.
+ * ------------------------------------------------------------------------- */
+
+/* y[t, c] = f(bias[c] + sum_k weight[c, k] x[t - taps + 1 + k, c]), f = SiLU (silu = 1) or the
+ * identity; weight [C, taps] and bias [C] (or NULL) fp32, taps 2..8.  The taps - 1 inputs
+ * before the first token are `state` [B, taps - 1, C] in io_dtype (NULL: zero); new_state (or
+ * NULL) receives the last taps - 1 inputs of every sequence and must not overlap state. */
+int vh_causal_conv_forward(const void* x, int64_t x_batch, int64_t x_token, int32_t io_dtype, const float* weight,
+                           const float* bias, int32_t silu, const void* state, const int32_t* lengths, void* y,
+                           void* new_state, int64_t B, int64_t N, int64_t C, int32_t taps, void* stream);
+
+/* Gradients of vh_causal_conv_forward: dx [B, N, C] and dstate [B, taps - 1, C] (or NULL) in
+ * io_dtype, dweight [C, taps] and dbias [C] fp32 (each may be NULL); dnew_state (or NULL) is
+ * the gradient of new_state.  Parameter gradients are summed in a fixed order. */
+size_t vh_causal_conv_backward_workspace_bytes(int64_t B, int64_t N, int64_t C, int32_t taps);
+int vh_causal_conv_backward(const void* dy, int64_t dy_batch, int64_t dy_token, const void* x, int64_t x_batch,
+                            int64_t x_token, int32_t io_dtype, const float* weight, const float* bias, int32_t silu,
+                            const void* state, const int32_t* lengths, const void* dnew_state, void* dx, float* dweight,
+                            float* dbias, void* dstate, int64_t B, int64_t N, int64_t C, int32_t taps, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* One token of every sequence: x [B, C] (rows x_batch apart), state and new_state
+ * [B, taps - 1, C] (may be the same memory, must not overlap otherwise), y [B, C]. */
+int vh_causal_conv_step(const void* x, int64_t x_batch, int32_t io_dtype, const float* weight, const float* bias,
+                        int32_t silu, const void* state, void* new_state, void* y, int64_t B, int64_t C, int32_t taps,
+                        void* stream);
+
+/* Selective state space scan, S states a channel in FP32:
+ *   step = softplus(dt + dt_bias) (softplus = 1) or dt + dt_bias
+ *   h[n] = exp(step A[c, n]) h[n] + step x B[n],   y = (sum_n C[n] h[n] + D x) silu(gate)
+ * x, dt, gate (or NULL) [B, N, C] in io_dtype; b, c [B, N, groups, S] in bc_dtype (fp32, or
+ * bf16 with bf16 activations), the [groups, S] part dense, 4-byte aligned rows, channel c in
+ * group c / (C / groups); A [C, S], D and dt_bias [C] (or NULL) fp32; states S = 8, 16 or 32
+ * (zero-pad others: a state with A = B = C = 0 changes nothing).  state and new_state
+ * [B, C, S] fp32 (or NULL), 16-byte aligned, not overlapping.  kept (or NULL) receives what
+ * the backward starts from (vh_state_space_kept_bytes).  Workspace from the query (may be 0). */
+size_t vh_state_space_workspace_bytes(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states);
+size_t vh_state_space_kept_bytes(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states);
+int vh_state_space_forward(
+    const void* x, int64_t x_batch, int64_t x_token, const void* dt, int64_t dt_batch, int64_t dt_token,
+    const void* gate, int64_t gate_batch, int64_t gate_token, int32_t io_dtype,
+    const void* b, int64_t b_batch, int64_t b_token, const void* c, int64_t c_batch, int64_t c_token, int32_t bc_dtype,
+    const float* A, const float* D, const float* dt_bias, int32_t softplus, const float* state,
+    const int32_t* lengths, void* y, float* new_state, float* kept, int64_t B, int64_t N, int64_t C, int32_t groups,
+    int32_t states, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of vh_state_space_forward from its inputs and kept: dx, ddt, dgate (exactly with
+ * a gate) [B, N, C] and db, dc [B, N, groups, S] in io_dtype; dA [C, S], dD [C], ddt_bias [C]
+ * (each may be NULL) and dstate [B, C, S] (or NULL) fp32; dnew_state (or NULL) is the gradient
+ * of new_state.  Sums over tokens, channels and sequences run in a fixed order. */
+size_t vh_state_space_backward_workspace_bytes(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states);
+int vh_state_space_backward(
+    const void* dy, int64_t dy_batch, int64_t dy_token, const void* x, int64_t x_batch, int64_t x_token,
+    const void* dt, int64_t dt_batch, int64_t dt_token, const void* gate, int64_t gate_batch, int64_t gate_token,
+    int32_t io_dtype, const void* b, int64_t b_batch, int64_t b_token, const void* c, int64_t c_batch, int64_t c_token,
+    int32_t bc_dtype, const float* A, const float* D, const float* dt_bias, int32_t softplus, const int32_t* lengths,
+    const float* kept, const float* dnew_state, void* dx, void* ddt, void* dgate, void* db, void* dc, float* dA,
+    float* dD, float* ddt_bias, float* dstate, int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token of every sequence: x, dt, gate [B, C] and b, c [B, groups, S] in io_dtype, rows the
+ * given element strides apart; S = 1..32; state and new_state [B, C, S] fp32 (may be the same
+ * memory, must not overlap otherwise); y [B, C]. */
+int vh_state_space_step(
+    const void* x, int64_t x_batch, const void* dt, int64_t dt_batch, const void* gate, int64_t gate_batch,
+    int32_t io_dtype, const void* b, int64_t b_batch, const void* c, int64_t c_batch, const float* A, const float* D,
+    const float* dt_bias, int32_t softplus, const float* state, float* new_state, void* y, int64_t B, int64_t C,
+    int32_t groups, int32_t states, void* stream);
+
+/* LayerNorm of rows [rows, C] (C <= 8192; element strides between the rows) with an optional
+ * gate: y = ((x - mean) rstd weight + bias) silu(gate), biased variance, weight and bias [C]
+ * fp32; mean and rstd [rows] for the backward (both or neither).  The backward gives dx and
+ * dgate (exactly with a gate) in io_dtype, dweight and dbias [C] fp32 (each may be NULL),
+ * summed in a fixed order. */
+int vh_gated_layernorm_forward(const void* x, int64_t x_row, const void* gate, int64_t gate_row, int32_t io_dtype,
+                               const float* weight, const float* bias, void* y, float* mean, float* rstd, int64_t rows,
+                               int64_t channels, float eps, void* stream);
+size_t vh_gated_layernorm_backward_workspace_bytes(int64_t rows, int64_t channels);
+int vh_gated_layernorm_backward(const void* dy, int64_t dy_row, const void* x, int64_t x_row, const void* gate,
+                                int64_t gate_row, int32_t io_dtype, const float* weight, const float* bias,
+                                const float* mean, const float* rstd, void* dx, void* dgate, float* dweight,
+                                float* dbias, int64_t rows, int64_t channels, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -154,3 +154,71 @@ def residual_add_torch(residual, branch, gamma, drop_scale):
     """``residual + branch gamma_c drop_scale_b`` on NCHW tensors."""
     c = branch.shape[1]
     return residual + branch * gamma.reshape(1, c, 1, 1) * drop_scale.reshape(-1, 1, 1, 1)
+
+
+# ---- operators of token lines (no counterpart in the reference) -----------------------
+
+def _before(lengths, length):
+    """[B, N, 1] mask of the tokens before each sequence's end (True without lengths)."""
+    if lengths is None:
+        return torch.ones(1, 1, 1, dtype=torch.bool)
+    return (torch.arange(length)[None, :] < lengths.clamp(0, length)[:, None])[..., None]
+
+
+def causal_conv_torch(x, weight, bias=None, silu=False, state=None, lengths=None):
+    """Token by token: y[t] = f(bias + sum_k weight[k] x[t - K + 1 + k]); returns (y, last
+    K - 1 inputs of every sequence)."""
+    batch, length, channels = x.shape
+    taps = weight.shape[-1]
+    weight = weight.reshape(channels, taps)
+    if state is None:
+        state = torch.zeros(batch, taps - 1, channels, dtype=x.dtype)
+    live = _before(lengths, length)
+    line = torch.cat((state, torch.where(live, x, torch.zeros((), dtype=x.dtype))), dim=1)
+    rows = []
+    for t in range(length):
+        pre = (line[:, t:t + taps] * weight.t()).sum(1)
+        pre = pre if bias is None else pre + bias
+        rows.append(torch.nn.functional.silu(pre) if silu else pre)
+    y = torch.where(live, torch.stack(rows, 1), torch.zeros((), dtype=x.dtype))
+    ends = [length] * batch if lengths is None else lengths.clamp(0, length).tolist()
+    return y, torch.stack([line[i, n:n + taps - 1] for i, n in enumerate(ends)])
+
+
+def state_space_scan_torch(x, dt, A, B, C, D=None, gate=None, dt_bias=None, softplus=True, state=None, lengths=None):
+    """Token by token: h = exp(step A) h + step x B, y = (C h + D x) silu(gate), with B and C
+    [B, N, groups, S]; returns (y, last state of every sequence)."""
+    batch, length, channels = x.shape
+    groups, states = B.shape[2:]
+    live = _before(lengths, length)
+    none = torch.zeros((), dtype=x.dtype)
+    step = dt if dt_bias is None else dt + dt_bias
+    if softplus:
+        step = torch.nn.functional.softplus(step, threshold=200.0)
+    step, x = torch.where(live, step, none), torch.where(live, x, none)
+    B, C = torch.where(live[..., None], B, none), torch.where(live[..., None], C, none)
+    if gate is not None:
+        gate = torch.where(live, gate, none)
+    h = torch.zeros(batch, channels, states, dtype=x.dtype) if state is None else state
+
+    def spread(v):   # [B, groups, S] -> [B, C, S]
+        return v.repeat_interleave(channels // groups, dim=1)
+
+    rows = []
+    for t in range(length):
+        h = torch.exp(step[:, t, :, None] * A) * h + (step[:, t] * x[:, t])[..., None] * spread(B[:, t])
+        rows.append((spread(C[:, t]) * h).sum(-1))
+    y = torch.stack(rows, 1)
+    if D is not None:
+        y = y + D * x
+    if gate is not None:
+        y = y * torch.nn.functional.silu(gate)
+    return torch.where(live, y, none), h
+
+
+def gated_layernorm_torch(x, weight, bias, eps, gate=None):
+    """LayerNorm over the last dimension (biased variance), times silu(gate)."""
+    mean = x.mean(-1, keepdim=True)
+    var = ((x - mean) ** 2).mean(-1, keepdim=True)
+    y = (x - mean) / torch.sqrt(var + eps) * weight + bias
+    return y if gate is None else y * torch.nn.functional.silu(gate)

@@ -1,0 +1,119 @@
+// Device helpers and the argument block shared by the state space scan's forward
+// (state_space.hip) and backward (state_space_backward.hip).
+//
+// Layout of the work: one lane per channel, the channel's S states in registers, tokens in
+// order.  A wave takes 64 channels of one group of one sequence over one chunk of tokens, so
+// B[t] and C[t] are the same for all its lanes and stand in scalar registers: the scalar
+// unit loads and unpacks them while the vector unit computes.
+#pragma once
+
+#include "vh_common.h"
+
+namespace vh {
+
+constexpr float SS_LOG2E = 1.44269504088896341f;
+
+// Tokens between two states that a training forward keeps for the backward, by state count.
+constexpr int ss_block_tokens(int states) { return states <= 8 ? 32 : states <= 16 ? 16 : 8; }
+
+struct SSTokens {   // an activation [B, N, ...]: element strides of sequence and token
+    const void* data;
+    int64_t bs, ts;
+};
+
+struct SSArgs {
+    SSTokens x, dt, gate, b, c, dy;
+    const float *A, *D, *dt_bias, *state;
+    const int32_t* lengths;
+    void* y;
+    float* new_state;
+    float* kept;     // [B, ceil(N / block), S, padded C]: states before each block of tokens
+    float* slots;    // [B, chunks - 1, S, padded C]: states (or adjoints) between the chunks
+    float* sums;     // [B, chunks, padded C]: sum of dt over a chunk
+    int32_t softplus;
+    int32_t batches, tokens, channels, group_channels, group_tiles, tiles;   // tiles: of 64 channels, all groups
+    int32_t chunk, chunks, first_chunk, launch_chunks, blocks;
+    // backward
+    void *dx, *ddt, *dgate;
+    float* dstate;
+    float* bc_partial;     // [tiles, B, N, 2 S]
+    float* param_partial;  // [B * chunks, S + 2, padded C]
+    const float* dnew_state;
+};
+
+// Where a workgroup of one wave stands.  Consecutive indexes are the tiles of one chunk, which
+// share B and C, and one contiguous range of them goes to each XCD.
+struct SSPlace {
+    int32_t batch, chunk, tile, group, lane, channel;
+    int64_t column;     // of the padded channels
+    bool live;          // the lane has a channel
+    int32_t t0, t1, te; // tokens [t0, t1) of the chunk, of which [t0, te) belong to the sequence
+};
+
+__device__ __forceinline__ SSPlace ss_place(const SSArgs& a) {
+    SSPlace p;
+    const uint32_t bid = xcd_remap_any(blockIdx.x, gridDim.x);
+    const uint32_t rest = bid / static_cast<uint32_t>(a.tiles);
+    p.tile = static_cast<int32_t>(bid - rest * a.tiles);
+    p.batch = static_cast<int32_t>(rest / static_cast<uint32_t>(a.launch_chunks));
+    p.chunk = static_cast<int32_t>(rest) - p.batch * a.launch_chunks + a.first_chunk;
+    p.lane = static_cast<int32_t>(threadIdx.x);
+    p.group = p.tile / a.group_tiles;
+    const int32_t in_group = (p.tile - p.group * a.group_tiles) * 64 + p.lane;
+    p.live = in_group < a.group_channels;
+    p.channel = p.group * a.group_channels + (p.live ? in_group : a.group_channels - 1);
+    p.column = static_cast<int64_t>(p.tile) * 64 + p.lane;
+    p.t0 = p.chunk * a.chunk;
+    p.t1 = a.tokens - p.t0 < a.chunk ? a.tokens : p.t0 + a.chunk;
+    int32_t len = a.tokens;
+    if (a.lengths != nullptr) {
+        len = a.lengths[p.batch];
+        len = len < 0 ? 0 : len > a.tokens ? a.tokens : len;
+    }
+    p.te = len < p.t0 ? p.t0 : len > p.t1 ? p.t1 : len;
+    return p;
+}
+
+// One token's row of S values of B or C, read through the scalar cache (a uniform address in
+// memory that no kernel here writes): 16-bit pairs or FP32, 4-byte aligned.
+template <typename T, int S>
+struct SSRow {
+    uint32_t w[S * sizeof(T) / 4];
+    __device__ __forceinline__ void load(const void* base, int64_t elements) {
+        typedef const __attribute__((address_space(4))) uint32_t* cptr;
+        cptr p = (cptr)(reinterpret_cast<uintptr_t>(base) + elements * static_cast<int64_t>(sizeof(T)));
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(S * sizeof(T) / 4); ++i) w[i] = p[i];
+    }
+    __device__ __forceinline__ float operator[](int n) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[n]);
+        else return __uint_as_float((n & 1) ? (w[n / 2] & 0xffff0000u) : (w[n / 2] << 16));
+    }
+};
+
+// softplus(v) = max(v, 0) + log1p(exp(-|v|)).  log1p(e) = 2 artanh(s) with s = e / (2 + e) <=
+// 1/3, artanh(s) / s a polynomial in s^2 (least squares over [0, 1/9], 4e-9), so small steps
+// keep their relative accuracy (3e-7), which log2(1 + e) would lose.
+__device__ __forceinline__ float ss_softplus(float v) {
+    const float e = __builtin_amdgcn_exp2f(-SS_LOG2E * fabsf(v));
+    const float s = e * __builtin_amdgcn_rcpf(2.f + e);
+    const float w = s * s;
+    float p = 0.14087328f;
+    p = fmaf(p, w, 0.13980709f);
+    p = fmaf(p, w, 0.20012426f);
+    p = fmaf(p, w, 0.33333158f);
+    p = fmaf(p, w, 1.f);
+    return fmaf(s + s, p, fmaxf(v, 0.f));
+}
+
+inline int64_t ss_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Argument checks and the geometry common to forward and backward.
+int ss_fill(SSArgs& a, int32_t io_dtype, int32_t bc_dtype, int64_t B, int64_t N, int64_t C, int32_t groups,
+            int32_t states);
+
+// States (forward) or adjoints (backward) at the chunk boundaries from the chunks' own ones:
+// slots [B, chunks - 1, S, padded C] in place, one chunk after the other.
+int ss_join(const SSArgs& a, int64_t B, int32_t states, bool backward, const float* edge, hipStream_t stream);
+
+}  // namespace vh

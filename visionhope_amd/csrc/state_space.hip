@@ -1,0 +1,445 @@
+// Selective state space scan: forward of a prompt and the single-token step.
+//
+//   dt = softplus(dt_raw + dt_bias)                       per token and channel
+//   h[n] = exp(dt A[n]) h[n] + dt x B[n]                  S states a channel, FP32
+//   y = (sum_n C[n] h[n] + D x) silu(gate)
+//
+// A line of tokens is serial, so long lines are cut into chunks that run side by side: one
+// pass gives every chunk's state from a zero start and its sum of dt (the chunk's decay is
+// exp(A sum dt)), a join carries the states over the chunk boundaries, and the pass that
+// computes y starts from them.  With enough sequences and channels the line stays whole and
+// the first pass falls away.
+#include "state_space.h"
+
+namespace vh {
+namespace {
+
+constexpr int UNROLL = 4;   // tokens loaded together, one group ahead of the arithmetic
+
+// OUT: the output pass; otherwise the pass for the chunks' own states.
+template <typename T, typename BCT, int S, bool OUT>
+__global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
+    const SSPlace p = ss_place(a);
+    const int64_t cp = static_cast<int64_t>(a.tiles) * 64;
+    float A2[S], h[S];
+#pragma unroll
+    for (int n = 0; n < S; ++n) A2[n] = a.A[static_cast<int64_t>(p.channel) * S + n] * SS_LOG2E;
+    const float bias = a.dt_bias != nullptr ? a.dt_bias[p.channel] : 0.f;
+    const float D = OUT && a.D != nullptr ? a.D[p.channel] : 0.f;
+    if (OUT && p.chunk > 0) {
+        const float* from = a.slots + (static_cast<int64_t>(p.batch) * (a.chunks - 1) + p.chunk - 1) * S * cp + p.column;
+#pragma unroll
+        for (int n = 0; n < S; ++n) h[n] = from[n * cp];
+    } else if (OUT && a.state != nullptr) {
+        const float* from = a.state + (static_cast<int64_t>(p.batch) * a.channels + p.channel) * S;
+#pragma unroll
+        for (int n = 0; n < S; ++n) h[n] = p.live ? from[n] : 0.f;
+    } else {
+#pragma unroll
+        for (int n = 0; n < S; ++n) h[n] = 0.f;
+    }
+    const T* x = static_cast<const T*>(a.x.data) + p.batch * a.x.bs + p.t0 * a.x.ts;
+    const T* dt = static_cast<const T*>(a.dt.data) + p.batch * a.dt.bs + p.t0 * a.dt.ts;
+    const T* gate = OUT && a.gate.data != nullptr
+        ? static_cast<const T*>(a.gate.data) + p.batch * a.gate.bs + p.t0 * a.gate.ts : nullptr;
+    const int64_t bc0 = static_cast<int64_t>(p.group) * S;
+    int64_t brow = p.batch * a.b.bs + p.t0 * a.b.ts + bc0, crow = p.batch * a.c.bs + p.t0 * a.c.ts + bc0;
+    T* y = OUT ? static_cast<T*>(a.y) + (static_cast<int64_t>(p.batch) * a.tokens + p.t0) * a.channels : nullptr;
+    const int32_t count = p.te - p.t0;
+    const int32_t block = ss_block_tokens(S);
+    float total = 0.f;
+
+    T xr[UNROLL], dr[UNROLL], gr[UNROLL], xn[UNROLL], dn[UNROLL], gn[UNROLL];
+    auto fetch = [&](int32_t t) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int32_t at = t + u < count ? t + u : count - 1;   // a token of the sequence
+            xn[u] = x[at * a.x.ts + p.channel];
+            dn[u] = dt[at * a.dt.ts + p.channel];
+            if (OUT && gate != nullptr) gn[u] = gate[at * a.gate.ts + p.channel];
+        }
+    };
+    if (count > 0) fetch(0);
+    for (int32_t t = 0; t < count; t += UNROLL) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) { xr[u] = xn[u]; dr[u] = dn[u]; gr[u] = gn[u]; }
+        if (t + UNROLL < count) fetch(t + UNROLL);
+        if (OUT && a.kept != nullptr && t % block == 0) {
+            float* to = a.kept + (static_cast<int64_t>(p.batch) * a.blocks + (p.t0 + t) / block) * S * cp + p.column;
+#pragma unroll
+            for (int n = 0; n < S; ++n) to[n * cp] = h[n];
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            if (t + u >= count) break;
+            SSRow<BCT, S> b, c;
+            b.load(a.b.data, brow);
+            if (OUT) c.load(a.c.data, crow);
+            float step = to_f32(dr[u]) + bias;
+            if (a.softplus) step = ss_softplus(step);
+            const float xv = p.live ? to_f32(xr[u]) : 0.f;
+            const float dtx = step * xv;
+            float acc = D * xv;
+            if (!OUT) total += step;
+#pragma unroll
+            for (int n = 0; n < S; ++n) {
+                h[n] = fmaf(dtx, b[n], h[n] * __builtin_amdgcn_exp2f(step * A2[n]));
+                if (OUT) acc = fmaf(c[n], h[n], acc);
+            }
+            if (OUT) {
+                if (gate != nullptr) {
+                    const float z = to_f32(gr[u]);
+                    acc *= z * sigmoid_fast(z);
+                }
+                if (p.live) y[static_cast<int64_t>(t + u) * a.channels + p.channel] = from_f32<T>(acc);
+            }
+            brow += a.b.ts;
+            crow += a.c.ts;
+        }
+    }
+    if (OUT) {
+        for (int32_t t = count; t < p.t1 - p.t0; ++t)   // behind the sequence's end
+            if (p.live) y[static_cast<int64_t>(t) * a.channels + p.channel] = from_f32<T>(0.f);
+        if (a.new_state != nullptr && p.chunk == a.chunks - 1 && p.live) {
+            float* to = a.new_state + (static_cast<int64_t>(p.batch) * a.channels + p.channel) * S;
+#pragma unroll
+            for (int n = 0; n < S; n += 4)
+                *reinterpret_cast<float4*>(to + n) = make_float4(h[n], h[n + 1], h[n + 2], h[n + 3]);
+        }
+    } else {
+        float* to = a.slots + (static_cast<int64_t>(p.batch) * (a.chunks - 1) + p.chunk) * S * cp + p.column;
+#pragma unroll
+        for (int n = 0; n < S; ++n) to[n * cp] = h[n];
+        a.sums[(static_cast<int64_t>(p.batch) * a.chunks + p.chunk) * cp + p.column] = total;
+    }
+}
+
+// Carries states over chunk boundaries.  Forward: slots[k] holds the state that chunk k adds
+// from a zero start and becomes the state at the start of chunk k + 1; chunk k's decay is
+// exp(A sums[k]).  Backward: slots[k] holds the adjoint that chunk k + 1 hands to chunk k from
+// a zero adjoint behind it and becomes the whole one; the order is reversed and the decay is
+// that of chunk k + 1.  A workgroup takes one state of 64 channels, its waves ranges of the
+// chunks: each folds its range, the ranges' results go through LDS, and each walks its range
+// again from the value before it.
+__global__ void state_space_join_kernel(float* slots, const float* sums, const float* A, const float* edge,
+                                        int32_t S, int32_t channels, int32_t group_channels, int32_t group_tiles,
+                                        int32_t tiles, int32_t slots_n, int32_t backward) {
+    __shared__ float fold_h[16][64], fold_p[16][64];
+    const int32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int32_t tile = blockIdx.x % tiles, n = (blockIdx.x / tiles) % S;
+    const int64_t batch = blockIdx.x / (tiles * S);
+    const int32_t group = tile / group_tiles, in_group = (tile - group * group_tiles) * 64 + lane;
+    const bool live = in_group < group_channels;
+    const int32_t channel = group * group_channels + (live ? in_group : group_channels - 1);
+    const int64_t cp = static_cast<int64_t>(tiles) * 64, column = static_cast<int64_t>(tile) * 64 + lane;
+    const float A2 = A[static_cast<int64_t>(channel) * S + n] * SS_LOG2E;
+    float* slot = slots + (batch * slots_n * S + n) * cp + column;
+    const float* sum = sums + batch * (slots_n + 1) * cp + column;
+    const int32_t per = (slots_n + waves - 1) / waves;
+    const int32_t i0 = wave * per, i1 = i0 + per < slots_n ? i0 + per : slots_n;
+    // step i of the walk touches this slot, with the decay of this chunk
+    auto slot_of = [&](int32_t i) { return backward ? slots_n - 1 - i : i; };
+    auto chunk_of = [&](int32_t i) { return backward ? slots_n - i : i; };
+    // exp(A sum) h, and nothing from an empty state even where the decay (A > 0) overflows
+    auto decayed = [&](float p, float h) { return h == 0.f ? 0.f : h * __builtin_amdgcn_exp2f(A2 * p); };
+    float h = 0.f, ps = 0.f;
+    if (waves > 1) {
+#pragma unroll 8
+        for (int32_t i = i0; i < i1; ++i) {
+            const float p = sum[chunk_of(i) * cp], v = slot[static_cast<int64_t>(slot_of(i)) * S * cp];
+            h = decayed(p, h) + v;
+            ps += p;
+        }
+        fold_h[wave][lane] = h;
+        fold_p[wave][lane] = ps;
+        __syncthreads();
+    }
+    h = edge != nullptr && live ? edge[(batch * channels + channel) * S + n] : 0.f;
+    for (int32_t w = 0; w < wave; ++w) h = decayed(fold_p[w][lane], h) + fold_h[w][lane];
+#pragma unroll 8
+    for (int32_t i = i0; i < i1; ++i) {
+        float* at = slot + static_cast<int64_t>(slot_of(i)) * S * cp;
+        h = decayed(sum[chunk_of(i) * cp], h) + *at;
+        *at = h;
+    }
+}
+
+// One token of every sequence.  Four states a lane; the lanes of a channel stand side by side,
+// so the states are read and written in whole rows of 16 bytes a lane (element by element
+// where the state count or an address does not allow that).  Bound by the states' bytes (FP32,
+// read and written) once the batch is large, by the launch before.
+struct StepArgs {
+    const void *x, *dt, *gate, *b, *c;
+    int64_t x_bs, dt_bs, gate_bs, b_bs, c_bs;
+    const float *A, *D, *dt_bias, *state;
+    float* new_state;
+    void* y;
+    int64_t total;   // sequences x channels
+    int32_t softplus, channels, group_channels, states, wide;
+};
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void state_space_step_kernel(const StepArgs a) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t row = i / LANES;    // sequence and channel
+    if (row >= a.total) return;       // whole channels: the lanes of one stay together
+    const int32_t part = static_cast<int32_t>(i % LANES) * 4;
+    const int64_t batch = row / a.channels;
+    const int32_t channel = static_cast<int32_t>(row - batch * a.channels);
+    const int32_t group = channel / a.group_channels;
+    const float* state = a.state + row * a.states + part;
+    const float* rates = a.A + static_cast<int64_t>(channel) * a.states + part;
+    const T* b = static_cast<const T*>(a.b) + batch * a.b_bs + static_cast<int64_t>(group) * a.states + part;
+    const T* c = static_cast<const T*>(a.c) + batch * a.c_bs + static_cast<int64_t>(group) * a.states + part;
+    float h[4], A[4], bv[4], cv[4];
+    if (a.wide) {
+        const float4 h4 = *reinterpret_cast<const float4*>(state), A4 = *reinterpret_cast<const float4*>(rates);
+        h[0] = h4.x; h[1] = h4.y; h[2] = h4.z; h[3] = h4.w;
+        A[0] = A4.x; A[1] = A4.y; A[2] = A4.z; A[3] = A4.w;
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const bool in = part + n < a.states;
+        bv[n] = in ? to_f32(b[n]) : 0.f;
+        cv[n] = in ? to_f32(c[n]) : 0.f;
+        if (!a.wide) {
+            h[n] = in ? state[n] : 0.f;
+            A[n] = in ? rates[n] : 0.f;
+        }
+    }
+    const float xv = to_f32(static_cast<const T*>(a.x)[batch * a.x_bs + channel]);
+    float step = to_f32(static_cast<const T*>(a.dt)[batch * a.dt_bs + channel]);
+    if (a.dt_bias != nullptr) step += a.dt_bias[channel];
+    if (a.softplus) step = ss_softplus(step);
+    const float dtx = step * xv;
+    float acc = 0.f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        h[n] = fmaf(dtx, bv[n], h[n] * __builtin_amdgcn_exp2f(step * (A[n] * SS_LOG2E)));
+        acc = fmaf(cv[n], h[n], acc);
+    }
+    float* next = a.new_state + row * a.states + part;
+    if (a.wide) {
+        *reinterpret_cast<float4*>(next) = make_float4(h[0], h[1], h[2], h[3]);
+    } else {
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            if (part + n < a.states) next[n] = h[n];
+    }
+    acc = ln_lane_sum(acc, LANES == 1 ? 0 : LANES == 2 ? 1 : LANES == 4 ? 2 : 3);
+    if (part == 0) {
+        if (a.D != nullptr) acc = fmaf(a.D[channel], xv, acc);
+        if (a.gate != nullptr) {
+            const float z = to_f32(static_cast<const T*>(a.gate)[batch * a.gate_bs + channel]);
+            acc *= z * sigmoid_fast(z);
+        }
+        static_cast<T*>(a.y)[row] = from_f32<T>(acc);
+    }
+}
+
+// Waves that a chunked pass aims at: four a SIMD (1024 SIMDs), and the fewest tokens a chunk
+// is worth cutting to.
+constexpr int64_t TARGET_WAVES = 4096;
+constexpr int64_t MIN_CHUNK = 32;
+
+int64_t forward_chunk(int64_t B, int64_t N, int64_t tiles) {
+    int64_t chunks = TARGET_WAVES / (B * tiles);
+    if (chunks > ss_ceil(N, MIN_CHUNK)) chunks = ss_ceil(N, MIN_CHUNK);
+    if (chunks < 2) return ss_ceil(N, MIN_CHUNK) * MIN_CHUNK;
+    // whole blocks of every state count (8, 16 or 32 tokens)
+    return ss_ceil(ss_ceil(N, chunks), MIN_CHUNK) * MIN_CHUNK;
+}
+
+template <typename T, typename BCT, int S>
+int launch_forward(SSArgs& a, int64_t B, hipStream_t s) {
+    if (a.chunks > 1) {
+        a.first_chunk = 0;
+        a.launch_chunks = a.chunks - 1;
+        state_space_chunk_kernel<T, BCT, S, false>
+            <<<static_cast<uint32_t>(B * a.launch_chunks * a.tiles), 64, 0, s>>>(a);
+        if (int rc = check_launch("state_space chunk states")) return rc;
+        if (int rc = ss_join(a, B, S, false, a.state, s)) return rc;
+    }
+    a.first_chunk = 0;
+    a.launch_chunks = a.chunks;
+    state_space_chunk_kernel<T, BCT, S, true><<<static_cast<uint32_t>(B * a.chunks * a.tiles), 64, 0, s>>>(a);
+    return check_launch("state_space forward");
+}
+
+template <typename T>
+int launch_step(const StepArgs& a, hipStream_t s) {
+    const int lanes = a.states <= 4 ? 1 : a.states <= 8 ? 2 : a.states <= 16 ? 4 : 8;
+    const int64_t blocks = ss_ceil(a.total * lanes, 256);
+    VH_REQUIRE(blocks < (1ll << 24), VH_ERR_SHAPE, "state space step: too many sequences and channels for one launch");
+    const uint32_t grid = static_cast<uint32_t>(blocks);
+    if (lanes == 1) state_space_step_kernel<T, 1><<<grid, 256, 0, s>>>(a);
+    else if (lanes == 2) state_space_step_kernel<T, 2><<<grid, 256, 0, s>>>(a);
+    else if (lanes == 4) state_space_step_kernel<T, 4><<<grid, 256, 0, s>>>(a);
+    else state_space_step_kernel<T, 8><<<grid, 256, 0, s>>>(a);
+    return check_launch("state_space step");
+}
+
+int dispatch_forward(int32_t io, int32_t bc, int32_t S, SSArgs& a, int64_t B, hipStream_t s) {
+    auto by_states = [&](auto t, auto u) -> int {
+        using T = decltype(t);
+        using U = decltype(u);
+        if (S == 8) return launch_forward<T, U, 8>(a, B, s);
+        if (S == 16) return launch_forward<T, U, 16>(a, B, s);
+        return launch_forward<T, U, 32>(a, B, s);
+    };
+    if (io == VH_DTYPE_F32) return by_states(float{}, float{});
+    if (io == VH_DTYPE_F16) return by_states(f16_t{}, float{});
+    if (bc == VH_DTYPE_F32) return by_states(bf16_t{}, float{});
+    return by_states(bf16_t{}, bf16_t{});
+}
+int check_sizes(int64_t B, int64_t N, int64_t C, int32_t groups) {
+    VH_REQUIRE(B > 0 && N > 0 && C > 0 && groups > 0 && C % groups == 0, VH_ERR_SHAPE,
+               "state space scan needs nonempty sizes and channels divisible by groups, got B=%lld N=%lld C=%lld groups=%d",
+               (long long)B, (long long)N, (long long)C, groups);
+    VH_REQUIRE(N < (1ll << 30) && C < (1ll << 24) && B < (1ll << 24), VH_ERR_SHAPE,
+               "state space scan: sizes out of range (B=%lld N=%lld C=%lld)", (long long)B, (long long)N, (long long)C);
+    return VH_OK;
+}
+
+int check_bc(const SSTokens& t, int32_t bc_dtype, const char* name) {
+    // the scalar unit reads whole words
+    const int64_t e = dtype_bytes(bc_dtype);
+    VH_REQUIRE(t.data != nullptr && reinterpret_cast<uintptr_t>(t.data) % 4 == 0 && t.bs * e % 4 == 0 &&
+                   t.ts * e % 4 == 0, VH_ERR_ARG, "%s must be given, its rows 4-byte aligned", name);
+    return VH_OK;
+}
+
+}  // namespace
+
+int ss_fill(SSArgs& a, int32_t io_dtype, int32_t bc_dtype, int64_t B, int64_t N, int64_t C, int32_t groups,
+            int32_t states) {
+    VH_REQUIRE(valid_dtype(io_dtype), VH_ERR_DTYPE, "unsupported io_dtype %d", io_dtype);
+    VH_REQUIRE(bc_dtype == VH_DTYPE_F32 || (bc_dtype == VH_DTYPE_BF16 && io_dtype == VH_DTYPE_BF16), VH_ERR_DTYPE,
+               "B and C must be fp32, or bf16 with bf16 activations, got dtype %d", bc_dtype);
+    if (int rc = check_sizes(B, N, C, groups)) return rc;
+    VH_REQUIRE(states == 8 || states == 16 || states == 32, VH_ERR_SHAPE, "states must be 8, 16 or 32, got %d", states);
+    VH_REQUIRE(a.A != nullptr && reinterpret_cast<uintptr_t>(a.A) % 16 == 0, VH_ERR_ARG,
+               "A must be given, 16-byte aligned");
+    VH_REQUIRE(a.x.data != nullptr && a.dt.data != nullptr, VH_ERR_ARG, "x and dt must not be null");
+    VH_REQUIRE(reinterpret_cast<uintptr_t>(a.state) % 16 == 0 && reinterpret_cast<uintptr_t>(a.new_state) % 16 == 0,
+               VH_ERR_ARG, "states must be 16-byte aligned");
+    if (int rc = check_bc(a.b, bc_dtype, "B")) return rc;
+    if (int rc = check_bc(a.c, bc_dtype, "C")) return rc;
+    a.batches = static_cast<int32_t>(B);
+    a.tokens = static_cast<int32_t>(N);
+    a.channels = static_cast<int32_t>(C);
+    a.group_channels = static_cast<int32_t>(C / groups);
+    a.group_tiles = static_cast<int32_t>(ss_ceil(a.group_channels, 64));
+    a.tiles = a.group_tiles * groups;
+    a.blocks = static_cast<int32_t>(ss_ceil(N, ss_block_tokens(states)));
+    // a launch has one wave for each tile of a chunk (8 tokens at least, and no more chunks than
+    // the aimed-at waves where there are that many sequences), and one for each state
+    VH_REQUIRE(B * a.tiles < (1ll << 24), VH_ERR_SHAPE,
+               "state space scan: too many sequences and channels for one launch");
+    return VH_OK;
+}
+
+int ss_join(const SSArgs& a, int64_t B, int32_t states, bool backward, const float* edge, hipStream_t stream) {
+    const int32_t slots = a.chunks - 1;
+    const int32_t waves = slots >= 64 ? 16 : slots >= 16 ? 4 : 1;
+    state_space_join_kernel<<<static_cast<uint32_t>(B * states * a.tiles), 64 * waves, 0, stream>>>(
+        a.slots, a.sums, a.A, edge, states, a.channels, a.group_channels, a.group_tiles, a.tiles, slots, backward);
+    return check_launch("state_space join");
+}
+
+}  // namespace vh
+
+extern "C" {
+
+size_t vh_state_space_workspace_bytes(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
+    using namespace vh;
+    if (B <= 0 || N <= 0 || C <= 0 || groups <= 0 || C % groups || states <= 0) return 0;
+    const int64_t tiles = ss_ceil(C / groups, 64) * groups;
+    const int64_t chunks = ss_ceil(N, forward_chunk(B, N, tiles));
+    if (chunks < 2) return 0;
+    return static_cast<size_t>(B) * tiles * 64 * ((chunks - 1) * states + chunks) * sizeof(float);
+}
+
+size_t vh_state_space_kept_bytes(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
+    using namespace vh;
+    if (B <= 0 || N <= 0 || C <= 0 || groups <= 0 || C % groups || states <= 0) return 0;
+    return static_cast<size_t>(B) * ss_ceil(N, ss_block_tokens(states)) * states * ss_ceil(C / groups, 64) * groups * 64 *
+           sizeof(float);
+}
+
+int vh_state_space_forward(
+    const void* x, int64_t x_batch, int64_t x_token, const void* dt, int64_t dt_batch, int64_t dt_token,
+    const void* gate, int64_t gate_batch, int64_t gate_token, int32_t io_dtype,
+    const void* b, int64_t b_batch, int64_t b_token, const void* c, int64_t c_batch, int64_t c_token, int32_t bc_dtype,
+    const float* A, const float* D, const float* dt_bias, int32_t softplus, const float* state,
+    const int32_t* lengths, void* y, float* new_state, float* kept, int64_t B, int64_t N, int64_t C, int32_t groups,
+    int32_t states, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace vh;
+    SSArgs a{};
+    a.x = {x, x_batch, x_token};
+    a.dt = {dt, dt_batch, dt_token};
+    a.gate = {gate, gate_batch, gate_token};
+    a.b = {b, b_batch, b_token};
+    a.c = {c, c_batch, c_token};
+    a.A = A;
+    a.D = D;
+    a.dt_bias = dt_bias;
+    a.softplus = softplus;
+    a.state = state;
+    a.lengths = lengths;
+    a.y = y;
+    a.new_state = new_state;
+    a.kept = kept;
+    if (int rc = ss_fill(a, io_dtype, bc_dtype, B, N, C, groups, states)) return rc;
+    VH_REQUIRE(y != nullptr, VH_ERR_ARG, "y must not be null");
+    a.chunk = static_cast<int32_t>(forward_chunk(B, N, a.tiles));
+    a.chunks = static_cast<int32_t>(ss_ceil(N, a.chunk));
+    const size_t need = vh_state_space_workspace_bytes(B, N, C, groups, states);
+    VH_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), VH_ERR_WORKSPACE,
+               "state space scan needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
+    a.slots = static_cast<float*>(workspace);
+    a.sums = a.slots + static_cast<int64_t>(B) * (a.chunks - 1) * states * a.tiles * 64;
+    return dispatch_forward(io_dtype, bc_dtype, states, a, B, static_cast<hipStream_t>(stream));
+}
+
+int vh_state_space_step(
+    const void* x, int64_t x_batch, const void* dt, int64_t dt_batch, const void* gate, int64_t gate_batch,
+    int32_t io_dtype, const void* b, int64_t b_batch, const void* c, int64_t c_batch, const float* A, const float* D,
+    const float* dt_bias, int32_t softplus, const float* state, float* new_state, void* y, int64_t B, int64_t C,
+    int32_t groups, int32_t states, void* stream) {
+    using namespace vh;
+    VH_REQUIRE(valid_dtype(io_dtype), VH_ERR_DTYPE, "unsupported io_dtype %d", io_dtype);
+    if (int rc = check_sizes(B, 1, C, groups)) return rc;
+    VH_REQUIRE(states >= 1 && states <= 32, VH_ERR_SHAPE, "states must be 1 to 32, got %d", states);
+    VH_REQUIRE(x != nullptr && dt != nullptr && b != nullptr && c != nullptr && A != nullptr && state != nullptr &&
+                   new_state != nullptr && y != nullptr, VH_ERR_ARG,
+               "x, dt, B, C, A, state, new_state and y must not be null");
+    StepArgs a{};
+    a.x = x;
+    a.x_bs = x_batch;
+    a.dt = dt;
+    a.dt_bs = dt_batch;
+    a.gate = gate;
+    a.gate_bs = gate_batch;
+    a.b = b;
+    a.b_bs = b_batch;
+    a.c = c;
+    a.c_bs = c_batch;
+    a.A = A;
+    a.D = D;
+    a.dt_bias = dt_bias;
+    a.state = state;
+    a.new_state = new_state;
+    a.y = y;
+    a.total = B * C;
+    a.softplus = softplus;
+    a.channels = static_cast<int32_t>(C);
+    a.group_channels = static_cast<int32_t>(C / groups);
+    a.states = states;
+    a.wide = states % 4 == 0 && reinterpret_cast<uintptr_t>(A) % 16 == 0 && reinterpret_cast<uintptr_t>(state) % 16 == 0 &&
+             reinterpret_cast<uintptr_t>(new_state) % 16 == 0;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (io_dtype == VH_DTYPE_F32) return launch_step<float>(a, s);
+    return io_dtype == VH_DTYPE_BF16 ? launch_step<bf16_t>(a, s) : launch_step<f16_t>(a, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,127 @@
+"""LayerNorm of token rows with an optional SiLU gate (native, ``csrc/row_norm.hip``).
+
+    y = ((x - mean) / sqrt(var + eps) * weight + bias) * silu(gate)
+
+over the last dimension (biased variance).  Statistics and sums are FP32; y and the
+gradients of x and gate are rounded once to x's dtype, those of weight and bias are summed in
+FP32 in a fixed order.  ``utils/layer_norm_cuda.py`` is the LayerNorm of ``[B, C, H, W]`` maps.
+"""
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import hip
+from .cuda import on_tensor_device
+from .token_lines import IO_DTYPES, check_like, check_param, fp32_param
+
+MAX_CHANNELS = 8192
+
+
+def _rows(t):
+    """``t`` as rows a fixed number of elements apart: ``(tensor, stride)``.  Leading dimensions
+    that do not fold into one are copied."""
+    channels = t.shape[-1]
+    if t.ndim == 1:
+        t = t[None]
+    if t.stride(-1) != 1 and channels > 1:
+        t = t.contiguous()
+    # the stride of the innermost leading dimension of more than one row, which the others must
+    # continue
+    stride, expected = None, None
+    for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if stride is None:
+            stride, expected = step, step * size
+        elif step != expected:
+            return t.contiguous(), channels
+        else:
+            expected = step * size
+    return t, channels if stride is None else stride
+
+
+def _forward(x, weight, bias, gate, eps, keep):
+    channels = x.shape[-1]
+    rows = x.numel() // channels
+    x, x_row = _rows(x)
+    gate_row = 0
+    if gate is not None:
+        gate, gate_row = _rows(gate)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    mean = rstd = None
+    if keep:
+        mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32).unbind(0)
+    hip.check(hip.load_library().vh_gated_layernorm_forward(
+        hip.ptr(x), x_row, hip.ptr(gate), gate_row, hip.dtype_code(x.dtype), hip.ptr(weight), hip.ptr(bias),
+        hip.ptr(y), hip.ptr(mean), hip.ptr(rstd), rows, channels, float(eps), hip.stream_of(x)),
+        "vh_gated_layernorm_forward")
+    return y, mean, rstd
+
+
+class _GatedLayerNormFunction(Function):
+    @staticmethod
+    @on_tensor_device
+    def forward(ctx, x, weight, bias, gate, eps):
+        weight32, bias32 = fp32_param(weight), fp32_param(bias)
+        y, mean, rstd = _forward(x, weight32, bias32, gate, eps, True)
+        ctx.save_for_backward(x, weight32, bias32, gate, mean, rstd)
+        ctx.param_dtypes = (weight.dtype, bias.dtype)
+        return y.view(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return _GatedLayerNormFunction._gradients(*ctx.saved_tensors, ctx, dy)
+
+    @staticmethod
+    @on_tensor_device
+    def _gradients(x, weight, bias, gate, mean, rstd, ctx, dy):
+        shape, channels = x.shape, x.shape[-1]
+        rows = x.numel() // channels
+        need = ctx.needs_input_grad
+        x, x_row = _rows(x)
+        dy, dy_row = _rows(dy.to(x.dtype))
+        gate_row, dgate = 0, None
+        if gate is not None:
+            gate, gate_row = _rows(gate)
+            dgate = torch.empty(shape, device=x.device, dtype=x.dtype)
+        dx = torch.empty(shape, device=x.device, dtype=x.dtype)
+        dweight = torch.empty(channels, device=x.device, dtype=torch.float32) if need[1] else None
+        dbias = torch.empty(channels, device=x.device, dtype=torch.float32) if need[2] else None
+        lib = hip.load_library()
+        ws = hip.workspace(lib.vh_gated_layernorm_backward_workspace_bytes(rows, channels), x.device)
+        hip.check(lib.vh_gated_layernorm_backward(
+            hip.ptr(dy), dy_row, hip.ptr(x), x_row, hip.ptr(gate), gate_row, hip.dtype_code(x.dtype), hip.ptr(weight),
+            hip.ptr(bias), hip.ptr(mean), hip.ptr(rstd), hip.ptr(dx), hip.ptr(dgate), hip.ptr(dweight), hip.ptr(dbias),
+            rows, channels, hip.ptr(ws), ws.numel() * 4, hip.stream_of(x)), "vh_gated_layernorm_backward")
+        return (dx, dweight.to(ctx.param_dtypes[0]) if need[1] else None,
+                dbias.to(ctx.param_dtypes[1]) if need[2] else None, dgate, None)
+
+
+def visionhope_gated_layernorm(x, weight, bias, eps=1e-6, *, gate=None):
+    """LayerNorm of ``x`` ``[..., C]`` over its last dimension (C of up to 8192), times
+    ``silu(gate)`` with a gate of x's shape and dtype (module docstring).  ``weight`` and ``bias``
+    ``[C]``.  ``x`` and ``gate`` may be slices of wider tensors; y is dense, in x's dtype."""
+    name = "visionhope_gated_layernorm"
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError(f"{name} expects CUDA tensors")
+    if x.dtype not in IO_DTYPES:
+        raise TypeError(f"{name} supports FP16, BF16 and FP32 tensors, got {x.dtype}")
+    if x.ndim < 1 or x.numel() == 0:
+        raise ValueError(f"{name} expects nonempty rows, got shape {tuple(x.shape)}")
+    channels = x.shape[-1]
+    if channels > MAX_CHANNELS:
+        raise ValueError(f"{name} supports at most {MAX_CHANNELS} channels, got {channels}")
+    check_param(name, "weight", weight, (channels,), x.device)
+    check_param(name, "bias", bias, (channels,), x.device)
+    if gate is not None:
+        check_like(name, "gate", gate, x.shape, x.dtype, x.device)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, gate)):
+        return _GatedLayerNormFunction.apply(x, weight, bias, gate, float(eps))
+    return _no_grad_forward(x, weight, bias, gate, eps)
+
+
+@on_tensor_device
+def _no_grad_forward(x, weight, bias, gate, eps):
+    return _forward(x, fp32_param(weight), fp32_param(bias), gate, eps, False)[0].view(x.shape)

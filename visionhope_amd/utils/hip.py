@@ -42,6 +42,10 @@ EXPORTED_SYMBOLS = (
     "vh_grn_backward_workspace_bytes", "vh_grn_backward", "vh_layernorm2d_backward_workspace_bytes",
     "vh_layernorm2d_backward", "vh_qnorm_backward", "vh_residual_add_backward_workspace_bytes",
     "vh_residual_add_backward",
+    "vh_causal_conv_forward", "vh_causal_conv_backward_workspace_bytes", "vh_causal_conv_backward",
+    "vh_causal_conv_step", "vh_state_space_workspace_bytes", "vh_state_space_kept_bytes", "vh_state_space_forward",
+    "vh_state_space_backward_workspace_bytes", "vh_state_space_backward", "vh_state_space_step",
+    "vh_gated_layernorm_forward", "vh_gated_layernorm_backward_workspace_bytes", "vh_gated_layernorm_backward",
 )
 
 
@@ -151,6 +155,32 @@ _SIGNATURES = {
     "vh_qnorm_forward": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp]),
     "vh_residual_add_forward": (ctypes.c_int, [
         _vp, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "vh_causal_conv_forward": (ctypes.c_int, [
+        _vp, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
+    "vh_causal_conv_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
+    "vh_causal_conv_backward": (ctypes.c_int, [
+        _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+        _i64, _i64, _i64, _i32, _vp, _sz, _vp]),
+    "vh_causal_conv_step": (ctypes.c_int, [
+        _vp, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "vh_state_space_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
+    "vh_state_space_kept_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
+    "vh_state_space_forward": (ctypes.c_int, [
+        _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i32,
+        _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _sz, _vp]),
+    "vh_state_space_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
+    "vh_state_space_backward": (ctypes.c_int, [
+        _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64,
+        _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+        _i64, _i64, _i64, _i32, _i32, _vp, _sz, _vp]),
+    "vh_state_space_step": (ctypes.c_int, [
+        _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _vp,
+        _i64, _i64, _i32, _i32, _vp]),
+    "vh_gated_layernorm_forward": (ctypes.c_int, [
+        _vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _vp]),
+    "vh_gated_layernorm_backward_workspace_bytes": (_sz, [_i64, _i64]),
+    "vh_gated_layernorm_backward": (ctypes.c_int, [
+        _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz, _vp]),
 }
 
 _LIB = None

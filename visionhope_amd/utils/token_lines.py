@@ -1,0 +1,68 @@
+"""Argument handling shared by the operators of token lines ``[B, N, C]``."""
+
+import torch
+
+IO_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def check_io(name, x, ndim):
+    """``x`` is a CUDA tensor of a supported type with ``ndim`` nonempty dimensions."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError(f"{name} expects CUDA tensors")
+    if x.dtype not in IO_DTYPES:
+        raise TypeError(f"{name} supports FP16, BF16 and FP32 tensors, got {x.dtype}")
+    if x.ndim != ndim or min(x.shape) <= 0:
+        raise ValueError(f"{name} expects a nonempty tensor of {ndim} dimensions, got shape {tuple(x.shape)}")
+
+
+def check_like(name, what, t, shape, dtype, device):
+    """``t`` has exactly this shape, dtype and device."""
+    if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape):
+        got = tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__
+        raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {got}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: {what} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name}: {what} must be on {device}, got {t.device}")
+
+
+def check_param(name, what, t, shape, device):
+    """A floating-point parameter of this shape on this device."""
+    if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape):
+        got = tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__
+        raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {got}")
+    if not t.is_floating_point():
+        raise TypeError(f"{name}: {what} must be floating point, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name}: {what} must be on {device}, got {t.device}")
+
+
+def line_lengths(name, lengths, batch, device):
+    """Sequence lengths as int32 ``[B]`` on the device, or None."""
+    if lengths is None:
+        return None
+    if not isinstance(lengths, torch.Tensor) or tuple(lengths.shape) != (batch,):
+        raise ValueError(f"{name}: lengths must be a tensor of shape ({batch},)")
+    if lengths.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name}: lengths must be int32 or int64, got {lengths.dtype}")
+    if lengths.device != device:
+        raise ValueError(f"{name}: lengths must be on {device}, got {lengths.device}")
+    if lengths.dtype == torch.int64:   # clamped first: the kernels clamp what int32 holds
+        lengths = lengths.clamp(0, 2**31 - 1).to(torch.int32)
+    return lengths.contiguous()
+
+
+def dense_channels(t):
+    """``t`` with its last dimension dense; the strides of the others are the kernels' arguments."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def fp32_param(t):
+    """A parameter as the kernels read it: FP32, dense, without autograd."""
+    return None if t is None else t.detach().float().contiguous()
+
+
+def refuse_gradients(name, *tensors):
+    """Single-token calls write states in place and record no graph."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} is for inference; call it under torch.no_grad() or on detached tensors")
