@@ -88,7 +88,7 @@ def test_refused_before_any_launch(lib, name, defaults, change, status, message)
 
 def test_workspace_sizes(lib):
     assert lib.vh_state_space_kept_bytes(2, 33, 70, 1, 16) == 2 * 3 * 16 * 128 * 4
-    assert lib.vh_state_space_kept_bytes(2, 33, 70, 2, 8) == 2 * 2 * 8 * 128 * 4
+    assert lib.vh_state_space_kept_bytes(2, 33, 70, 2, 8) == 2 * 3 * 8 * 128 * 4
     assert lib.vh_state_space_workspace_bytes(1, 1, 64, 1, 16) == 0          # one chunk
     assert lib.vh_state_space_workspace_bytes(0, 5, 64, 1, 16) == 0
     for name, args in (("vh_causal_conv_backward_workspace_bytes", (2, 10, 8, 4)),

@@ -13,8 +13,8 @@ namespace vh {
 
 constexpr float SS_LOG2E = 1.44269504088896341f;
 
-// Tokens between two states that a training forward keeps for the backward, by state count.
-constexpr int ss_block_tokens(int states) { return states <= 8 ? 32 : states <= 16 ? 16 : 8; }
+// Tokens between two states that a training forward keeps for the backward.
+constexpr int SS_BLOCK = 16;
 
 struct SSTokens {   // an activation [B, N, ...]: element strides of sequence and token
     const void* data;
@@ -32,8 +32,9 @@ struct SSArgs {
     float* sums;     // [B, chunks, padded C]: sum of dt over a chunk
     int32_t softplus;
     int32_t batches, tokens, channels, group_channels, group_tiles, tiles;   // tiles: of 64 channels, all groups
-    int32_t chunk, chunks, first_chunk, launch_chunks, blocks;
+    int32_t groups, chunk, chunks, first_chunk, launch_chunks, blocks;
     // backward
+    int32_t wide_tiles, fine_chunks, fine_per_chunk;
     void *dx, *ddt, *dgate;
     float* dstate;
     float* bc_partial;     // [tiles, B, N, 2 S]

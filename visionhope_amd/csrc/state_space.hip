@@ -46,7 +46,6 @@ __global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
     int64_t brow = p.batch * a.b.bs + p.t0 * a.b.ts + bc0, crow = p.batch * a.c.bs + p.t0 * a.c.ts + bc0;
     T* y = OUT ? static_cast<T*>(a.y) + (static_cast<int64_t>(p.batch) * a.tokens + p.t0) * a.channels : nullptr;
     const int32_t count = p.te - p.t0;
-    const int32_t block = ss_block_tokens(S);
     float total = 0.f;
 
     T xr[UNROLL], dr[UNROLL], gr[UNROLL], xn[UNROLL], dn[UNROLL], gn[UNROLL];
@@ -64,8 +63,8 @@ __global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) { xr[u] = xn[u]; dr[u] = dn[u]; gr[u] = gn[u]; }
         if (t + UNROLL < count) fetch(t + UNROLL);
-        if (OUT && a.kept != nullptr && t % block == 0) {
-            float* to = a.kept + (static_cast<int64_t>(p.batch) * a.blocks + (p.t0 + t) / block) * S * cp + p.column;
+        if (OUT && a.kept != nullptr && t % SS_BLOCK == 0) {
+            float* to = a.kept + (static_cast<int64_t>(p.batch) * a.blocks + (p.t0 + t) / SS_BLOCK) * S * cp + p.column;
 #pragma unroll
             for (int n = 0; n < S; ++n) to[n * cp] = h[n];
         }
@@ -324,13 +323,14 @@ int ss_fill(SSArgs& a, int32_t io_dtype, int32_t bc_dtype, int64_t B, int64_t N,
                VH_ERR_ARG, "states must be 16-byte aligned");
     if (int rc = check_bc(a.b, bc_dtype, "B")) return rc;
     if (int rc = check_bc(a.c, bc_dtype, "C")) return rc;
+    a.groups = groups;
     a.batches = static_cast<int32_t>(B);
     a.tokens = static_cast<int32_t>(N);
     a.channels = static_cast<int32_t>(C);
     a.group_channels = static_cast<int32_t>(C / groups);
     a.group_tiles = static_cast<int32_t>(ss_ceil(a.group_channels, 64));
     a.tiles = a.group_tiles * groups;
-    a.blocks = static_cast<int32_t>(ss_ceil(N, ss_block_tokens(states)));
+    a.blocks = static_cast<int32_t>(ss_ceil(N, SS_BLOCK));
     // a launch has one wave for each tile of a chunk (8 tokens at least, and no more chunks than
     // the aimed-at waves where there are that many sequences), and one for each state
     VH_REQUIRE(B * a.tiles < (1ll << 24), VH_ERR_SHAPE,
@@ -362,7 +362,7 @@ size_t vh_state_space_workspace_bytes(int64_t B, int64_t N, int64_t C, int32_t g
 size_t vh_state_space_kept_bytes(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
     using namespace vh;
     if (B <= 0 || N <= 0 || C <= 0 || groups <= 0 || C % groups || states <= 0) return 0;
-    return static_cast<size_t>(B) * ss_ceil(N, ss_block_tokens(states)) * states * ss_ceil(C / groups, 64) * groups * 64 *
+    return static_cast<size_t>(B) * ss_ceil(N, SS_BLOCK) * states * ss_ceil(C / groups, 64) * groups * 64 *
            sizeof(float);
 }
 

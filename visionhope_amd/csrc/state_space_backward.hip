@@ -78,210 +78,328 @@ __global__ __launch_bounds__(64) void state_space_adjoint_kernel(const SSArgs a)
     a.sums[(static_cast<int64_t>(p.batch) * a.chunks + p.chunk) * cp + p.column] = total;
 }
 
-// Sums over the 64 lanes of M values a lane: each stage exchanges one bit of the lane index
-// and halves the values, so lane l ends with value l * M / 64 (M = 16, 32 or 64).  The first
-// two bits go by the row swaps, the others by DPP within 16 lanes.
-template <int CTRL>
-__device__ __forceinline__ float fold_dpp(float lo, float hi, bool upper) {
-    const float keep = upper ? hi : lo, send = upper ? lo : hi;
-    return keep + ln_dpp<CTRL>(send);
+// Sum over lane bits 1 .. 5 above the LANES lanes of a channel, of 2 SPL values a lane: the row
+// swaps halve the values (lanes 32 .. 63 end with the second half, odd rows of 16 with the
+// second quarter), the bits inside a row are added up in every lane.
+template <int LANES, int SPL>
+__device__ __forceinline__ void channel_sums(float (&v)[2 * SPL]) {
+#pragma unroll
+    for (int i = 0; i < SPL; ++i) {
+        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + SPL]), false, false);
+        v[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < SPL / 2; ++i) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + SPL / 2]), false, false);
+        v[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < SPL / 2; ++i) {
+        v[i] += ln_dpp<0x128>(v[i]);                        // row_ror 8
+        v[i] += ln_dpp<0x124>(v[i]);                        // row_ror 4
+        if constexpr (LANES == 2) v[i] += ln_dpp<0x4E>(v[i]);   // lanes (2, 3, 0, 1)
+    }
 }
-template <int M>
-__device__ __forceinline__ float lane_fold(float (&v)[M]) {
-    const int32_t lane = threadIdx.x & 63;
-    static_assert(M == 16 || M == 32 || M == 64, "values a lane");
-#pragma unroll
-    for (int i = 0; i < M / 2; ++i) {
-        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + M / 2]), false, false);
-        v[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-    }
-#pragma unroll
-    for (int i = 0; i < M / 4; ++i) {
-        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + M / 4]), false, false);
-        v[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-    }
-#pragma unroll
-    for (int i = 0; i < M / 8; ++i) v[i] = fold_dpp<0x128>(v[i], v[i + M / 8], lane & 8);      // row_ror 8
-#pragma unroll
-    for (int i = 0; i < M / 16; ++i) v[i] = fold_dpp<0x141>(v[i], v[i + M / 16], lane & 4);    // i <-> 7 - i
-    if constexpr (M >= 32) {
-#pragma unroll
-        for (int i = 0; i < M / 32; ++i) v[i] = fold_dpp<0x4E>(v[i], v[i + M / 32], lane & 2); // i <-> i ^ 2
-    } else {
-        v[0] += ln_dpp<0x4E>(v[0]);
-    }
-    if constexpr (M >= 64) return fold_dpp<0xB1>(v[0], v[1], lane & 1);                       // i <-> i ^ 1
-    return v[0] + ln_dpp<0xB1>(v[0]);
+// Sum over the LANES lanes of a channel.
+template <int LANES>
+__device__ __forceinline__ float state_sum(float v) {
+    v += ln_dpp<0xB1>(v);
+    if constexpr (LANES == 4) v += ln_dpp<0x4E>(v);
+    return v;
 }
 
-template <typename T, typename BCT, int S>
-__global__ __launch_bounds__(64) void state_space_backward_kernel(const SSArgs a) {
-    constexpr int BLOCK = ss_block_tokens(S);
-    constexpr int SUB = 64 / S, SUBS = BLOCK / SUB;   // tokens whose decays and states stand in registers
-    static_assert(SUBS == 4, "a block is four sub-blocks");
-    __shared__ float starts[SUBS][S][64];             // states before each sub-block
-    const SSPlace p = ss_place(a);
-    const int32_t lane = p.lane;
+// An element `offset` bytes behind a uniform address.  The offset passes through a register the
+// compiler cannot see behind, or it would keep a 64-bit address a lane for every tensor in
+// vector registers over the whole walk.
+__device__ __forceinline__ uint32_t opaque(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T load_at(const T* base, uint32_t offset) {
+    return *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + offset);
+}
+template <typename T>
+__device__ __forceinline__ void store_at(void* base, int64_t element, uint32_t offset, float v) {
+    *reinterpret_cast<T*>(reinterpret_cast<char*>(static_cast<T*>(base) + element) + offset) = from_f32<T>(v);
+}
+
+// Waves a SIMD that the registers of the gradients' pass allow.
+constexpr int backward_waves(int states) { return states <= 8 ? 3 : states <= 16 ? 4 : 2; }
+
+// The gradients of one chunk.  LANES lanes share a channel, SPL states each, so the decays and
+// states of SUB tokens stand in registers with room for four waves a SIMD (a wave alone issues
+// a vector instruction only every 7 cycles, four together one every 4.6).  A workgroup takes
+// 256 / LANES channels through blocks of SS_BLOCK tokens:
+//   1. by token and channel: step, step x and dz of the block go to LDS, as do B and C;
+//   2. by channel and states: the states before each sub-block from the kept ones, then from
+//      the last sub-block the decays and states again and the adjoints; the sums over states
+//      go to LDS in place of 1., those over a wave's channels beside them;
+//   3. by token and channel: dx, ddt and dgate; and the sums of dB and dC over the waves.
+template <typename T, typename BCT, int LANES, int SPL>
+__global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_backward_kernel(const SSArgs a) {
+    constexpr int S = LANES * SPL, CHANNELS = 256 / LANES;
+    constexpr int SUB = 4, SUBS = SS_BLOCK / SUB;
+    constexpr int TOKENS = SS_BLOCK * CHANNELS / 256;   // of a thread in 1. and 3.
+    __shared__ float4 tok[SS_BLOCK][CHANNELS];
+    __shared__ float maps[SS_BLOCK][2 * S];             // C, then B
+    __shared__ float parts[4][SS_BLOCK][2 * S];
+
+    const uint32_t bid = xcd_remap_any(blockIdx.x, gridDim.x);
+    const uint32_t rest = bid / static_cast<uint32_t>(a.wide_tiles);
+    const int32_t tile = static_cast<int32_t>(bid - rest * a.wide_tiles);
+    const int32_t batch = static_cast<int32_t>(rest / static_cast<uint32_t>(a.chunks));
+    const int32_t chunk = static_cast<int32_t>(rest) - batch * a.chunks;
+    const int32_t tiles_of_group = a.wide_tiles / a.groups, group = tile / tiles_of_group;
+    const int32_t first = (tile - group * tiles_of_group) * CHANNELS;   // in the group
+    const int32_t t0 = chunk * a.chunk, t1 = a.tokens - t0 < a.chunk ? a.tokens : t0 + a.chunk;
+    int32_t te = a.tokens;
+    if (a.lengths != nullptr) te = a.lengths[batch];
+    te = te < t0 ? t0 : te > t1 ? t1 : te;
+    const int32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t cp = static_cast<int64_t>(a.tiles) * 64;
-    float A2[S], carry[S], dA[S];
+
+    // by channel and states
+    const int32_t part = tid & (LANES - 1), mine = tid / LANES;   // mine: of the workgroup's channels
+    const bool live = first + mine < a.group_channels;
+    const int32_t in_group = live ? first + mine : a.group_channels - 1;
+    const int32_t channel = group * a.group_channels + in_group;
+    const int64_t column = static_cast<int64_t>(group) * a.group_tiles * 64 + in_group;
+    float A2[SPL], carry[SPL], dA[SPL];
 #pragma unroll
-    for (int n = 0; n < S; ++n) {
-        A2[n] = a.A[static_cast<int64_t>(p.channel) * S + n] * SS_LOG2E;
-        dA[n] = 0.f;
+    for (int j = 0; j < SPL; ++j) {
+        A2[j] = a.A[static_cast<int64_t>(channel) * S + part * SPL + j] * SS_LOG2E;
+        dA[j] = 0.f;
     }
     // the adjoint behind the chunk, times the decay of the token behind it
-    if (p.chunk < a.chunks - 1) {
-        const float* from = a.slots + (static_cast<int64_t>(p.batch) * (a.chunks - 1) + p.chunk) * S * cp + p.column;
+    if (chunk < a.chunks - 1) {
+        const int64_t slot = static_cast<int64_t>(batch) * (a.fine_chunks - 1) + (chunk + 1) * a.fine_per_chunk - 1;
+        const float* from = a.slots + (slot * S + part * SPL) * cp + column;
 #pragma unroll
-        for (int n = 0; n < S; ++n) carry[n] = from[n * cp];
+        for (int j = 0; j < SPL; ++j) carry[j] = live ? from[j * cp] : 0.f;
     } else {
         const float* from = a.dnew_state != nullptr
-            ? a.dnew_state + (static_cast<int64_t>(p.batch) * a.channels + p.channel) * S : nullptr;
+            ? a.dnew_state + (static_cast<int64_t>(batch) * a.channels + channel) * S + part * SPL : nullptr;
 #pragma unroll
-        for (int n = 0; n < S; ++n) carry[n] = from != nullptr && p.live ? from[n] : 0.f;
+        for (int j = 0; j < SPL; ++j) carry[j] = from != nullptr && live ? from[j] : 0.f;
     }
-    const float bias = a.dt_bias != nullptr ? a.dt_bias[p.channel] : 0.f;
-    const float D = a.D != nullptr ? a.D[p.channel] : 0.f;
-    float dD = 0.f, dbias = 0.f;
-    const T* x = static_cast<const T*>(a.x.data) + p.batch * a.x.bs + p.channel;
-    const T* dt = static_cast<const T*>(a.dt.data) + p.batch * a.dt.bs + p.channel;
-    const T* dy = static_cast<const T*>(a.dy.data) + p.batch * a.dy.bs + p.channel;
-    const T* gate = a.gate.data != nullptr
-        ? static_cast<const T*>(a.gate.data) + p.batch * a.gate.bs + p.channel : nullptr;
-    const int64_t b0 = p.batch * a.b.bs + static_cast<int64_t>(p.group) * S;
-    const int64_t c0 = p.batch * a.c.bs + static_cast<int64_t>(p.group) * S;
-    const int64_t out0 = static_cast<int64_t>(p.batch) * a.tokens * a.channels + p.channel;
-    const int64_t bc_row0 = (static_cast<int64_t>(p.tile) * a.batches + p.batch) * a.tokens;
 
-    const int32_t count = p.te - p.t0;
-    for (int32_t blk = (count + BLOCK - 1) / BLOCK - 1; blk >= 0; --blk) {
-        const int32_t tb = p.t0 + blk * BLOCK;                      // first token of the block
-        const int32_t nb = p.te - tb < BLOCK ? p.te - tb : BLOCK;   // its tokens
-        const int32_t last = (nb - 1) / SUB;
-        {
-            const float* from = a.kept + (static_cast<int64_t>(p.batch) * a.blocks + tb / BLOCK) * S * cp + p.column;
-            float h[S];
+    // by token and channel
+    const int32_t tc = tid % CHANNELS, tr = wave / (CHANNELS / 64) * TOKENS;   // channel and first token
+    const bool tlive = first + tc < a.group_channels;
+    const int32_t tchannel = group * a.group_channels + (tlive ? first + tc : a.group_channels - 1);
+    const float bias = a.dt_bias != nullptr ? a.dt_bias[tchannel] : 0.f;
+    const float D = a.D != nullptr ? a.D[tchannel] : 0.f;
+    const T* x = static_cast<const T*>(a.x.data) + batch * a.x.bs;
+    const T* dt = static_cast<const T*>(a.dt.data) + batch * a.dt.bs;
+    const T* dy = static_cast<const T*>(a.dy.data) + batch * a.dy.bs;
+    const T* gate = a.gate.data != nullptr
+        ? static_cast<const T*>(a.gate.data) + batch * a.gate.bs : nullptr;
+    const BCT* bmap = static_cast<const BCT*>(a.b.data) + batch * a.b.bs + static_cast<int64_t>(group) * S;
+    const BCT* cmap = static_cast<const BCT*>(a.c.data) + batch * a.c.bs + static_cast<int64_t>(group) * S;
+    const int64_t out0 = static_cast<int64_t>(batch) * a.tokens * a.channels;
+    float* bc = a.bc_partial + (static_cast<int64_t>(tile) * a.batches + batch) * a.tokens * (2 * S);
+    float dD = 0.f, dbias = 0.f;
+
+    constexpr int MAPS = (SS_BLOCK * 2 * S + 255) / 256;   // values of B and C a thread brings
+    struct Raw { T x[TOKENS], dt[TOKENS], dy[TOKENS], gate[TOKENS]; };
+    Raw next;
+    float next_maps[MAPS];
+    auto fetch = [&](int32_t tb) {
+        const uint32_t at = opaque(static_cast<uint32_t>(tchannel) * sizeof(T));
 #pragma unroll
-            for (int n = 0; n < S; ++n) h[n] = from[n * cp];
-            for (int32_t sub = 0; sub < last; ++sub) {
-#pragma unroll
-                for (int n = 0; n < S; ++n) starts[sub][n][lane] = h[n];
-#pragma unroll
-                for (int u = 0; u < SUB; ++u) {
-                    const int64_t t = tb + sub * SUB + u;
-                    SSRow<BCT, S> b;
-                    b.load(a.b.data, b0 + t * a.b.ts);
-                    float step = to_f32(dt[t * a.dt.ts]) + bias;
-                    if (a.softplus) step = ss_softplus(step);
-                    const float dtx = step * (p.live ? to_f32(x[t * a.x.ts]) : 0.f);
-#pragma unroll
-                    for (int n = 0; n < S; ++n)
-                        h[n] = fmaf(dtx, b[n], h[n] * __builtin_amdgcn_exp2f(step * A2[n]));
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < S; ++n) starts[last][n][lane] = h[n];
+        for (int i = 0; i < TOKENS; ++i) {
+            const int64_t t = tb + tr + i < te ? tb + tr + i : te - 1;   // a token of the sequence
+            next.x[i] = load_at(x + t * a.x.ts, at);
+            next.dt[i] = load_at(dt + t * a.dt.ts, at);
+            next.dy[i] = load_at(dy + t * a.dy.ts, at);
+            if (gate != nullptr) next.gate[i] = load_at(gate + t * a.gate.ts, at);
         }
-        for (int32_t sub = last; sub >= 0; --sub) {
-            const int32_t ts = tb + sub * SUB;
-            const int32_t ns = p.te - ts < SUB ? p.te - ts : SUB;
-            float decay[SUB][S], q[SUB][S], h[S];
-            float raw[SUB], step[SUB], xv[SUB], gy[SUB], z[SUB];
+        const int32_t tid = opaque(threadIdx.x);
 #pragma unroll
-            for (int u = 0; u < SUB; ++u) {
-                const int64_t t = u < ns ? ts + u : ts + ns - 1;
-                raw[u] = to_f32(dt[t * a.dt.ts]) + bias;
-                xv[u] = to_f32(x[t * a.x.ts]);
-                gy[u] = to_f32(dy[t * a.dy.ts]);
-                z[u] = gate != nullptr ? to_f32(gate[t * a.gate.ts]) : 0.f;
+        for (int i = 0; i < MAPS; ++i) {
+            const int32_t v = tid + i * 256, r = v / (2 * S), n = v % (2 * S);
+            const int64_t t = tb + r;
+            next_maps[i] = v < SS_BLOCK * 2 * S && t < te
+                ? to_f32(n < S ? cmap[t * a.c.ts + n] : bmap[t * a.b.ts + n - S]) : 0.f;
+        }
+    };
+
+    const int32_t blocks = (te - t0 + SS_BLOCK - 1) / SS_BLOCK;
+    if (blocks > 0) fetch(t0 + (blocks - 1) * SS_BLOCK);
+    for (int32_t blk = blocks - 1; blk >= 0; --blk) {
+        const int32_t tb = t0 + blk * SS_BLOCK;
+        const Raw raw = next;
+        float h[SPL];
+        {
+            const float* from = a.kept + (static_cast<int64_t>(batch) * a.blocks + tb / SS_BLOCK) * S * cp;
+            const uint32_t at = opaque(static_cast<uint32_t>((part * SPL * cp + column) * sizeof(float)));
+#pragma unroll
+            for (int j = 0; j < SPL; ++j) h[j] = live ? load_at(from + j * cp, at) : 0.f;
+        }
+        // 1.  Tokens behind the sequence decay by one and add nothing.
+#pragma unroll
+        for (int i = 0; i < TOKENS; ++i) {
+            const bool in = tb + tr + i < te;
+            float step = to_f32(raw.dt[i]) + bias;
+            if (a.softplus) step = ss_softplus(step);
+            float dz = to_f32(raw.dy[i]);
+            if (gate != nullptr) {
+                const float z = to_f32(raw.gate[i]);
+                dz *= z * sigmoid_fast(z);
             }
+            const float dtx = step * to_f32(raw.x[i]);
+            tok[tr + i][tc] = make_float4(in ? step : 0.f, in && tlive ? dtx : 0.f, in && tlive ? dz : 0.f, 0.f);
+        }
 #pragma unroll
-            for (int n = 0; n < S; ++n) h[n] = starts[sub][n][lane];
+        for (int i = 0; i < MAPS; ++i)
+            if (tid + i * 256 < SS_BLOCK * 2 * S) (&maps[0][0])[tid + i * 256] = next_maps[i];
+        __syncthreads();
+        // 2.
+        float start[SUBS][SPL];
+#pragma unroll
+        for (int sub = 0; sub < SUBS; ++sub) {
+#pragma unroll
+            for (int j = 0; j < SPL; ++j) start[sub][j] = h[j];
+            if (sub == SUBS - 1) break;
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
-                // tokens behind the sequence decay by one and add nothing
-                const bool mine = p.live && u < ns;
-                step[u] = a.softplus ? ss_softplus(raw[u]) : raw[u];
-                step[u] = u < ns ? step[u] : 0.f;
-                xv[u] = mine ? xv[u] : 0.f;
-                gy[u] = mine ? gy[u] : 0.f;
-                const float dtx = step[u] * xv[u];
-                SSRow<BCT, S> b;
-                b.load(a.b.data, b0 + static_cast<int64_t>(u < ns ? ts + u : ts + ns - 1) * a.b.ts);
+                const float4 k = tok[sub * SUB + u][mine];
+                const float* b = &maps[sub * SUB + u][S + part * SPL];
 #pragma unroll
-                for (int n = 0; n < S; ++n) {
-                    decay[u][n] = __builtin_amdgcn_exp2f(step[u] * A2[n]);
-                    q[u][n] = decay[u][n] * h[n];
-                    h[n] = fmaf(dtx, b[n], q[u][n]);
+                for (int j = 0; j < SPL; ++j) h[j] = fmaf(k.y, b[j], h[j] * __builtin_amdgcn_exp2f(k.x * A2[j]));
+                if (u % 2) __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+#pragma unroll
+        for (int sub = SUBS - 1; sub >= 0; --sub) {
+            float decay[SUB][SPL], q[SUB][SPL];
+            // the tokens' entries are read again from LDS in each walk, not kept from the last
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < SPL; ++j) h[j] = start[sub][j];
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+                const float4 k = tok[sub * SUB + u][mine];
+                const float* b = &maps[sub * SUB + u][S + part * SPL];
+#pragma unroll
+                for (int j = 0; j < SPL; ++j) {
+                    decay[u][j] = __builtin_amdgcn_exp2f(k.x * A2[j]);
+                    q[u][j] = decay[u][j] * h[j];
+                    h[j] = fmaf(k.y, b[j], q[u][j]);
                 }
+                if (u % 2) __builtin_amdgcn_sched_barrier(0);
             }
+            asm volatile("" ::: "memory");
 #pragma unroll
             for (int u = SUB - 1; u >= 0; --u) {
-                if (u >= ns) continue;
-                const int64_t t = ts + u;
-                SSRow<BCT, S> b, c;
-                b.load(a.b.data, b0 + t * a.b.ts);
-                c.load(a.c.data, c0 + t * a.c.ts);
-                float silu = 1.f, dsilu = 0.f;
-                if (gate != nullptr) {
-                    const float sig = sigmoid_fast(z[u]);
-                    silu = z[u] * sig;
-                    dsilu = sig * fmaf(z[u], 1.f - sig, 1.f);
-                }
-                const float dz = gy[u] * silu, dtx = step[u] * xv[u];
-                float y = D * xv[u], gb = 0.f, ga = 0.f;
-                float v[2 * S];
+                const int32_t t = sub * SUB + u;
+                const float4 k = tok[t][mine];
+                const float* c = &maps[t][part * SPL];
+                const float* b = &maps[t][S + part * SPL];
+                float y = 0.f, gb = 0.f, ga = 0.f, v[2 * SPL];
 #pragma unroll
-                for (int n = 0; n < S; ++n) {
-                    const float hn = fmaf(dtx, b[n], q[u][n]);
-                    const float g = fmaf(c[n], dz, carry[n]);
-                    y = fmaf(c[n], hn, y);
-                    gb = fmaf(g, b[n], gb);
-                    const float gq = g * q[u][n];
-                    ga = fmaf(gq, A2[n], ga);
-                    dA[n] = fmaf(gq, step[u], dA[n]);
-                    carry[n] = g * decay[u][n];
-                    v[n] = dz * hn;
-                    v[S + n] = dtx * g;
+                for (int j = 0; j < SPL; ++j) {
+                    const float hj = fmaf(k.y, b[j], q[u][j]);
+                    const float g = fmaf(c[j], k.z, carry[j]);
+                    y = fmaf(c[j], hj, y);
+                    gb = fmaf(g, b[j], gb);
+                    const float gq = g * q[u][j];
+                    ga = fmaf(gq, A2[j], ga);
+                    dA[j] = fmaf(gq, k.x, dA[j]);
+                    carry[j] = g * decay[u][j];
+                    v[j] = k.z * hj;
+                    v[SPL + j] = k.y * g;
                 }
-                const float sum = lane_fold<2 * S>(v);
-                constexpr int SHARE = 64 / (2 * S);
-                if (lane % SHARE == 0) a.bc_partial[(bc_row0 + t) * (2 * S) + lane / SHARE] = sum;
-                // A2 is A log2(e)
-                float ddt = fmaf(xv[u], gb, ga * 0.6931471805599453f);
-                if (a.softplus) ddt *= sigmoid_fast(raw[u]);
-                const float dxv = fmaf(step[u], gb, D * dz);
-                dD = fmaf(dz, xv[u], dD);
-                dbias += ddt;
-                if (p.live) {
-                    const int64_t at = out0 + t * a.channels;
-                    static_cast<T*>(a.dx)[at] = from_f32<T>(dxv);
-                    static_cast<T*>(a.ddt)[at] = from_f32<T>(ddt);
-                    if (gate != nullptr) static_cast<T*>(a.dgate)[at] = from_f32<T>(gy[u] * y * dsilu);
+                y = state_sum<LANES>(y);
+                gb = state_sum<LANES>(gb);
+                ga = state_sum<LANES>(ga);
+                // dA's sums are formed here and not put off to the end of the walk, where each
+                // would still need its g q
+#pragma unroll
+                for (int j = 0; j < SPL; ++j) asm volatile("" : "+v"(dA[j]));
+                // the channel's lanes have read this token's entry: its last use here
+                if (part == 0) tok[t][mine] = make_float4(y, gb, ga, 0.f);
+                channel_sums<LANES, SPL>(v);
+                // lanes 0 .. LANES - 1 of each row of 16: C in rows 0 and 1, B in 2 and 3
+                const int32_t lane = tid & 63, row = lane >> 4;
+                if ((lane & 15) < LANES) {
+                    float* to = &parts[wave][t][(row >> 1) * S + part * SPL + (row & 1) * (SPL / 2)];
+#pragma unroll
+                    for (int j = 0; j < SPL / 2; ++j) to[j] = v[j];
                 }
+                if (u % 2 == 0) __builtin_amdgcn_sched_barrier(0);
             }
+        }
+        __syncthreads();
+        // 3.
+        if (blk > 0) fetch(tb - SS_BLOCK);
+        const uint32_t lane_at = opaque(static_cast<uint32_t>(tchannel) * sizeof(T));
+#pragma unroll
+        for (int i = 0; i < TOKENS; ++i) {
+            const int64_t t = tb + tr + i;
+            if (t >= te) continue;
+            const float4 r = tok[tr + i][tc];   // C h, g B, g A q over the states
+            const float xv = to_f32(raw.x[i]), gy = to_f32(raw.dy[i]), v = to_f32(raw.dt[i]) + bias;
+            const float step = a.softplus ? ss_softplus(v) : v;
+            float dz = gy, dgate = 0.f;
+            if (gate != nullptr) {
+                const float z = to_f32(raw.gate[i]), sig = sigmoid_fast(z);
+                dz *= z * sig;
+                dgate = gy * fmaf(D, xv, r.x) * (sig * fmaf(z, 1.f - sig, 1.f));
+            }
+            // A2 is A log2(e)
+            float ddt = fmaf(xv, r.y, r.z * 0.6931471805599453f);
+            if (a.softplus) ddt *= sigmoid_fast(v);
+            dD = fmaf(dz, xv, dD);
+            dbias += ddt;
+            if (tlive) {
+                const int64_t at = out0 + t * a.channels;
+                store_at<T>(a.dx, at, lane_at, fmaf(step, r.y, D * dz));
+                store_at<T>(a.ddt, at, lane_at, ddt);
+                if (gate != nullptr) store_at<T>(a.dgate, at, lane_at, dgate);
+            }
+        }
+        for (int32_t v = opaque(tid); v < SS_BLOCK * 2 * S; v += 256) {
+            const int32_t r = v / (2 * S), n = v % (2 * S);
+            if (tb + r < te)
+                bc[static_cast<int64_t>(tb) * (2 * S) + v] = (parts[0][r][n] + parts[1][r][n]) + (parts[2][r][n] + parts[3][r][n]);
         }
     }
     // behind the sequence's end
-    for (int64_t t = p.te; t < p.t1; ++t) {
-        if (p.live) {
-            const int64_t at = out0 + t * a.channels;
-            static_cast<T*>(a.dx)[at] = from_f32<T>(0.f);
-            static_cast<T*>(a.ddt)[at] = from_f32<T>(0.f);
-            if (gate != nullptr) static_cast<T*>(a.dgate)[at] = from_f32<T>(0.f);
-        }
-        if (lane < 2 * S) a.bc_partial[(bc_row0 + t) * (2 * S) + lane] = 0.f;
+    for (int64_t t = te + tid / CHANNELS; t < t1; t += 256 / CHANNELS) {
+        if (!tlive) break;
+        const int64_t at = out0 + t * a.channels + tchannel;
+        static_cast<T*>(a.dx)[at] = from_f32<T>(0.f);
+        static_cast<T*>(a.ddt)[at] = from_f32<T>(0.f);
+        if (gate != nullptr) static_cast<T*>(a.dgate)[at] = from_f32<T>(0.f);
     }
-    float* to = a.param_partial + (static_cast<int64_t>(p.batch) * a.chunks + p.chunk) * (S + 2) * cp + p.column;
+    for (int64_t v = static_cast<int64_t>(te) * (2 * S) + tid; v < static_cast<int64_t>(t1) * (2 * S); v += 256) bc[v] = 0.f;
+
+    float* to = a.param_partial + (static_cast<int64_t>(batch) * a.chunks + chunk) * (S + 2) * cp;
+    if (live) {
 #pragma unroll
-    for (int n = 0; n < S; ++n) to[n * cp] = dA[n];
-    to[S * cp] = dD;
-    to[(S + 1) * cp] = dbias;
-    if (a.dstate != nullptr && p.chunk == 0 && p.live) {
-        float* ds = a.dstate + (static_cast<int64_t>(p.batch) * a.channels + p.channel) * S;
+        for (int j = 0; j < SPL; ++j) to[(part * SPL + j) * cp + column] = dA[j];
+        if (a.dstate != nullptr && chunk == 0) {
+            float* ds = a.dstate + (static_cast<int64_t>(batch) * a.channels + channel) * S + part * SPL;
 #pragma unroll
-        for (int n = 0; n < S; n += 4)
-            *reinterpret_cast<float4*>(ds + n) = make_float4(carry[n], carry[n + 1], carry[n + 2], carry[n + 3]);
+            for (int j = 0; j < SPL; ++j) ds[j] = carry[j];
+        }
+    }
+    // dD and dbias: the threads of a channel, in order
+    __syncthreads();
+    tok[tid / CHANNELS][tc] = make_float4(dD, dbias, 0.f, 0.f);
+    __syncthreads();
+    if (tid < CHANNELS && tlive) {
+        float sum_D = 0.f, sum_bias = 0.f;
+#pragma unroll
+        for (int i = 0; i < 256 / CHANNELS; ++i) {
+            sum_D += tok[i][tc].x;
+            sum_bias += tok[i][tc].y;
+        }
+        const int64_t at = static_cast<int64_t>(group) * a.group_tiles * 64 + first + tc;
+        to[S * cp + at] = sum_D;
+        to[(S + 1) * cp + at] = sum_bias;
     }
 }
 
@@ -301,57 +419,81 @@ __global__ __launch_bounds__(256) void state_space_bc_kernel(const float* partia
     }
 }
 
-// Chunks of the backward: two waves a SIMD (its registers allow no more), whole blocks.
-constexpr int64_t TARGET_WAVES = 2048;
+// How the backward cuts a line.  A workgroup of the gradients' pass takes a chunk of 256 /
+// lanes channels; as many as the 256 CUs hold at once have one.  The adjoints' pass is one wave
+// for 64 channels and cuts each chunk into fine ones, to give every SIMD four waves.
+constexpr int64_t CUS = 256, TARGET_WAVES = 4096;
 
-int64_t backward_chunk(int64_t B, int64_t N, int64_t tiles, int32_t states) {
-    const int64_t block = ss_block_tokens(states), blocks = ss_ceil(N, block);
-    int64_t chunks = TARGET_WAVES / (B * tiles);
-    if (chunks < 1) chunks = 1;
-    if (chunks > blocks) chunks = blocks;
-    return ss_ceil(blocks, chunks) * block;
+struct Cut {
+    int64_t tiles, wide_tiles;               // of 64 channels, and of a workgroup's
+    int64_t chunk, chunks;                   // tokens a chunk, chunks a line
+    int64_t fine, fine_chunks, per_chunk;    // the same of the adjoints' pass
+};
+Cut make_cut(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
+    Cut c;
+    c.tiles = ss_ceil(C / groups, 64) * groups;
+    c.wide_tiles = ss_ceil(C / groups, states <= 8 ? 128 : 64) * groups;
+    const int64_t blocks = ss_ceil(N, SS_BLOCK);
+    int64_t chunks = CUS * backward_waves(states) / (B * c.wide_tiles);
+    chunks = chunks < 1 ? 1 : chunks > blocks ? blocks : chunks;
+    const int64_t per = ss_ceil(blocks, chunks);             // blocks a chunk
+    c.chunk = per * SS_BLOCK;
+    c.chunks = ss_ceil(N, c.chunk);
+    int64_t pieces = TARGET_WAVES / (B * c.tiles * c.chunks);
+    pieces = c.chunks == 1 || pieces < 1 ? 1 : pieces > per ? per : pieces;
+    while (per % pieces) --pieces;                           // whole blocks each
+    c.per_chunk = pieces;
+    c.fine = c.chunk / pieces;
+    c.fine_chunks = c.chunks == 1 ? 1 : ss_ceil(N, c.fine);
+    return c;
 }
 
 struct Space {   // the workspace, in floats
     int64_t slots, sums, bc, params, total_floats;
     size_t sum_bytes;
 };
-Space backward_space(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
-    const int64_t tiles = ss_ceil(C / groups, 64) * groups, cp = tiles * 64;
-    const int64_t chunks = ss_ceil(N, backward_chunk(B, N, tiles, states));
+Space backward_space(const Cut& c, int64_t B, int64_t N, int32_t states) {
+    const int64_t cp = c.tiles * 64;
     Space s;
     s.slots = 0;
-    s.sums = s.slots + B * (chunks - 1) * states * cp;
-    s.bc = s.sums + B * chunks * cp;
-    s.params = s.bc + tiles * B * N * 2 * states;
-    s.total_floats = s.params + B * chunks * (states + 2) * cp;
-    s.sum_bytes = param_sum_workspace_bytes(B * chunks, states + 2, cp);
+    s.sums = s.slots + B * (c.fine_chunks - 1) * states * cp;
+    s.bc = s.sums + B * c.fine_chunks * cp;
+    s.params = s.bc + c.wide_tiles * B * N * 2 * states;
+    s.total_floats = s.params + B * c.chunks * (states + 2) * cp;
+    s.sum_bytes = param_sum_workspace_bytes(B * c.chunks, states + 2, cp);
     return s;
 }
 
 template <typename T, typename BCT, int S>
-int launch_backward(SSArgs& a, int64_t B, hipStream_t s) {
-    if (a.chunks > 1) {
+int launch_backward(SSArgs& a, const Cut& c, int64_t B, hipStream_t s) {
+    constexpr int LANES = S == 8 ? 2 : 4;
+    a.wide_tiles = static_cast<int32_t>(c.wide_tiles);
+    a.fine_chunks = static_cast<int32_t>(c.fine_chunks);
+    a.fine_per_chunk = static_cast<int32_t>(c.per_chunk);
+    if (c.chunks > 1) {
+        a.chunk = static_cast<int32_t>(c.fine);
+        a.chunks = static_cast<int32_t>(c.fine_chunks);
         a.first_chunk = 1;
         a.launch_chunks = a.chunks - 1;
         state_space_adjoint_kernel<T, BCT, S><<<static_cast<uint32_t>(B * a.launch_chunks * a.tiles), 64, 0, s>>>(a);
         if (int rc = check_launch("state_space chunk adjoints")) return rc;
         if (int rc = ss_join(a, B, S, true, a.dnew_state, s)) return rc;
     }
-    a.first_chunk = 0;
-    a.launch_chunks = a.chunks;
-    state_space_backward_kernel<T, BCT, S><<<static_cast<uint32_t>(B * a.chunks * a.tiles), 64, 0, s>>>(a);
+    a.chunk = static_cast<int32_t>(c.chunk);
+    a.chunks = static_cast<int32_t>(c.chunks);
+    state_space_backward_kernel<T, BCT, LANES, S / LANES>
+        <<<static_cast<uint32_t>(B * c.chunks * c.wide_tiles), 256, 0, s>>>(a);
     return check_launch("state_space backward");
 }
 
 template <typename T, typename BCT>
-int launch_states(SSArgs& a, int64_t B, int32_t S, void* db, void* dc, int32_t groups, hipStream_t s) {
-    int rc = S == 8 ? launch_backward<T, BCT, 8>(a, B, s)
-           : S == 16 ? launch_backward<T, BCT, 16>(a, B, s) : launch_backward<T, BCT, 32>(a, B, s);
+int launch_states(SSArgs& a, const Cut& c, int64_t B, int32_t S, void* db, void* dc, hipStream_t s) {
+    int rc = S == 8 ? launch_backward<T, BCT, 8>(a, c, B, s)
+           : S == 16 ? launch_backward<T, BCT, 16>(a, c, B, s) : launch_backward<T, BCT, 32>(a, c, B, s);
     if (rc) return rc;
-    const int64_t rows = B * a.tokens, blocks = ss_ceil(rows * groups * 2 * S, 256);
+    const int64_t rows = B * a.tokens, blocks = ss_ceil(rows * a.groups * 2 * S, 256);
     state_space_bc_kernel<T><<<static_cast<uint32_t>(blocks < 65536 ? blocks : 65536), 256, 0, s>>>(
-        a.bc_partial, static_cast<T*>(db), static_cast<T*>(dc), rows, S, groups, a.group_tiles);
+        a.bc_partial, static_cast<T*>(db), static_cast<T*>(dc), rows, S, a.groups, a.wide_tiles / a.groups);
     return check_launch("state_space dB and dC");
 }
 
@@ -363,7 +505,7 @@ extern "C" {
 size_t vh_state_space_backward_workspace_bytes(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
     using namespace vh;
     if (B <= 0 || N <= 0 || C <= 0 || groups <= 0 || C % groups || states <= 0) return 0;
-    const Space s = backward_space(B, N, C, groups, states);
+    const Space s = backward_space(make_cut(B, N, C, groups, states), B, N, states);
     return static_cast<size_t>(s.total_floats) * sizeof(float) + s.sum_bytes;
 }
 
@@ -399,7 +541,8 @@ int vh_state_space_backward(
                    (gate == nullptr) == (dgate == nullptr), VH_ERR_ARG,
                "dy, kept, dx, ddt, db and dc must be given, dgate exactly with a gate");
     VH_REQUIRE(reinterpret_cast<uintptr_t>(dstate) % 16 == 0, VH_ERR_ARG, "dstate must be 16-byte aligned");
-    const Space sp = backward_space(B, N, C, groups, states);
+    const Cut cut = make_cut(B, N, C, groups, states);
+    const Space sp = backward_space(cut, B, N, states);
     const size_t need = static_cast<size_t>(sp.total_floats) * sizeof(float) + sp.sum_bytes;
     VH_REQUIRE(workspace != nullptr && workspace_bytes >= need, VH_ERR_WORKSPACE,
                "state space backward needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
@@ -408,18 +551,16 @@ int vh_state_space_backward(
     a.sums = ws + sp.sums;
     a.bc_partial = ws + sp.bc;
     a.param_partial = ws + sp.params;
-    a.chunk = static_cast<int32_t>(backward_chunk(B, N, a.tiles, states));
-    a.chunks = static_cast<int32_t>(ss_ceil(N, a.chunk));
     hipStream_t s = static_cast<hipStream_t>(stream);
     int rc;
-    if (io_dtype == VH_DTYPE_F32) rc = launch_states<float, float>(a, B, states, db, dc, groups, s);
-    else if (io_dtype == VH_DTYPE_F16) rc = launch_states<f16_t, float>(a, B, states, db, dc, groups, s);
-    else if (bc_dtype == VH_DTYPE_F32) rc = launch_states<bf16_t, float>(a, B, states, db, dc, groups, s);
-    else rc = launch_states<bf16_t, bf16_t>(a, B, states, db, dc, groups, s);
+    if (io_dtype == VH_DTYPE_F32) rc = launch_states<float, float>(a, cut, B, states, db, dc, s);
+    else if (io_dtype == VH_DTYPE_F16) rc = launch_states<f16_t, float>(a, cut, B, states, db, dc, s);
+    else if (bc_dtype == VH_DTYPE_F32) rc = launch_states<bf16_t, float>(a, cut, B, states, db, dc, s);
+    else rc = launch_states<bf16_t, bf16_t>(a, cut, B, states, db, dc, s);
     if (rc) return rc;
     ParamSum sum{};
     sum.partial = a.param_partial;
-    sum.rows = B * a.chunks;
+    sum.rows = B * cut.chunks;
     sum.quantities = states + 2;
     sum.columns = a.tiles * 64;
     sum.per_channel = states;
