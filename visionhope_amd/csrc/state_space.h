@@ -47,7 +47,9 @@ struct SSArgs {
 struct SSPlace {
     int32_t batch, chunk, tile, group, lane, channel;
     int64_t column;     // of the padded channels
-    bool live;          // the lane has a channel
+    // the lane has a channel of its own; the others take the group's last one too, compute and
+    // store the same as its lane, and so need no branch in the token loop
+    bool live;
     int32_t t0, t1, te; // tokens [t0, t1) of the chunk, of which [t0, te) belong to the sequence
 };
 
@@ -74,6 +76,31 @@ __device__ __forceinline__ SSPlace ss_place(const SSArgs& a) {
     p.te = len < p.t0 ? p.t0 : len > p.t1 ? p.t1 : len;
     return p;
 }
+
+// An element `offset` bytes behind a uniform address.  The offset passes through a register the
+// compiler cannot see behind, or it would keep a 64-bit address a lane for every tensor in
+// vector registers over the whole walk.
+__device__ __forceinline__ uint32_t opaque(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T load_at(const T* base, uint32_t offset) {
+    return *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + offset);
+}
+template <typename T>
+__device__ __forceinline__ void store_at(void* base, int64_t element, uint32_t offset, float v) {
+    *reinterpret_cast<T*>(reinterpret_cast<char*>(static_cast<T*>(base) + element) + offset) = from_f32<T>(v);
+}
+
+// An activation at the first token of a wave's chunk.
+template <typename T>
+__device__ __forceinline__ const T* ss_tokens(const SSTokens& t, const SSPlace& p) {
+    return static_cast<const T*>(t.data) + p.batch * t.bs + p.t0 * t.ts;
+}
+
+// Tokens that a wave loads together, one group ahead of the arithmetic.
+constexpr int SS_UNROLL = 4;
 
 // One token's row of S values of B or C, read through the scalar cache (a uniform address in
 // memory that no kernel here writes): 16-bit pairs or FP32, 4-byte aligned.

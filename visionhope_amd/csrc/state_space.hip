@@ -14,8 +14,6 @@
 namespace vh {
 namespace {
 
-constexpr int UNROLL = 4;   // tokens loaded together, one group ahead of the arithmetic
-
 // OUT: the output pass; otherwise the pass for the chunks' own states.
 template <typename T, typename BCT, int S, bool OUT>
 __global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
@@ -33,73 +31,90 @@ __global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
     } else if (OUT && a.state != nullptr) {
         const float* from = a.state + (static_cast<int64_t>(p.batch) * a.channels + p.channel) * S;
 #pragma unroll
-        for (int n = 0; n < S; ++n) h[n] = p.live ? from[n] : 0.f;
+        for (int n = 0; n < S; ++n) h[n] = from[n];
     } else {
 #pragma unroll
         for (int n = 0; n < S; ++n) h[n] = 0.f;
     }
-    const T* x = static_cast<const T*>(a.x.data) + p.batch * a.x.bs + p.t0 * a.x.ts;
-    const T* dt = static_cast<const T*>(a.dt.data) + p.batch * a.dt.bs + p.t0 * a.dt.ts;
-    const T* gate = OUT && a.gate.data != nullptr
-        ? static_cast<const T*>(a.gate.data) + p.batch * a.gate.bs + p.t0 * a.gate.ts : nullptr;
-    const int64_t bc0 = static_cast<int64_t>(p.group) * S;
-    int64_t brow = p.batch * a.b.bs + p.t0 * a.b.ts + bc0, crow = p.batch * a.c.bs + p.t0 * a.c.ts + bc0;
-    T* y = OUT ? static_cast<T*>(a.y) + (static_cast<int64_t>(p.batch) * a.tokens + p.t0) * a.channels : nullptr;
+    const uint32_t lane_at = static_cast<uint32_t>(p.channel) * sizeof(T);
+    const bool gated = OUT && a.gate.data != nullptr, soft = a.softplus != 0;
+    const T* x = ss_tokens<T>(a.x, p);
+    const T* dt = ss_tokens<T>(a.dt, p);
+    const T* gate = gated ? ss_tokens<T>(a.gate, p) : x;
+    const int64_t gate_ts = gated ? a.gate.ts : a.x.ts;
+    const int64_t b0 = p.batch * a.b.bs + p.t0 * a.b.ts + static_cast<int64_t>(p.group) * S;
+    const int64_t c0 = p.batch * a.c.bs + p.t0 * a.c.ts + static_cast<int64_t>(p.group) * S;
+    const int64_t out0 = (static_cast<int64_t>(p.batch) * a.tokens + p.t0) * a.channels;
     const int32_t count = p.te - p.t0;
     float total = 0.f;
 
-    T xr[UNROLL], dr[UNROLL], gr[UNROLL], xn[UNROLL], dn[UNROLL], gn[UNROLL];
-    auto fetch = [&](int32_t t) {
+    // B and C of a token are loaded during the one before it where the scalar registers hold two
+    // rows of each; the barrier keeps the compiler from loading the rows of all the tokens of
+    // an iteration first and moving them to vector registers.
+    constexpr bool AHEAD = S * sizeof(BCT) <= 64;
+    SSRow<BCT, S> bn, cn;
+    auto rows = [&](int32_t t) {
+        bn.load(a.b.data, b0 + t * a.b.ts);
+        if (OUT) cn.load(a.c.data, c0 + t * a.c.ts);
+    };
+    auto token = [&](T xr, T dr, T gr, int32_t t) {
+        if (!AHEAD) rows(t);
+        const SSRow<BCT, S> b = bn, c = cn;
+        if (AHEAD) {
+            rows(t + 1 < count ? t + 1 : t);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const float raw = to_f32(dr) + bias, xv = to_f32(xr), z = to_f32(gr);
+        const float plus = ss_softplus(raw), step = soft ? plus : raw;   // no branch in the loop
+        const float dtx = step * xv;
+        float acc = D * xv;
+        if (!OUT) total += step;
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int32_t at = t + u < count ? t + u : count - 1;   // a token of the sequence
-            xn[u] = x[at * a.x.ts + p.channel];
-            dn[u] = dt[at * a.dt.ts + p.channel];
-            if (OUT && gate != nullptr) gn[u] = gate[at * a.gate.ts + p.channel];
+        for (int n = 0; n < S; ++n) {
+            h[n] = fmaf(dtx, b[n], h[n] * __builtin_amdgcn_exp2f(step * A2[n]));
+            if (OUT) acc = fmaf(c[n], h[n], acc);
+        }
+        const float silu = z * sigmoid_fast(z);
+        if (OUT) store_at<T>(a.y, out0 + static_cast<int64_t>(t) * a.channels, lane_at, acc * (gated ? silu : 1.f));
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    T xn[SS_UNROLL], dn[SS_UNROLL], gn[SS_UNROLL];
+    auto fetch = [&](int32_t t) {
+        const uint32_t at = opaque(lane_at);
+#pragma unroll
+        for (int u = 0; u < SS_UNROLL; ++u) {
+            const int64_t i = t + u < count ? t + u : count - 1;   // a token of the sequence
+            xn[u] = load_at(x + i * a.x.ts, at);
+            dn[u] = load_at(dt + i * a.dt.ts, at);
+            if (OUT) gn[u] = load_at(gate + i * gate_ts, at);
         }
     };
-    if (count > 0) fetch(0);
-    for (int32_t t = 0; t < count; t += UNROLL) {
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) { xr[u] = xn[u]; dr[u] = dn[u]; gr[u] = gn[u]; }
-        if (t + UNROLL < count) fetch(t + UNROLL);
+    if (count > 0) {
+        fetch(0);
+        if (AHEAD) rows(0);
+    }
+    int32_t t = 0;
+    for (; t < count; t += SS_UNROLL) {
         if (OUT && a.kept != nullptr && t % SS_BLOCK == 0) {
             float* to = a.kept + (static_cast<int64_t>(p.batch) * a.blocks + (p.t0 + t) / SS_BLOCK) * S * cp + p.column;
 #pragma unroll
             for (int n = 0; n < S; ++n) to[n * cp] = h[n];
         }
+        if (t + SS_UNROLL > count) break;
+        T xr[SS_UNROLL], dr[SS_UNROLL], gr[SS_UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            if (t + u >= count) break;
-            SSRow<BCT, S> b, c;
-            b.load(a.b.data, brow);
-            if (OUT) c.load(a.c.data, crow);
-            float step = to_f32(dr[u]) + bias;
-            if (a.softplus) step = ss_softplus(step);
-            const float xv = p.live ? to_f32(xr[u]) : 0.f;
-            const float dtx = step * xv;
-            float acc = D * xv;
-            if (!OUT) total += step;
+        for (int u = 0; u < SS_UNROLL; ++u) { xr[u] = xn[u]; dr[u] = dn[u]; gr[u] = gn[u]; }
+        fetch(t + SS_UNROLL);
 #pragma unroll
-            for (int n = 0; n < S; ++n) {
-                h[n] = fmaf(dtx, b[n], h[n] * __builtin_amdgcn_exp2f(step * A2[n]));
-                if (OUT) acc = fmaf(c[n], h[n], acc);
-            }
-            if (OUT) {
-                if (gate != nullptr) {
-                    const float z = to_f32(gr[u]);
-                    acc *= z * sigmoid_fast(z);
-                }
-                if (p.live) y[static_cast<int64_t>(t + u) * a.channels + p.channel] = from_f32<T>(acc);
-            }
-            brow += a.b.ts;
-            crow += a.c.ts;
-        }
+        for (int u = 0; u < SS_UNROLL; ++u) token(xr[u], dr[u], gr[u], t + u);
     }
+#pragma unroll
+    for (int u = 0; u < SS_UNROLL - 1; ++u)
+        if (t + u < count) token(xn[u], dn[u], gn[u], t + u);
     if (OUT) {
-        for (int32_t t = count; t < p.t1 - p.t0; ++t)   // behind the sequence's end
-            if (p.live) y[static_cast<int64_t>(t) * a.channels + p.channel] = from_f32<T>(0.f);
-        if (a.new_state != nullptr && p.chunk == a.chunks - 1 && p.live) {
+        for (t = count; t < p.t1 - p.t0; ++t)   // behind the sequence's end
+            store_at<T>(a.y, out0 + static_cast<int64_t>(t) * a.channels, lane_at, 0.f);
+        if (a.new_state != nullptr && p.chunk == a.chunks - 1) {
             float* to = a.new_state + (static_cast<int64_t>(p.batch) * a.channels + p.channel) * S;
 #pragma unroll
             for (int n = 0; n < S; n += 4)
@@ -128,8 +143,8 @@ __global__ void state_space_join_kernel(float* slots, const float* sums, const f
     const int32_t tile = blockIdx.x % tiles, n = (blockIdx.x / tiles) % S;
     const int64_t batch = blockIdx.x / (tiles * S);
     const int32_t group = tile / group_tiles, in_group = (tile - group * group_tiles) * 64 + lane;
-    const bool live = in_group < group_channels;
-    const int32_t channel = group * group_channels + (live ? in_group : group_channels - 1);
+    // lanes without a channel carry the group's last one, as in the other passes
+    const int32_t channel = group * group_channels + (in_group < group_channels ? in_group : group_channels - 1);
     const int64_t cp = static_cast<int64_t>(tiles) * 64, column = static_cast<int64_t>(tile) * 64 + lane;
     const float A2 = A[static_cast<int64_t>(channel) * S + n] * SS_LOG2E;
     float* slot = slots + (batch * slots_n * S + n) * cp + column;
@@ -153,7 +168,7 @@ __global__ void state_space_join_kernel(float* slots, const float* sums, const f
         fold_p[wave][lane] = ps;
         __syncthreads();
     }
-    h = edge != nullptr && live ? edge[(batch * channels + channel) * S + n] : 0.f;
+    h = edge != nullptr ? edge[(batch * channels + channel) * S + n] : 0.f;
     for (int32_t w = 0; w < wave; ++w) h = decayed(fold_p[w][lane], h) + fold_h[w][lane];
 #pragma unroll 8
     for (int32_t i = i0; i < i1; ++i) {
@@ -235,17 +250,29 @@ __global__ __launch_bounds__(256) void state_space_step_kernel(const StepArgs a)
     }
 }
 
-// Waves that a chunked pass aims at: four a SIMD (1024 SIMDs), and the fewest tokens a chunk
-// is worth cutting to.
-constexpr int64_t TARGET_WAVES = 4096;
-constexpr int64_t MIN_CHUNK = 32;
-
+// Tokens a chunk.  A line stays whole where sequences and channels alone give every SIMD a
+// wave (1024 SIMDs); otherwise the count of chunks is the one whose passes take the least time
+// by what a wave costs: a SIMD issues a vector instruction every 7.2, 5.3, 4.9, 4.6, 4.5
+// cycles with 1, 2, 3, 4, 5 and more waves (measured), every chunk spends about 8 tokens'
+// time around its loop, and chunks are whole blocks of 16 tokens.
 int64_t forward_chunk(int64_t B, int64_t N, int64_t tiles) {
-    int64_t chunks = TARGET_WAVES / (B * tiles);
-    if (chunks > ss_ceil(N, MIN_CHUNK)) chunks = ss_ceil(N, MIN_CHUNK);
-    if (chunks < 2) return ss_ceil(N, MIN_CHUNK) * MIN_CHUNK;
-    // whole blocks of every state count (8, 16 or 32 tokens)
-    return ss_ceil(ss_ceil(N, chunks), MIN_CHUNK) * MIN_CHUNK;
+    const int64_t blocks = ss_ceil(N, SS_BLOCK), lines = B * tiles;
+    static const double issue[] = {0., 7.2, 5.3, 4.9, 4.6, 4.5, 4.5};
+    if (lines >= 1024 || blocks < 3) return blocks * SS_BLOCK;
+    int64_t best = blocks;
+    double least = 0.;
+    for (int64_t waves = 1; waves <= 6; ++waves) {
+        int64_t chunks = waves * 1024 / lines;
+        chunks = chunks < 2 ? 2 : chunks > blocks ? blocks : chunks;
+        const int64_t per = ss_ceil(blocks, chunks);
+        const int64_t each = ss_ceil(ss_ceil(blocks, per) * lines, 1024);
+        const double time = static_cast<double>(per * SS_BLOCK + 8) * each * issue[each < 6 ? each : 6];
+        if (least == 0. || time < least) {
+            least = time;
+            best = per;
+        }
+    }
+    return best * SS_BLOCK;
 }
 
 template <typename T, typename BCT, int S>

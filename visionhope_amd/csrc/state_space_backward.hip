@@ -17,8 +17,6 @@
 namespace vh {
 namespace {
 
-constexpr int UNROLL = 4;
-
 // Adjoint that each chunk hands to the one before it from a zero adjoint behind it, and the
 // chunk's sum of dt.
 template <typename T, typename BCT, int S>
@@ -32,46 +30,55 @@ __global__ __launch_bounds__(64) void state_space_adjoint_kernel(const SSArgs a)
         carry[n] = 0.f;
     }
     const float bias = a.dt_bias != nullptr ? a.dt_bias[p.channel] : 0.f;
-    const T* dt = static_cast<const T*>(a.dt.data) + p.batch * a.dt.bs + p.t0 * a.dt.ts;
-    const T* dy = static_cast<const T*>(a.dy.data) + p.batch * a.dy.bs + p.t0 * a.dy.ts;
-    const T* gate = a.gate.data != nullptr
-        ? static_cast<const T*>(a.gate.data) + p.batch * a.gate.bs + p.t0 * a.gate.ts : nullptr;
+    const uint32_t lane_at = static_cast<uint32_t>(p.channel) * sizeof(T);
+    const bool gated = a.gate.data != nullptr, soft = a.softplus != 0;
+    const T* dt = ss_tokens<T>(a.dt, p);
+    const T* dy = ss_tokens<T>(a.dy, p);
+    const T* gate = gated ? ss_tokens<T>(a.gate, p) : dy;
+    const int64_t gate_ts = gated ? a.gate.ts : a.dy.ts;
     const int64_t c0 = p.batch * a.c.bs + p.t0 * a.c.ts + static_cast<int64_t>(p.group) * S;
     const int32_t count = p.te - p.t0;
     float total = 0.f;
-    T dr[UNROLL], yr[UNROLL], gr[UNROLL], dn[UNROLL], yn[UNROLL], gn[UNROLL];
-    auto fetch = [&](int32_t t) {   // tokens t, t - 1, ...
+    SSRow<BCT, S> cn;   // loaded a token ahead, as the forward loads B and C
+    auto token = [&](T dr, T yr, T gr, int32_t t) {
+        const SSRow<BCT, S> c = cn;
+        cn.load(a.c.data, c0 + (t > 0 ? t - 1 : 0) * a.c.ts);
+        __builtin_amdgcn_sched_barrier(0);
+        const float raw = to_f32(dr) + bias, z = to_f32(gr);
+        const float plus = ss_softplus(raw), step = soft ? plus : raw;   // no branch in the loop
+        const float silu = z * sigmoid_fast(z), dz = to_f32(yr) * (gated ? silu : 1.f);
+        total += step;
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int32_t at = t - u > 0 ? t - u : 0;
-            dn[u] = dt[at * a.dt.ts + p.channel];
-            yn[u] = dy[at * a.dy.ts + p.channel];
-            if (gate != nullptr) gn[u] = gate[at * a.gate.ts + p.channel];
+        for (int n = 0; n < S; ++n) carry[n] = fmaf(c[n], dz, carry[n]) * __builtin_amdgcn_exp2f(step * A2[n]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    int32_t t = count - 1;
+    T dn[SS_UNROLL], yn[SS_UNROLL], gn[SS_UNROLL];
+    auto fetch = [&](int32_t t) {   // tokens t, t - 1, ...
+        const uint32_t at = opaque(lane_at);
+#pragma unroll
+        for (int u = 0; u < SS_UNROLL; ++u) {
+            const int64_t i = t - u > 0 ? t - u : 0;
+            dn[u] = load_at(dt + i * a.dt.ts, at);
+            yn[u] = load_at(dy + i * a.dy.ts, at);
+            gn[u] = load_at(gate + i * gate_ts, at);
         }
     };
-    if (count > 0) fetch(count - 1);
-    for (int32_t t = count - 1; t >= 0; t -= UNROLL) {
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) { dr[u] = dn[u]; yr[u] = yn[u]; gr[u] = gn[u]; }
-        if (t >= UNROLL) fetch(t - UNROLL);
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            if (t - u < 0) break;
-            SSRow<BCT, S> c;
-            c.load(a.c.data, c0 + (t - u) * a.c.ts);
-            float step = to_f32(dr[u]) + bias;
-            if (a.softplus) step = ss_softplus(step);
-            total += step;
-            float dz = p.live ? to_f32(yr[u]) : 0.f;
-            if (gate != nullptr) {
-                const float z = to_f32(gr[u]);
-                dz *= z * sigmoid_fast(z);
-            }
-#pragma unroll
-            for (int n = 0; n < S; ++n)
-                carry[n] = fmaf(c[n], dz, carry[n]) * __builtin_amdgcn_exp2f(step * A2[n]);
-        }
+    if (count > 0) {
+        fetch(t);
+        cn.load(a.c.data, c0 + t * a.c.ts);
     }
+    for (; t >= SS_UNROLL - 1; t -= SS_UNROLL) {
+        T dr[SS_UNROLL], yr[SS_UNROLL], gr[SS_UNROLL];
+#pragma unroll
+        for (int u = 0; u < SS_UNROLL; ++u) { dr[u] = dn[u]; yr[u] = yn[u]; gr[u] = gn[u]; }
+        fetch(t - SS_UNROLL);
+#pragma unroll
+        for (int u = 0; u < SS_UNROLL; ++u) token(dr[u], yr[u], gr[u], t - u);
+    }
+#pragma unroll
+    for (int u = 0; u < SS_UNROLL - 1; ++u)
+        if (t - u >= 0) token(dn[u], yn[u], gn[u], t - u);
     float* to = a.slots + (static_cast<int64_t>(p.batch) * (a.chunks - 1) + p.chunk - 1) * S * cp + p.column;
 #pragma unroll
     for (int n = 0; n < S; ++n) to[n * cp] = carry[n];
@@ -106,22 +113,6 @@ __device__ __forceinline__ float state_sum(float v) {
     v += ln_dpp<0xB1>(v);
     if constexpr (LANES == 4) v += ln_dpp<0x4E>(v);
     return v;
-}
-
-// An element `offset` bytes behind a uniform address.  The offset passes through a register the
-// compiler cannot see behind, or it would keep a 64-bit address a lane for every tensor in
-// vector registers over the whole walk.
-__device__ __forceinline__ uint32_t opaque(uint32_t v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
-template <typename T>
-__device__ __forceinline__ T load_at(const T* base, uint32_t offset) {
-    return *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + offset);
-}
-template <typename T>
-__device__ __forceinline__ void store_at(void* base, int64_t element, uint32_t offset, float v) {
-    *reinterpret_cast<T*>(reinterpret_cast<char*>(static_cast<T*>(base) + element) + offset) = from_f32<T>(v);
 }
 
 // Waves a SIMD that the registers of the gradients' pass allow.
@@ -439,9 +430,10 @@ Cut make_cut(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
     const int64_t per = ss_ceil(blocks, chunks);             // blocks a chunk
     c.chunk = per * SS_BLOCK;
     c.chunks = ss_ceil(N, c.chunk);
-    int64_t pieces = TARGET_WAVES / (B * c.tiles * c.chunks);
-    pieces = c.chunks == 1 || pieces < 1 ? 1 : pieces > per ? per : pieces;
-    while (per % pieces) --pieces;                           // whole blocks each
+    // (a chunk is a multiple of 16 tokens, so the fine ones divide it)
+    int64_t pieces = 1;
+    while (pieces < 16 && c.chunks > 1 && c.chunk / pieces >= 32 && B * c.tiles * c.chunks * pieces * 2 <= TARGET_WAVES * 5 / 4)
+        pieces *= 2;
     c.per_chunk = pieces;
     c.fine = c.chunk / pieces;
     c.fine_chunks = c.chunks == 1 ? 1 : ss_ceil(N, c.fine);
