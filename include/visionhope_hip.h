@@ -583,18 +583,18 @@ int vh_causal_conv_step(const void* x, int64_t x_batch, int32_t io_dtype, const 
 /* Selective state space scan, S states a channel in FP32:
  *   step = softplus(dt + dt_bias) (softplus = 1) or dt + dt_bias
  *   h[n] = exp(step A[c, n]) h[n] + step x B[n],   y = (sum_n C[n] h[n] + D x) silu(gate)
- * x, dt, gate (or NULL) [B, N, C] in io_dtype; b, c [B, N, groups, S] in bc_dtype (fp32, or
- * bf16 with bf16 activations), the [groups, S] part dense, 4-byte aligned rows, channel c in
- * group c / (C / groups); A [C, S], D and dt_bias [C] (or NULL) fp32; states S = 8, 16 or 32
- * (zero-pad others: a state with A = B = C = 0 changes nothing).  state and new_state
- * [B, C, S] fp32 (or NULL), 16-byte aligned, not overlapping.  kept (or NULL) receives what
- * the backward starts from (vh_state_space_kept_bytes).  Workspace from the query (may be 0). */
+ * x, dt, gate (or NULL) [B, N, C] and b, c [B, N, groups, S] in io_dtype, the [groups, S] part
+ * of a token dense, channel c in group c / (C / groups); A [C, S], D and dt_bias [C] (or NULL)
+ * fp32; S = 1..32 (8, 16 and 32 with fp32 or bf16 rows of whole words are read in place, others
+ * packed into the workspace first).  state and new_state [B, C, S] fp32 (or NULL), not
+ * overlapping.  kept (or NULL) receives what the backward starts from
+ * (vh_state_space_kept_bytes).  Workspaces from the queries, 16-byte aligned. */
 size_t vh_state_space_workspace_bytes(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states);
 size_t vh_state_space_kept_bytes(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states);
 int vh_state_space_forward(
     const void* x, int64_t x_batch, int64_t x_token, const void* dt, int64_t dt_batch, int64_t dt_token,
     const void* gate, int64_t gate_batch, int64_t gate_token, int32_t io_dtype,
-    const void* b, int64_t b_batch, int64_t b_token, const void* c, int64_t c_batch, int64_t c_token, int32_t bc_dtype,
+    const void* b, int64_t b_batch, int64_t b_token, const void* c, int64_t c_batch, int64_t c_token,
     const float* A, const float* D, const float* dt_bias, int32_t softplus, const float* state,
     const int32_t* lengths, void* y, float* new_state, float* kept, int64_t B, int64_t N, int64_t C, int32_t groups,
     int32_t states, void* workspace, size_t workspace_bytes, void* stream);
@@ -608,7 +608,7 @@ int vh_state_space_backward(
     const void* dy, int64_t dy_batch, int64_t dy_token, const void* x, int64_t x_batch, int64_t x_token,
     const void* dt, int64_t dt_batch, int64_t dt_token, const void* gate, int64_t gate_batch, int64_t gate_token,
     int32_t io_dtype, const void* b, int64_t b_batch, int64_t b_token, const void* c, int64_t c_batch, int64_t c_token,
-    int32_t bc_dtype, const float* A, const float* D, const float* dt_bias, int32_t softplus, const int32_t* lengths,
+    const float* A, const float* D, const float* dt_bias, int32_t softplus, const int32_t* lengths,
     const float* kept, const float* dnew_state, void* dx, void* ddt, void* dgate, void* db, void* dc, float* dA,
     float* dD, float* ddt_bias, float* dstate, int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states,
     void* workspace, size_t workspace_bytes, void* stream);

@@ -8,7 +8,7 @@ import pytest
 from visionhope_amd.utils import hip
 
 P = 0x1000   # never dereferenced: validation fails first
-F32, BF16, F16 = hip.VH_DTYPE_F32, hip.VH_DTYPE_BF16, hip.VH_DTYPE_F16
+F32 = hip.VH_DTYPE_F32
 
 
 @pytest.fixture(scope="module")
@@ -29,10 +29,10 @@ CONV_BACK = dict(dy=P, dyb=80, dyt=8, x=P, xb=80, xt=8, io=F32, weight=P, bias=N
                  stream=None)
 CONV_STEP = dict(x=P, xb=8, io=F32, weight=P, bias=None, silu=0, state=P, new_state=P, y=P, B=2, C=8, taps=4, stream=None)
 SCAN = dict(x=P, xb=80, xt=8, dt=P, dtb=80, dtt=8, gate=None, gb=0, gt=0, io=F32, b=P, bb=160, bt=16, c=P, cb=160,
-            ct=16, bc=F32, A=P, D=None, bias=None, softplus=1, state=None, lengths=None, y=P, new_state=None, kept=None,
+            ct=16, A=P, D=None, bias=None, softplus=1, state=None, lengths=None, y=P, new_state=None, kept=None,
             B=2, N=10, C=8, groups=1, states=16, ws=P, wsn=1 << 30, stream=None)
 SCAN_BACK = dict(dy=P, dyb=80, dyt=8, x=P, xb=80, xt=8, dt=P, dtb=80, dtt=8, gate=None, gb=0, gt=0, io=F32, b=P,
-                 bb=160, bt=16, c=P, cb=160, ct=16, bc=F32, A=P, D=None, bias=None, softplus=1, lengths=None, kept=P,
+                 bb=160, bt=16, c=P, cb=160, ct=16, A=P, D=None, bias=None, softplus=1, lengths=None, kept=P,
                  dnew=None, dx=P, ddt=P, dgate=None, db=P, dc=P, dA=P, dD=None, dbias=None, dstate=None, B=2, N=10,
                  C=8, groups=1, states=16, ws=P, wsn=1 << 30, stream=None)
 SCAN_STEP = dict(x=P, xb=8, dt=P, dtb=8, gate=None, gb=0, io=F32, b=P, bb=16, c=P, cb=16, A=P, D=None, bias=None,
@@ -55,18 +55,16 @@ REFUSED = [
     ("vh_causal_conv_step", CONV_STEP, dict(state=None), hip.VH_ERR_ARG, "null"),
     ("vh_causal_conv_step", CONV_STEP, dict(taps=0), hip.VH_ERR_SHAPE, "taps"),
     ("vh_state_space_forward", SCAN, dict(io=-1), hip.VH_ERR_DTYPE, "io_dtype"),
-    ("vh_state_space_forward", SCAN, dict(bc=BF16), hip.VH_ERR_DTYPE, "B and C"),
-    ("vh_state_space_forward", SCAN, dict(io=F16, bc=F16), hip.VH_ERR_DTYPE, "B and C"),
-    ("vh_state_space_forward", SCAN, dict(states=12), hip.VH_ERR_SHAPE, "states"),
+    ("vh_state_space_forward", SCAN, dict(states=0), hip.VH_ERR_SHAPE, "states"),
+    ("vh_state_space_forward", SCAN, dict(states=33), hip.VH_ERR_SHAPE, "states"),
     ("vh_state_space_forward", SCAN, dict(groups=3), hip.VH_ERR_SHAPE, "groups"),
-    ("vh_state_space_forward", SCAN, dict(b=None), hip.VH_ERR_ARG, "B must"),
-    ("vh_state_space_forward", SCAN, dict(io=BF16, bc=BF16, ct=15), hip.VH_ERR_ARG, "C must"),
-    ("vh_state_space_forward", SCAN, dict(A=P + 4), hip.VH_ERR_ARG, "A must"),
-    ("vh_state_space_forward", SCAN, dict(state=P + 4), hip.VH_ERR_ARG, "aligned"),
+    ("vh_state_space_forward", SCAN, dict(b=None), hip.VH_ERR_ARG, "null"),
+    ("vh_state_space_forward", SCAN, dict(A=None), hip.VH_ERR_ARG, "null"),
     ("vh_state_space_forward", SCAN, dict(N=4096, wsn=16), hip.VH_ERR_WORKSPACE, "workspace"),
     ("vh_state_space_forward", SCAN, dict(B=1 << 23, C=1 << 20), hip.VH_ERR_SHAPE, "one launch"),
     ("vh_state_space_backward", SCAN_BACK, dict(kept=None), hip.VH_ERR_ARG, "kept"),
     ("vh_state_space_backward", SCAN_BACK, dict(gate=P), hip.VH_ERR_ARG, "dgate"),
+    ("vh_state_space_backward", SCAN_BACK, dict(ws=P + 4), hip.VH_ERR_WORKSPACE, "aligned"),
     ("vh_state_space_backward", SCAN_BACK, dict(wsn=16), hip.VH_ERR_WORKSPACE, "workspace"),
     ("vh_state_space_step", SCAN_STEP, dict(states=33), hip.VH_ERR_SHAPE, "states"),
     ("vh_state_space_step", SCAN_STEP, dict(B=0), hip.VH_ERR_SHAPE, "nonempty"),
@@ -89,7 +87,7 @@ def test_refused_before_any_launch(lib, name, defaults, change, status, message)
 def test_workspace_sizes(lib):
     assert lib.vh_state_space_kept_bytes(2, 33, 70, 1, 16) == 2 * 3 * 16 * 128 * 4
     assert lib.vh_state_space_kept_bytes(2, 33, 70, 2, 8) == 2 * 3 * 8 * 128 * 4
-    assert lib.vh_state_space_workspace_bytes(1, 1, 64, 1, 16) == 0          # one chunk
+    assert lib.vh_state_space_workspace_bytes(1, 1, 64, 1, 12) == 2 * 16 * 4   # packed B and C, one chunk
     assert lib.vh_state_space_workspace_bytes(0, 5, 64, 1, 16) == 0
     for name, args in (("vh_causal_conv_backward_workspace_bytes", (2, 10, 8, 4)),
                        ("vh_state_space_backward_workspace_bytes", (2, 10, 8, 1, 16)),

@@ -19,7 +19,8 @@ struct ConvArgs {
     const int32_t* lengths;
     const void* dnew_state;
     void *y, *new_state, *dx, *dstate;
-    float* partial;   // [B * segments, K + 1, C]
+    float* partial;   // [B * strips, K + 1, C]; a strip is SEGMENTS segments
+    int32_t strips;
     int32_t silu, tokens, channels, groups, segment, segments;
     int64_t threads;
 };
@@ -149,11 +150,29 @@ __global__ __launch_bounds__(256) void causal_conv_kernel(const ConvArgs a) {
 // K - 1 tokens past its end for the g that its last inputs need.  The inputs before the
 // first token (the state's) belong to segment 0, and the new state's gradient is added to
 // the inputs that it holds.
+// A workgroup takes 16 channel groups and SEGMENTS segments that follow each other, and sums
+// their weight gradients in LDS before they go to memory.
+constexpr int SEGMENTS = 16;
 template <typename T, int VEC, int K>
 __global__ __launch_bounds__(256) void causal_conv_backward_kernel(const ConvArgs a) {
     constexpr int BROWS = 4;
+    __shared__ float sums[SEGMENTS][K + 1][16 * VEC];
+    const int32_t row = threadIdx.x >> 4, column = threadIdx.x & 15;
+    const int32_t across = (a.groups + 15) / 16;
     ConvPlace p;
-    if (!conv_place<VEC>(a, a.segments, p)) return;
+    const int64_t rest = blockIdx.x / across;
+    const int32_t group = static_cast<int32_t>(blockIdx.x - rest * across) * 16 + column;
+    p.batch = rest / a.strips;
+    const int32_t strip = static_cast<int32_t>(rest - p.batch * a.strips);
+    p.segment = strip * SEGMENTS + row;
+    // lanes and segments past the end take part in the sums with nothing
+    const bool live = group < a.groups && p.segment < a.segments;
+    p.channel = (group < a.groups ? group : a.groups - 1) * VEC;
+    p.len = a.tokens;
+    if (a.lengths != nullptr) {
+        const int32_t l = a.lengths[p.batch];
+        p.len = l < 0 ? 0 : l > a.tokens ? a.tokens : l;
+    }
     float w[K][VEC], bias[VEC], window[K][VEC], g[K][VEC], dw[K][VEC], db[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
@@ -165,13 +184,14 @@ __global__ __launch_bounds__(256) void causal_conv_backward_kernel(const ConvArg
             dw[k][i] = g[k][i] = 0.f;
         }
     }
-    const int32_t t0 = p.segment * a.segment;
+    const int32_t t0 = live ? p.segment * a.segment : a.tokens;
     const int32_t t1 = a.tokens - t0 < a.segment ? a.tokens : t0 + a.segment;
     const int32_t te = p.len < t0 ? t0 : p.len < t1 ? p.len : t1;   // tokens of the sequence
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
         Vec<T, VEC> v;
-        conv_input<T, VEC, K>(a, p, t0 - (K - 1) + k, v);
+        if (live) conv_input<T, VEC, K>(a, p, t0 - (K - 1) + k, v);
+        else v.zero();
 #pragma unroll
         for (int i = 0; i < VEC; ++i) window[k + 1][i] = v[i];
     }
@@ -184,7 +204,7 @@ __global__ __launch_bounds__(256) void causal_conv_backward_kernel(const ConvArg
         ? static_cast<const T*>(a.dnew_state) + p.batch * (K - 1) * a.channels + p.channel : nullptr;
     // The input s = t - (K - 1) is complete once g[t] is known.  Segment 0 begins with the
     // state's inputs, the others with the first input of their own.
-    const bool own = te > t0 || p.segment == 0;
+    const bool own = live && (te > t0 || p.segment == 0);
     const int32_t s0 = p.segment == 0 ? -(K - 1) : t0;
     const int32_t stop = own ? te + K - 1 : t0;
     for (int32_t t = t0; t < stop; t += BROWS) {
@@ -247,11 +267,20 @@ __global__ __launch_bounds__(256) void causal_conv_backward_kernel(const ConvArg
     Vec<T, VEC> none;
     none.zero();
     for (int32_t t = te; t < t1; ++t) none.store(dx + static_cast<int64_t>(t) * a.channels);
-    float* to = a.partial + (p.batch * a.segments + p.segment) * (K + 1) * a.channels + p.channel;
 #pragma unroll
     for (int k = 0; k <= K; ++k)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) to[static_cast<int64_t>(k) * a.channels + i] = k < K ? dw[k][i] : db[i];
+        for (int i = 0; i < VEC; ++i) sums[row][k][column * VEC + i] = k < K ? dw[k][i] : db[i];
+    __syncthreads();
+    float* to = a.partial + (p.batch * a.strips + strip) * (K + 1) * a.channels;
+    const int32_t first = (static_cast<int32_t>(blockIdx.x - rest * across) * 16) * VEC;
+    for (int32_t v = threadIdx.x; v < (K + 1) * 16 * VEC; v += 256) {
+        const int32_t k = v / (16 * VEC), c = v % (16 * VEC);
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < SEGMENTS; ++r) sum += sums[r][k][c];
+        if (first + c < a.channels) to[static_cast<int64_t>(k) * a.channels + first + c] = sum;
+    }
 }
 
 // One token a sequence: the window is the state and the token.  A thread reads all of its
@@ -282,10 +311,11 @@ __global__ __launch_bounds__(256) void causal_conv_step_kernel(const ConvArgs a)
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tokens a thread takes: the work is cut until about 8 waves a SIMD (1024 SIMDs) have some,
-// down to 16 tokens (the K - 1 inputs before a segment are read twice).
-int64_t segment_tokens(int64_t B, int64_t N, int64_t groups) {
-    const int64_t wanted = 8192 * 64;
+// Tokens a thread takes: the work is cut until about `waves` waves a SIMD (1024 SIMDs) have
+// some, down to 16 tokens (the K - 1 inputs before a segment are read twice).
+constexpr int64_t FORWARD_WAVES = 8, BACKWARD_WAVES = 4;
+int64_t segment_tokens(int64_t B, int64_t N, int64_t groups, int64_t waves) {
+    const int64_t wanted = waves * 1024 * 64;
     int64_t segments = wanted / (B * groups);
     if (segments < 1) segments = 1;
     int64_t tokens = ceil_div(ceil_div(N, segments), ROWS) * ROWS;
@@ -313,7 +343,7 @@ enum Kind { FORWARD, BACKWARD, STEP };
 
 template <typename T, int VEC, int K>
 int launch(Kind kind, const ConvArgs& a, hipStream_t s) {
-    const int64_t blocks = ceil_div(a.threads, 256);
+    const int64_t blocks = kind == BACKWARD ? a.threads / 256 : ceil_div(a.threads, 256);
     VH_REQUIRE(blocks < (1ll << 24), VH_ERR_SHAPE, "causal convolution: too many sequences for one launch");
     const uint32_t grid = static_cast<uint32_t>(blocks);
     if (kind == FORWARD) causal_conv_kernel<T, VEC, K><<<grid, 256, 0, s>>>(a);
@@ -383,7 +413,7 @@ int vh_causal_conv_forward(const void* x, int64_t x_batch, int64_t x_token, int3
     a.channels = static_cast<int32_t>(C);
     const int e = dtype_bytes(io_dtype), vec = vec_of(C, e, 4 * e, {y, state, new_state}, {a});
     a.groups = static_cast<int32_t>(C / vec);
-    a.segment = static_cast<int32_t>(segment_tokens(B, N, a.groups));
+    a.segment = static_cast<int32_t>(segment_tokens(B, N, a.groups, FORWARD_WAVES));
     a.segments = static_cast<int32_t>(ceil_div(N, a.segment));
     a.threads = B * (a.segments + (new_state != nullptr ? 1 : 0)) * a.groups;
     return dispatch(FORWARD, a, io_dtype, vec, taps, static_cast<hipStream_t>(stream));
@@ -392,13 +422,14 @@ int vh_causal_conv_forward(const void* x, int64_t x_batch, int64_t x_token, int3
 size_t vh_causal_conv_backward_workspace_bytes(int64_t B, int64_t N, int64_t C, int32_t taps) {
     using namespace vh;
     if (B <= 0 || N <= 0 || C <= 0 || taps <= 0) return 0;
-    // with four channels a thread or with one: the more segments
-    const int64_t s4 = ceil_div(N, segment_tokens(B, N, C / 4 > 0 ? C / 4 : 1)), s1 = ceil_div(N, segment_tokens(B, N, C));
-    const int64_t rows = B * (s4 > s1 ? s4 : s1);
+    // with four channels a thread or with one
+    int64_t rows = 0;
     size_t sums = 0;
-    for (int64_t s : {s4, s1}) {
-        const size_t one = param_sum_workspace_bytes(B * s, taps + 1, C);
-        sums = one > sums ? one : sums;
+    for (int64_t groups : {C / 4 > 0 ? C / 4 : 1, C}) {
+        const int64_t one = B * ceil_div(ceil_div(N, segment_tokens(B, N, groups, BACKWARD_WAVES)), SEGMENTS);
+        const size_t bytes = param_sum_workspace_bytes(one, taps + 1, C);
+        rows = one > rows ? one : rows;
+        sums = bytes > sums ? bytes : sums;
     }
     return static_cast<size_t>(rows) * (taps + 1) * C * sizeof(float) + sums;
 }
@@ -434,18 +465,19 @@ int vh_causal_conv_backward(const void* dy, int64_t dy_batch, int64_t dy_token, 
     a.channels = static_cast<int32_t>(C);
     const int e = dtype_bytes(io_dtype), vec = vec_of(C, e, 4 * e, {dx, state, dstate, dnew_state}, {a});
     a.groups = static_cast<int32_t>(C / vec);
-    a.segment = static_cast<int32_t>(segment_tokens(B, N, a.groups));
+    a.segment = static_cast<int32_t>(segment_tokens(B, N, a.groups, BACKWARD_WAVES));
     a.segments = static_cast<int32_t>(ceil_div(N, a.segment));
-    a.threads = B * a.segments * a.groups;
+    a.strips = static_cast<int32_t>(ceil_div(a.segments, SEGMENTS));
+    a.threads = B * a.strips * ceil_div(a.groups, 16) * 256;
     a.partial = static_cast<float*>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (int rc = dispatch(BACKWARD, a, io_dtype, vec, taps, s)) return rc;
     ParamSum sum{};
     sum.partial = a.partial;
-    sum.rows = B * a.segments;
+    sum.rows = B * a.strips;
     sum.quantities = taps + 1;
     sum.columns = static_cast<int32_t>(C);
-    sum.per_channel = taps;
+    sum.per_channel = sum.padded = taps;
     sum.out0 = dweight;
     sum.out1 = dbias;
     return launch_param_sum(sum, a.partial + sum.rows * (taps + 1) * C, s);

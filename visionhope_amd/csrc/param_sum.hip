@@ -51,18 +51,18 @@ __global__ __launch_bounds__(64 * WAVES) void param_sum_kernel(ParamSum p, int64
     }
     if (q < p.per_channel) {
         if (p.out0 != nullptr) p.out0[static_cast<int64_t>(channel) * p.per_channel + q] = sum;
-    } else {
-        float* out = q == p.per_channel ? p.out1 : p.out2;
+    } else if (q >= p.padded) {
+        float* out = q == p.padded ? p.out1 : p.out2;
         if (out != nullptr) out[channel] = sum;
     }
 }
 
 // Workgroups that the rows of a 64-column strip are split over: about 512 in all, at least
-// 64 rows each.
+// 256 rows each (16 loads a wave; a second launch costs as much as some 300 rows more).
 int64_t splits(int64_t rows, int64_t width) {
     const int64_t strips = (width + 63) / 64;
     int64_t s = 512 / strips;
-    if (s > rows / 64) s = rows / 64;
+    if (s > rows / 256) s = rows / 256;
     return s < 2 ? 1 : s;
 }
 

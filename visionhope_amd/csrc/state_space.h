@@ -31,6 +31,7 @@ struct SSArgs {
     float* slots;    // [B, chunks - 1, S, padded C]: states (or adjoints) between the chunks
     float* sums;     // [B, chunks, padded C]: sum of dt over a chunk
     int32_t softplus;
+    int32_t states;   // of a channel as the tensors hold them; the kernels' S is the padded count
     int32_t batches, tokens, channels, group_channels, group_tiles, tiles;   // tiles: of 64 channels, all groups
     int32_t groups, chunk, chunks, first_chunk, launch_chunks, blocks;
     // backward
@@ -136,12 +137,41 @@ __device__ __forceinline__ float ss_softplus(float v) {
 
 inline int64_t ss_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// A channel's decay rates times log2(e), zero for the padding (whose states stay zero, as B and
+// C are zero there).
+template <int S>
+__device__ __forceinline__ void ss_rates(const SSArgs& a, int32_t channel, float (&A2)[S]) {
+    const float* from = a.A + static_cast<int64_t>(channel) * a.states;
+    if (a.states == S && (reinterpret_cast<uintptr_t>(a.A) & 15) == 0) {
+#pragma unroll
+        for (int n = 0; n < S; n += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(from + n);
+            A2[n] = v.x; A2[n + 1] = v.y; A2[n + 2] = v.z; A2[n + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < S; ++n) A2[n] = n < a.states ? from[n] : 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < S; ++n) A2[n] *= SS_LOG2E;
+}
+
+// State count that the kernels are built for.
+inline int32_t ss_padded(int32_t states) { return states <= 8 ? 8 : states <= 16 ? 16 : 32; }
+
 // Argument checks and the geometry common to forward and backward.
-int ss_fill(SSArgs& a, int32_t io_dtype, int32_t bc_dtype, int64_t B, int64_t N, int64_t C, int32_t groups,
-            int32_t states);
+int ss_fill(SSArgs& a, int32_t io_dtype, int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states);
+
+// B and C as the kernels read them: where they stand (*bc_dtype the activations') if the states
+// need no padding and every row is whole words of FP32 or bf16, otherwise as padded FP32 rows
+// that this packs into `maps` (ss_maps_floats of them, always set aside).
+inline int64_t ss_maps_floats(int64_t B, int64_t N, int32_t groups, int32_t states) {
+    return 2 * B * N * groups * ss_padded(states);
+}
+int ss_maps(SSArgs& a, int32_t io_dtype, float* maps, int32_t* bc_dtype, hipStream_t stream);
 
 // States (forward) or adjoints (backward) at the chunk boundaries from the chunks' own ones:
 // slots [B, chunks - 1, S, padded C] in place, one chunk after the other.
-int ss_join(const SSArgs& a, int64_t B, int32_t states, bool backward, const float* edge, hipStream_t stream);
+int ss_join(const SSArgs& a, int64_t B, int32_t padded, bool backward, const float* edge, hipStream_t stream);
 
 }  // namespace vh

@@ -20,8 +20,7 @@ __global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
     const SSPlace p = ss_place(a);
     const int64_t cp = static_cast<int64_t>(a.tiles) * 64;
     float A2[S], h[S];
-#pragma unroll
-    for (int n = 0; n < S; ++n) A2[n] = a.A[static_cast<int64_t>(p.channel) * S + n] * SS_LOG2E;
+    ss_rates<S>(a, p.channel, A2);
     const float bias = a.dt_bias != nullptr ? a.dt_bias[p.channel] : 0.f;
     const float D = OUT && a.D != nullptr ? a.D[p.channel] : 0.f;
     if (OUT && p.chunk > 0) {
@@ -29,9 +28,9 @@ __global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
 #pragma unroll
         for (int n = 0; n < S; ++n) h[n] = from[n * cp];
     } else if (OUT && a.state != nullptr) {
-        const float* from = a.state + (static_cast<int64_t>(p.batch) * a.channels + p.channel) * S;
+        const float* from = a.state + (static_cast<int64_t>(p.batch) * a.channels + p.channel) * a.states;
 #pragma unroll
-        for (int n = 0; n < S; ++n) h[n] = from[n];
+        for (int n = 0; n < S; ++n) h[n] = n < a.states ? from[n] : 0.f;
     } else {
 #pragma unroll
         for (int n = 0; n < S; ++n) h[n] = 0.f;
@@ -115,10 +114,10 @@ __global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
         for (t = count; t < p.t1 - p.t0; ++t)   // behind the sequence's end
             store_at<T>(a.y, out0 + static_cast<int64_t>(t) * a.channels, lane_at, 0.f);
         if (a.new_state != nullptr && p.chunk == a.chunks - 1) {
-            float* to = a.new_state + (static_cast<int64_t>(p.batch) * a.channels + p.channel) * S;
+            float* to = a.new_state + (static_cast<int64_t>(p.batch) * a.channels + p.channel) * a.states;
 #pragma unroll
-            for (int n = 0; n < S; n += 4)
-                *reinterpret_cast<float4*>(to + n) = make_float4(h[n], h[n + 1], h[n + 2], h[n + 3]);
+            for (int n = 0; n < S; ++n)
+                if (n < a.states) to[n] = h[n];
         }
     } else {
         float* to = a.slots + (static_cast<int64_t>(p.batch) * (a.chunks - 1) + p.chunk) * S * cp + p.column;
@@ -134,21 +133,22 @@ __global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
 // a zero adjoint behind it and becomes the whole one; the order is reversed and the decay is
 // that of chunk k + 1.  A workgroup takes one state of 64 channels, its waves ranges of the
 // chunks: each folds its range, the ranges' results go through LDS, and each walks its range
-// again from the value before it.
-__global__ void state_space_join_kernel(float* slots, const float* sums, const float* A, const float* edge,
-                                        int32_t S, int32_t channels, int32_t group_channels, int32_t group_tiles,
-                                        int32_t tiles, int32_t slots_n, int32_t backward) {
+// again from the value before it.  Ranges of up to JOIN slots stand in registers, so each slot
+// is read once, all at the same time.
+constexpr int JOIN = 16;
+__global__ __launch_bounds__(1024) void state_space_join_kernel(const SSArgs a, const float* edge, int32_t S,
+                                                                int32_t slots_n, int32_t backward) {
     __shared__ float fold_h[16][64], fold_p[16][64];
     const int32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int32_t tile = blockIdx.x % tiles, n = (blockIdx.x / tiles) % S;
-    const int64_t batch = blockIdx.x / (tiles * S);
-    const int32_t group = tile / group_tiles, in_group = (tile - group * group_tiles) * 64 + lane;
+    const int32_t tile = blockIdx.x % a.tiles, n = (blockIdx.x / a.tiles) % S;
+    const int64_t batch = blockIdx.x / (a.tiles * S);
+    const int32_t group = tile / a.group_tiles, in_group = (tile - group * a.group_tiles) * 64 + lane;
     // lanes without a channel carry the group's last one, as in the other passes
-    const int32_t channel = group * group_channels + (in_group < group_channels ? in_group : group_channels - 1);
-    const int64_t cp = static_cast<int64_t>(tiles) * 64, column = static_cast<int64_t>(tile) * 64 + lane;
-    const float A2 = A[static_cast<int64_t>(channel) * S + n] * SS_LOG2E;
-    float* slot = slots + (batch * slots_n * S + n) * cp + column;
-    const float* sum = sums + batch * (slots_n + 1) * cp + column;
+    const int32_t channel = group * a.group_channels + (in_group < a.group_channels ? in_group : a.group_channels - 1);
+    const int64_t cp = static_cast<int64_t>(a.tiles) * 64, column = static_cast<int64_t>(tile) * 64 + lane;
+    const float A2 = n < a.states ? a.A[static_cast<int64_t>(channel) * a.states + n] * SS_LOG2E : 0.f;
+    float* slot = a.slots + (batch * slots_n * S + n) * cp + column;
+    const float* sum = a.sums + batch * (slots_n + 1) * cp + column;
     const int32_t per = (slots_n + waves - 1) / waves;
     const int32_t i0 = wave * per, i1 = i0 + per < slots_n ? i0 + per : slots_n;
     // step i of the walk touches this slot, with the decay of this chunk
@@ -156,25 +156,56 @@ __global__ void state_space_join_kernel(float* slots, const float* sums, const f
     auto chunk_of = [&](int32_t i) { return backward ? slots_n - i : i; };
     // exp(A sum) h, and nothing from an empty state even where the decay (A > 0) overflows
     auto decayed = [&](float p, float h) { return h == 0.f ? 0.f : h * __builtin_amdgcn_exp2f(A2 * p); };
-    float h = 0.f, ps = 0.f;
+    float v[JOIN], p[JOIN];
+    auto read = [&](int32_t from) {   // steps outside the range change nothing
+#pragma unroll
+        for (int i = 0; i < JOIN; ++i) {
+            const bool in = from + i < i1;
+            v[i] = in ? slot[static_cast<int64_t>(slot_of(from + i)) * S * cp] : 0.f;
+            p[i] = in ? sum[chunk_of(from + i) * cp] : 0.f;
+        }
+    };
+    read(i0);
+    float h = 0.f;
     if (waves > 1) {
-#pragma unroll 8
-        for (int32_t i = i0; i < i1; ++i) {
-            const float p = sum[chunk_of(i) * cp], v = slot[static_cast<int64_t>(slot_of(i)) * S * cp];
-            h = decayed(p, h) + v;
-            ps += p;
+        float ps = 0.f;
+        for (int32_t from = i0; from < i1; from += JOIN) {
+            if (from != i0) read(from);
+#pragma unroll
+            for (int i = 0; i < JOIN; ++i) {
+                h = decayed(p[i], h) + v[i];
+                ps += p[i];
+            }
         }
         fold_h[wave][lane] = h;
         fold_p[wave][lane] = ps;
         __syncthreads();
     }
-    h = edge != nullptr ? edge[(batch * channels + channel) * S + n] : 0.f;
+    h = edge != nullptr && n < a.states ? edge[(batch * a.channels + channel) * a.states + n] : 0.f;
     for (int32_t w = 0; w < wave; ++w) h = decayed(fold_p[w][lane], h) + fold_h[w][lane];
-#pragma unroll 8
-    for (int32_t i = i0; i < i1; ++i) {
-        float* at = slot + static_cast<int64_t>(slot_of(i)) * S * cp;
-        h = decayed(sum[chunk_of(i) * cp], h) + *at;
-        *at = h;
+    for (int32_t from = i0; from < i1; from += JOIN) {
+        if (per > JOIN) read(from);
+#pragma unroll
+        for (int i = 0; i < JOIN; ++i) {
+            h = decayed(p[i], h) + v[i];
+            if (from + i < i1) slot[static_cast<int64_t>(slot_of(from + i)) * S * cp] = h;
+        }
+    }
+}
+
+// B and C as FP32 rows of the padded state count, zero in the padding.
+template <typename T>
+__global__ __launch_bounds__(256) void state_space_maps_kernel(const SSTokens b, const SSTokens c, float* to,
+                                                               int64_t tokens, int64_t rows, int32_t groups,
+                                                               int32_t states, int32_t S) {
+    const int64_t total = 2 * rows * groups * S;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * 256) {
+        const bool second = i >= total / 2;
+        const int64_t k = second ? i - total / 2 : i, n = k % S, rest = k / S;   // S is 8, 16 or 32
+        const int64_t row = rest / groups, group = rest - row * groups, batch = row / tokens, t = row - batch * tokens;
+        const SSTokens& from = second ? c : b;
+        to[i] = n < states ? to_f32(static_cast<const T*>(from.data)[batch * from.bs + t * from.ts + group * states + n]) : 0.f;
     }
 }
 
@@ -326,30 +357,20 @@ int check_sizes(int64_t B, int64_t N, int64_t C, int32_t groups) {
     return VH_OK;
 }
 
-int check_bc(const SSTokens& t, int32_t bc_dtype, const char* name) {
-    // the scalar unit reads whole words
-    const int64_t e = dtype_bytes(bc_dtype);
-    VH_REQUIRE(t.data != nullptr && reinterpret_cast<uintptr_t>(t.data) % 4 == 0 && t.bs * e % 4 == 0 &&
-                   t.ts * e % 4 == 0, VH_ERR_ARG, "%s must be given, its rows 4-byte aligned", name);
-    return VH_OK;
+// The scalar unit reads whole words.
+bool whole_words(const SSTokens& t, int64_t e) {
+    return reinterpret_cast<uintptr_t>(t.data) % 4 == 0 && t.bs * e % 4 == 0 && t.ts * e % 4 == 0;
 }
 
 }  // namespace
 
-int ss_fill(SSArgs& a, int32_t io_dtype, int32_t bc_dtype, int64_t B, int64_t N, int64_t C, int32_t groups,
-            int32_t states) {
+int ss_fill(SSArgs& a, int32_t io_dtype, int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
     VH_REQUIRE(valid_dtype(io_dtype), VH_ERR_DTYPE, "unsupported io_dtype %d", io_dtype);
-    VH_REQUIRE(bc_dtype == VH_DTYPE_F32 || (bc_dtype == VH_DTYPE_BF16 && io_dtype == VH_DTYPE_BF16), VH_ERR_DTYPE,
-               "B and C must be fp32, or bf16 with bf16 activations, got dtype %d", bc_dtype);
     if (int rc = check_sizes(B, N, C, groups)) return rc;
-    VH_REQUIRE(states == 8 || states == 16 || states == 32, VH_ERR_SHAPE, "states must be 8, 16 or 32, got %d", states);
-    VH_REQUIRE(a.A != nullptr && reinterpret_cast<uintptr_t>(a.A) % 16 == 0, VH_ERR_ARG,
-               "A must be given, 16-byte aligned");
-    VH_REQUIRE(a.x.data != nullptr && a.dt.data != nullptr, VH_ERR_ARG, "x and dt must not be null");
-    VH_REQUIRE(reinterpret_cast<uintptr_t>(a.state) % 16 == 0 && reinterpret_cast<uintptr_t>(a.new_state) % 16 == 0,
-               VH_ERR_ARG, "states must be 16-byte aligned");
-    if (int rc = check_bc(a.b, bc_dtype, "B")) return rc;
-    if (int rc = check_bc(a.c, bc_dtype, "C")) return rc;
+    VH_REQUIRE(states >= 1 && states <= 32, VH_ERR_SHAPE, "states must be 1 to 32, got %d", states);
+    VH_REQUIRE(a.x.data != nullptr && a.dt.data != nullptr && a.b.data != nullptr && a.c.data != nullptr &&
+                   a.A != nullptr, VH_ERR_ARG, "x, dt, B, C and A must not be null");
+    a.states = states;
     a.groups = groups;
     a.batches = static_cast<int32_t>(B);
     a.tokens = static_cast<int32_t>(N);
@@ -358,18 +379,39 @@ int ss_fill(SSArgs& a, int32_t io_dtype, int32_t bc_dtype, int64_t B, int64_t N,
     a.group_tiles = static_cast<int32_t>(ss_ceil(a.group_channels, 64));
     a.tiles = a.group_tiles * groups;
     a.blocks = static_cast<int32_t>(ss_ceil(N, SS_BLOCK));
-    // a launch has one wave for each tile of a chunk (8 tokens at least, and no more chunks than
-    // the aimed-at waves where there are that many sequences), and one for each state
+    // a launch has one wave for each tile of a chunk (no more chunks than the aimed-at waves
+    // where there are that many sequences), and one for each state
     VH_REQUIRE(B * a.tiles < (1ll << 24), VH_ERR_SHAPE,
                "state space scan: too many sequences and channels for one launch");
     return VH_OK;
 }
 
-int ss_join(const SSArgs& a, int64_t B, int32_t states, bool backward, const float* edge, hipStream_t stream) {
+int ss_maps(SSArgs& a, int32_t io_dtype, float* maps, int32_t* bc_dtype, hipStream_t stream) {
+    const int32_t S = ss_padded(a.states);
+    const int64_t e = dtype_bytes(io_dtype);
+    *bc_dtype = io_dtype;
+    if (io_dtype != VH_DTYPE_F16 && a.states == S && whole_words(a.b, e) && whole_words(a.c, e)) return VH_OK;
+    const int64_t rows = static_cast<int64_t>(a.batches) * a.tokens, total = 2 * rows * a.groups * S;
+    const int64_t blocks = ss_ceil(total, 256);
+    const uint32_t grid = static_cast<uint32_t>(blocks < 16384 ? blocks : 16384);
+    auto go = [&](auto t) {
+        state_space_maps_kernel<decltype(t)><<<grid, 256, 0, stream>>>(a.b, a.c, maps, a.tokens, rows, a.groups, a.states, S);
+    };
+    if (io_dtype == VH_DTYPE_F32) go(float{});
+    else if (io_dtype == VH_DTYPE_BF16) go(bf16_t{});
+    else go(f16_t{});
+    const int64_t row = static_cast<int64_t>(a.groups) * S;
+    a.b = {maps, a.tokens * row, row};
+    a.c = {maps + total / 2, a.tokens * row, row};
+    *bc_dtype = VH_DTYPE_F32;
+    return check_launch("state_space maps");
+}
+
+int ss_join(const SSArgs& a, int64_t B, int32_t padded, bool backward, const float* edge, hipStream_t stream) {
     const int32_t slots = a.chunks - 1;
-    const int32_t waves = slots >= 64 ? 16 : slots >= 16 ? 4 : 1;
-    state_space_join_kernel<<<static_cast<uint32_t>(B * states * a.tiles), 64 * waves, 0, stream>>>(
-        a.slots, a.sums, a.A, edge, states, a.channels, a.group_channels, a.group_tiles, a.tiles, slots, backward);
+    const int32_t waves = slots > 16 * JOIN ? 16 : (slots + JOIN - 1) / JOIN;
+    state_space_join_kernel<<<static_cast<uint32_t>(B * padded * a.tiles), 64 * waves, 0, stream>>>(a, edge, padded,
+                                                                                                slots, backward);
     return check_launch("state_space join");
 }
 
@@ -379,24 +421,25 @@ extern "C" {
 
 size_t vh_state_space_workspace_bytes(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
     using namespace vh;
-    if (B <= 0 || N <= 0 || C <= 0 || groups <= 0 || C % groups || states <= 0) return 0;
+    if (B <= 0 || N <= 0 || C <= 0 || groups <= 0 || C % groups || states <= 0 || states > 32) return 0;
     const int64_t tiles = ss_ceil(C / groups, 64) * groups;
     const int64_t chunks = ss_ceil(N, forward_chunk(B, N, tiles));
-    if (chunks < 2) return 0;
-    return static_cast<size_t>(B) * tiles * 64 * ((chunks - 1) * states + chunks) * sizeof(float);
+    int64_t floats = ss_maps_floats(B, N, groups, states);
+    if (chunks > 1) floats += B * tiles * 64 * ((chunks - 1) * ss_padded(states) + chunks);
+    return static_cast<size_t>(floats) * sizeof(float);
 }
 
 size_t vh_state_space_kept_bytes(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
     using namespace vh;
-    if (B <= 0 || N <= 0 || C <= 0 || groups <= 0 || C % groups || states <= 0) return 0;
-    return static_cast<size_t>(B) * ss_ceil(N, SS_BLOCK) * states * ss_ceil(C / groups, 64) * groups * 64 *
+    if (B <= 0 || N <= 0 || C <= 0 || groups <= 0 || C % groups || states <= 0 || states > 32) return 0;
+    return static_cast<size_t>(B) * ss_ceil(N, SS_BLOCK) * ss_padded(states) * ss_ceil(C / groups, 64) * groups * 64 *
            sizeof(float);
 }
 
 int vh_state_space_forward(
     const void* x, int64_t x_batch, int64_t x_token, const void* dt, int64_t dt_batch, int64_t dt_token,
     const void* gate, int64_t gate_batch, int64_t gate_token, int32_t io_dtype,
-    const void* b, int64_t b_batch, int64_t b_token, const void* c, int64_t c_batch, int64_t c_token, int32_t bc_dtype,
+    const void* b, int64_t b_batch, int64_t b_token, const void* c, int64_t c_batch, int64_t c_token,
     const float* A, const float* D, const float* dt_bias, int32_t softplus, const float* state,
     const int32_t* lengths, void* y, float* new_state, float* kept, int64_t B, int64_t N, int64_t C, int32_t groups,
     int32_t states, void* workspace, size_t workspace_bytes, void* stream) {
@@ -416,16 +459,20 @@ int vh_state_space_forward(
     a.y = y;
     a.new_state = new_state;
     a.kept = kept;
-    if (int rc = ss_fill(a, io_dtype, bc_dtype, B, N, C, groups, states)) return rc;
+    if (int rc = ss_fill(a, io_dtype, B, N, C, groups, states)) return rc;
     VH_REQUIRE(y != nullptr, VH_ERR_ARG, "y must not be null");
+    const int32_t S = ss_padded(states);
     a.chunk = static_cast<int32_t>(forward_chunk(B, N, a.tiles));
     a.chunks = static_cast<int32_t>(ss_ceil(N, a.chunk));
     const size_t need = vh_state_space_workspace_bytes(B, N, C, groups, states);
-    VH_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), VH_ERR_WORKSPACE,
+    VH_REQUIRE(workspace != nullptr && workspace_bytes >= need, VH_ERR_WORKSPACE,
                "state space scan needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
-    a.slots = static_cast<float*>(workspace);
-    a.sums = a.slots + static_cast<int64_t>(B) * (a.chunks - 1) * states * a.tiles * 64;
-    return dispatch_forward(io_dtype, bc_dtype, states, a, B, static_cast<hipStream_t>(stream));
+    float* maps = static_cast<float*>(workspace);
+    a.slots = maps + ss_maps_floats(B, N, groups, states);
+    a.sums = a.slots + static_cast<int64_t>(B) * (a.chunks - 1) * S * a.tiles * 64;
+    int32_t bc_dtype = 0;
+    if (int rc = ss_maps(a, io_dtype, maps, &bc_dtype, static_cast<hipStream_t>(stream))) return rc;
+    return dispatch_forward(io_dtype, bc_dtype, S, a, B, static_cast<hipStream_t>(stream));
 }
 
 int vh_state_space_step(

@@ -24,11 +24,9 @@ __global__ __launch_bounds__(64) void state_space_adjoint_kernel(const SSArgs a)
     const SSPlace p = ss_place(a);
     const int64_t cp = static_cast<int64_t>(a.tiles) * 64;
     float A2[S], carry[S];
+    ss_rates<S>(a, p.channel, A2);
 #pragma unroll
-    for (int n = 0; n < S; ++n) {
-        A2[n] = a.A[static_cast<int64_t>(p.channel) * S + n] * SS_LOG2E;
-        carry[n] = 0.f;
-    }
+    for (int n = 0; n < S; ++n) carry[n] = 0.f;
     const float bias = a.dt_bias != nullptr ? a.dt_bias[p.channel] : 0.f;
     const uint32_t lane_at = static_cast<uint32_t>(p.channel) * sizeof(T);
     const bool gated = a.gate.data != nullptr, soft = a.softplus != 0;
@@ -159,7 +157,8 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
     float A2[SPL], carry[SPL], dA[SPL];
 #pragma unroll
     for (int j = 0; j < SPL; ++j) {
-        A2[j] = a.A[static_cast<int64_t>(channel) * S + part * SPL + j] * SS_LOG2E;
+        const int32_t n = part * SPL + j;
+        A2[j] = n < a.states ? a.A[static_cast<int64_t>(channel) * a.states + n] * SS_LOG2E : 0.f;
         dA[j] = 0.f;
     }
     // the adjoint behind the chunk, times the decay of the token behind it
@@ -170,9 +169,10 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
         for (int j = 0; j < SPL; ++j) carry[j] = live ? from[j * cp] : 0.f;
     } else {
         const float* from = a.dnew_state != nullptr
-            ? a.dnew_state + (static_cast<int64_t>(batch) * a.channels + channel) * S + part * SPL : nullptr;
+            ? a.dnew_state + (static_cast<int64_t>(batch) * a.channels + channel) * a.states : nullptr;
 #pragma unroll
-        for (int j = 0; j < SPL; ++j) carry[j] = from != nullptr && live ? from[j] : 0.f;
+        for (int j = 0; j < SPL; ++j)
+            carry[j] = from != nullptr && live && part * SPL + j < a.states ? from[part * SPL + j] : 0.f;
     }
 
     // by token and channel
@@ -372,9 +372,10 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
 #pragma unroll
         for (int j = 0; j < SPL; ++j) to[(part * SPL + j) * cp + column] = dA[j];
         if (a.dstate != nullptr && chunk == 0) {
-            float* ds = a.dstate + (static_cast<int64_t>(batch) * a.channels + channel) * S + part * SPL;
+            float* ds = a.dstate + (static_cast<int64_t>(batch) * a.channels + channel) * a.states;
 #pragma unroll
-            for (int j = 0; j < SPL; ++j) ds[j] = carry[j];
+            for (int j = 0; j < SPL; ++j)
+                if (part * SPL + j < a.states) ds[part * SPL + j] = carry[j];
         }
     }
     // dD and dbias: the threads of a channel, in order
@@ -394,19 +395,34 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
     }
 }
 
-// dC and dB from the tiles' sums, tile after tile.
+// dC and dB from the tiles' sums, tile after tile, four values a thread (S a power of two).
 template <typename T>
 __global__ __launch_bounds__(256) void state_space_bc_kernel(const float* partial, T* db, T* dc, int64_t rows,
-                                                             int32_t S, int32_t groups, int32_t group_tiles) {
-    const int64_t width = 2 * S, total = rows * groups * width;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+                                                             int32_t S, int32_t states, int32_t groups,
+                                                             int32_t group_tiles) {
+    const int32_t quads = S / 2, lg = 31 - __builtin_clz(static_cast<uint32_t>(quads)), group = blockIdx.y;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < rows << lg;
          i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t in = i % width, group = (i / width) % groups, row = i / (width * groups);
-        const float* at = partial + (group * group_tiles * rows + row) * width + in;
-        float sum = 0.f;
-        for (int32_t k = 0; k < group_tiles; ++k) sum += at[k * rows * width];
-        T* out = in < S ? dc : db;
-        out[(row * groups + group) * S + (in < S ? in : in - S)] = from_f32<T>(sum);
+        const int64_t row = i >> lg;
+        const int32_t in = static_cast<int32_t>(i & (quads - 1)) * 4, n = in < S ? in : in - S;
+        const float* at = partial + (static_cast<int64_t>(group) * group_tiles * rows + row) * (2 * S) + in;
+        float4 sum = *reinterpret_cast<const float4*>(at);
+        for (int32_t k = 1; k < group_tiles; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(at + k * rows * (2 * S));
+            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        }
+        T* out = (in < S ? dc : db) + (row * groups + group) * states + n;
+        alignas(16) const T v[4] = {from_f32<T>(sum.x), from_f32<T>(sum.y), from_f32<T>(sum.z), from_f32<T>(sum.w)};
+        if (states % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (sizeof(v) - 1)) == 0) {
+            if (n < states) {
+                if constexpr (sizeof(v) == 16) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(v);
+                else *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(v);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n + j < states) out[j] = v[j];
+        }
     }
 }
 
@@ -441,18 +457,19 @@ Cut make_cut(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
 }
 
 struct Space {   // the workspace, in floats
-    int64_t slots, sums, bc, params, total_floats;
+    int64_t bc, slots, sums, params, maps, total_floats;   // bc first: it is read 16 bytes at a time
     size_t sum_bytes;
 };
-Space backward_space(const Cut& c, int64_t B, int64_t N, int32_t states) {
-    const int64_t cp = c.tiles * 64;
+Space backward_space(const Cut& c, int64_t B, int64_t N, int32_t groups, int32_t states) {
+    const int64_t cp = c.tiles * 64, S = ss_padded(states);
     Space s;
-    s.slots = 0;
-    s.sums = s.slots + B * (c.fine_chunks - 1) * states * cp;
-    s.bc = s.sums + B * c.fine_chunks * cp;
-    s.params = s.bc + c.wide_tiles * B * N * 2 * states;
-    s.total_floats = s.params + B * c.chunks * (states + 2) * cp;
-    s.sum_bytes = param_sum_workspace_bytes(B * c.chunks, states + 2, cp);
+    s.bc = 0;
+    s.slots = s.bc + c.wide_tiles * B * N * 2 * S;
+    s.sums = s.slots + B * (c.fine_chunks - 1) * S * cp;
+    s.params = s.sums + B * c.fine_chunks * cp;
+    s.maps = s.params + B * c.chunks * (S + 2) * cp;
+    s.total_floats = s.maps + ss_maps_floats(B, N, groups, states);
+    s.sum_bytes = param_sum_workspace_bytes(B * c.chunks, S + 2, cp);
     return s;
 }
 
@@ -483,9 +500,10 @@ int launch_states(SSArgs& a, const Cut& c, int64_t B, int32_t S, void* db, void*
     int rc = S == 8 ? launch_backward<T, BCT, 8>(a, c, B, s)
            : S == 16 ? launch_backward<T, BCT, 16>(a, c, B, s) : launch_backward<T, BCT, 32>(a, c, B, s);
     if (rc) return rc;
-    const int64_t rows = B * a.tokens, blocks = ss_ceil(rows * a.groups * 2 * S, 256);
-    state_space_bc_kernel<T><<<static_cast<uint32_t>(blocks < 65536 ? blocks : 65536), 256, 0, s>>>(
-        a.bc_partial, static_cast<T*>(db), static_cast<T*>(dc), rows, S, a.groups, a.wide_tiles / a.groups);
+    const int64_t rows = B * a.tokens, blocks = ss_ceil(rows * S / 2, 256);
+    const dim3 grid(static_cast<uint32_t>(blocks < 16384 ? blocks : 16384), a.groups);
+    state_space_bc_kernel<T><<<grid, 256, 0, s>>>(a.bc_partial, static_cast<T*>(db), static_cast<T*>(dc), rows, S,
+                                                  a.states, a.groups, a.wide_tiles / a.groups);
     return check_launch("state_space dB and dC");
 }
 
@@ -496,8 +514,8 @@ extern "C" {
 
 size_t vh_state_space_backward_workspace_bytes(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
     using namespace vh;
-    if (B <= 0 || N <= 0 || C <= 0 || groups <= 0 || C % groups || states <= 0) return 0;
-    const Space s = backward_space(make_cut(B, N, C, groups, states), B, N, states);
+    if (B <= 0 || N <= 0 || C <= 0 || groups <= 0 || C % groups || states <= 0 || states > 32) return 0;
+    const Space s = backward_space(make_cut(B, N, C, groups, states), B, N, groups, states);
     return static_cast<size_t>(s.total_floats) * sizeof(float) + s.sum_bytes;
 }
 
@@ -505,7 +523,7 @@ int vh_state_space_backward(
     const void* dy, int64_t dy_batch, int64_t dy_token, const void* x, int64_t x_batch, int64_t x_token,
     const void* dt, int64_t dt_batch, int64_t dt_token, const void* gate, int64_t gate_batch, int64_t gate_token,
     int32_t io_dtype, const void* b, int64_t b_batch, int64_t b_token, const void* c, int64_t c_batch, int64_t c_token,
-    int32_t bc_dtype, const float* A, const float* D, const float* dt_bias, int32_t softplus, const int32_t* lengths,
+    const float* A, const float* D, const float* dt_bias, int32_t softplus, const int32_t* lengths,
     const float* kept, const float* dnew_state, void* dx, void* ddt, void* dgate, void* db, void* dc, float* dA,
     float* dD, float* ddt_bias, float* dstate, int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states,
     void* workspace, size_t workspace_bytes, void* stream) {
@@ -528,32 +546,36 @@ int vh_state_space_backward(
     a.ddt = ddt;
     a.dgate = dgate;
     a.dstate = dstate;
-    if (int rc = ss_fill(a, io_dtype, bc_dtype, B, N, C, groups, states)) return rc;
+    if (int rc = ss_fill(a, io_dtype, B, N, C, groups, states)) return rc;
     VH_REQUIRE(dy != nullptr && kept != nullptr && dx != nullptr && ddt != nullptr && db != nullptr && dc != nullptr &&
                    (gate == nullptr) == (dgate == nullptr), VH_ERR_ARG,
                "dy, kept, dx, ddt, db and dc must be given, dgate exactly with a gate");
-    VH_REQUIRE(reinterpret_cast<uintptr_t>(dstate) % 16 == 0, VH_ERR_ARG, "dstate must be 16-byte aligned");
     const Cut cut = make_cut(B, N, C, groups, states);
-    const Space sp = backward_space(cut, B, N, states);
+    const Space sp = backward_space(cut, B, N, groups, states);
     const size_t need = static_cast<size_t>(sp.total_floats) * sizeof(float) + sp.sum_bytes;
-    VH_REQUIRE(workspace != nullptr && workspace_bytes >= need, VH_ERR_WORKSPACE,
-               "state space backward needs a workspace of %zu bytes, got %zu", need, workspace_bytes);
+    VH_REQUIRE(workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+               VH_ERR_WORKSPACE, "state space backward needs a 16-byte aligned workspace of %zu bytes, got %zu", need,
+               workspace_bytes);
     float* ws = static_cast<float*>(workspace);
     a.slots = ws + sp.slots;
     a.sums = ws + sp.sums;
     a.bc_partial = ws + sp.bc;
     a.param_partial = ws + sp.params;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    int rc;
-    if (io_dtype == VH_DTYPE_F32) rc = launch_states<float, float>(a, cut, B, states, db, dc, s);
-    else if (io_dtype == VH_DTYPE_F16) rc = launch_states<f16_t, float>(a, cut, B, states, db, dc, s);
-    else if (bc_dtype == VH_DTYPE_F32) rc = launch_states<bf16_t, float>(a, cut, B, states, db, dc, s);
-    else rc = launch_states<bf16_t, bf16_t>(a, cut, B, states, db, dc, s);
+    const int32_t S = ss_padded(states);
+    int32_t bc_dtype = 0;
+    int rc = ss_maps(a, io_dtype, ws + sp.maps, &bc_dtype, s);
+    if (rc) return rc;
+    if (io_dtype == VH_DTYPE_F32) rc = launch_states<float, float>(a, cut, B, S, db, dc, s);
+    else if (io_dtype == VH_DTYPE_F16) rc = launch_states<f16_t, float>(a, cut, B, S, db, dc, s);
+    else if (bc_dtype == VH_DTYPE_F32) rc = launch_states<bf16_t, float>(a, cut, B, S, db, dc, s);
+    else rc = launch_states<bf16_t, bf16_t>(a, cut, B, S, db, dc, s);
     if (rc) return rc;
     ParamSum sum{};
     sum.partial = a.param_partial;
     sum.rows = B * cut.chunks;
-    sum.quantities = states + 2;
+    sum.quantities = S + 2;
+    sum.padded = S;
     sum.columns = a.tiles * 64;
     sum.per_channel = states;
     sum.group_channels = a.group_channels;

@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from . import hip
 from .cuda import on_tensor_device
-from .token_lines import (check_io, check_like, check_param, dense_channels, fp32_param, line_lengths,
+from .token_lines import (address, check_io, check_like, check_param, dense_channels, fp32_param, line_lengths,
                           refuse_gradients)
 
 MAX_TAPS = 8
@@ -27,8 +27,8 @@ def _forward(x, weight, bias, silu, state, lengths, return_state):
     new_state = (torch.empty((batch, taps - 1, channels), device=x.device, dtype=x.dtype)
                  if return_state else None)
     hip.check(hip.load_library().vh_causal_conv_forward(
-        hip.ptr(x), x.stride(0), x.stride(1), hip.dtype_code(x.dtype), hip.ptr(weight), hip.ptr(bias), int(silu),
-        hip.ptr(state), hip.ptr(lengths), hip.ptr(y), hip.ptr(new_state), batch, length, channels, taps,
+        address(x), x.stride(0), x.stride(1), hip.dtype_code(x.dtype), address(weight), address(bias), int(silu),
+        address(state), address(lengths), address(y), address(new_state), batch, length, channels, taps,
         hip.stream_of(x)), "vh_causal_conv_forward")
     return y, new_state
 
@@ -70,9 +70,9 @@ class _CausalConvFunction(Function):
         lib = hip.load_library()
         ws = hip.workspace(lib.vh_causal_conv_backward_workspace_bytes(batch, length, channels, taps), x.device)
         hip.check(lib.vh_causal_conv_backward(
-            hip.ptr(dy), dy.stride(0), dy.stride(1), hip.ptr(x), x.stride(0), x.stride(1), hip.dtype_code(x.dtype),
-            hip.ptr(weight), hip.ptr(bias), int(ctx.silu), hip.ptr(state), hip.ptr(lengths), hip.ptr(dnew_state),
-            hip.ptr(dx), hip.ptr(dweight), hip.ptr(dbias), hip.ptr(dstate), batch, length, channels, taps, hip.ptr(ws),
+            address(dy), dy.stride(0), dy.stride(1), address(x), x.stride(0), x.stride(1), hip.dtype_code(x.dtype),
+            address(weight), address(bias), int(ctx.silu), address(state), address(lengths), address(dnew_state),
+            address(dx), address(dweight), address(dbias), address(dstate), batch, length, channels, taps, address(ws),
             ws.numel() * 4, hip.stream_of(x)), "vh_causal_conv_backward")
         if dweight is not None:
             dweight = dweight.view(ctx.weight_like[0]).to(ctx.weight_like[1])
@@ -147,6 +147,6 @@ def visionhope_causal_conv_step(x, state, weight, bias=None, *, silu=False, new_
     weight, bias = fp32_param(weight).reshape(channels, -1), fp32_param(bias)
     y = torch.empty((batch, channels), device=x.device, dtype=x.dtype)
     hip.check(hip.load_library().vh_causal_conv_step(
-        hip.ptr(x), x.stride(0), hip.dtype_code(x.dtype), hip.ptr(weight), hip.ptr(bias), int(silu), hip.ptr(state),
-        hip.ptr(new_state), hip.ptr(y), batch, channels, taps, hip.stream_of(x)), "vh_causal_conv_step")
+        address(x), x.stride(0), hip.dtype_code(x.dtype), address(weight), address(bias), int(silu), address(state),
+        address(new_state), address(y), batch, channels, taps, hip.stream_of(x)), "vh_causal_conv_step")
     return y

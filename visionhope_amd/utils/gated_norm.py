@@ -13,7 +13,7 @@ from torch.autograd.function import once_differentiable
 
 from . import hip
 from .cuda import on_tensor_device
-from .token_lines import IO_DTYPES, check_like, check_param, fp32_param
+from .token_lines import IO_DTYPES, address, check_like, check_param, fp32_param
 
 MAX_CHANNELS = 8192
 
@@ -53,8 +53,8 @@ def _forward(x, weight, bias, gate, eps, keep):
     if keep:
         mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32).unbind(0)
     hip.check(hip.load_library().vh_gated_layernorm_forward(
-        hip.ptr(x), x_row, hip.ptr(gate), gate_row, hip.dtype_code(x.dtype), hip.ptr(weight), hip.ptr(bias),
-        hip.ptr(y), hip.ptr(mean), hip.ptr(rstd), rows, channels, float(eps), hip.stream_of(x)),
+        address(x), x_row, address(gate), gate_row, hip.dtype_code(x.dtype), address(weight), address(bias),
+        address(y), address(mean), address(rstd), rows, channels, float(eps), hip.stream_of(x)),
         "vh_gated_layernorm_forward")
     return y, mean, rstd
 
@@ -92,9 +92,9 @@ class _GatedLayerNormFunction(Function):
         lib = hip.load_library()
         ws = hip.workspace(lib.vh_gated_layernorm_backward_workspace_bytes(rows, channels), x.device)
         hip.check(lib.vh_gated_layernorm_backward(
-            hip.ptr(dy), dy_row, hip.ptr(x), x_row, hip.ptr(gate), gate_row, hip.dtype_code(x.dtype), hip.ptr(weight),
-            hip.ptr(bias), hip.ptr(mean), hip.ptr(rstd), hip.ptr(dx), hip.ptr(dgate), hip.ptr(dweight), hip.ptr(dbias),
-            rows, channels, hip.ptr(ws), ws.numel() * 4, hip.stream_of(x)), "vh_gated_layernorm_backward")
+            address(dy), dy_row, address(x), x_row, address(gate), gate_row, hip.dtype_code(x.dtype), address(weight),
+            address(bias), address(mean), address(rstd), address(dx), address(dgate), address(dweight), address(dbias),
+            rows, channels, address(ws), ws.numel() * 4, hip.stream_of(x)), "vh_gated_layernorm_backward")
         return (dx, dweight.to(ctx.param_dtypes[0]) if need[1] else None,
                 dbias.to(ctx.param_dtypes[1]) if need[2] else None, dgate, None)
 

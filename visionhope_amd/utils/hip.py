@@ -166,12 +166,12 @@ _SIGNATURES = {
     "vh_state_space_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
     "vh_state_space_kept_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
     "vh_state_space_forward": (ctypes.c_int, [
-        _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i32,
+        _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64,
         _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _sz, _vp]),
     "vh_state_space_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
     "vh_state_space_backward": (ctypes.c_int, [
         _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64,
-        _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+        _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
         _i64, _i64, _i64, _i32, _i32, _vp, _sz, _vp]),
     "vh_state_space_step": (ctypes.c_int, [
         _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _vp,

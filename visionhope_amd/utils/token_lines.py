@@ -58,8 +58,20 @@ def dense_channels(t):
 
 
 def fp32_param(t):
-    """A parameter as the kernels read it: FP32, dense, without autograd."""
-    return None if t is None else t.detach().float().contiguous()
+    """A parameter as the kernels read it: FP32, dense."""
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().float().contiguous()
+
+
+def address(t):
+    """A native pointer argument (an int: cheaper to pass than a ctypes object), or None."""
+    return None if t is None else t.data_ptr()
+
+
+def rows_of(t):
+    """Native arguments of a token tensor: address and element strides of sequence and token."""
+    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
 
 
 def refuse_gradients(name, *tensors):
