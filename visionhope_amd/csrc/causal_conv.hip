@@ -4,7 +4,7 @@
 //   y[t, c] = f(bias[c] + sum_k weight[c, k] x[t - K + 1 + k, c]),  f = identity or SiLU
 //
 // with the K - 1 inputs before the first token from a state (zero without one).  A thread
-// takes 16 bytes of channels (one channel where the sizes or alignments ask for it) and a
+// takes four channels (one where the sizes or alignments ask for it) and a
 // segment of tokens with the window in registers, so every input is read once but for the
 // K - 1 inputs before each segment.  Bound by the bytes of x and y.
 #include "param_sum.h"
@@ -82,7 +82,7 @@ __device__ __forceinline__ void conv_input(const ConvArgs& a, const ConvPlace& p
     }
 }
 
-constexpr int ROWS = 8;   // tokens loaded together
+constexpr int ROWS = 4;   // tokens loaded together
 
 template <typename T, int VEC, int K>
 __global__ __launch_bounds__(256) void causal_conv_kernel(const ConvArgs a) {
@@ -311,15 +311,22 @@ __global__ __launch_bounds__(256) void causal_conv_step_kernel(const ConvArgs a)
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tokens a thread takes: the work is cut until about `waves` waves a SIMD (1024 SIMDs) have
-// some, down to 16 tokens (the K - 1 inputs before a segment are read twice).
-constexpr int64_t FORWARD_WAVES = 8, BACKWARD_WAVES = 4;
-int64_t segment_tokens(int64_t B, int64_t N, int64_t groups, int64_t waves) {
-    const int64_t wanted = waves * 1024 * 64;
+// Tokens a thread of the forward takes: the work is cut until about 8 waves a SIMD (1024
+// SIMDs) have some, down to 16 tokens (the K - 1 inputs before a segment are read twice).
+int64_t segment_tokens(int64_t B, int64_t N, int64_t groups) {
+    const int64_t wanted = 8 * 1024 * 64;
     int64_t segments = wanted / (B * groups);
     if (segments < 1) segments = 1;
     int64_t tokens = ceil_div(ceil_div(N, segments), ROWS) * ROWS;
     return tokens < 16 ? 16 : tokens > 256 ? 256 : tokens;
+}
+
+// Strips (16 segments each) that the backward cuts a line into: about three waves a SIMD, what
+// its registers hold, of segments of at least 16 tokens.
+int64_t strip_count(int64_t B, int64_t N, int64_t groups) {
+    int64_t strips = 3 * 1024 / 4 / (B * ceil_div(groups, 16));
+    if (strips > ceil_div(N, 16 * SEGMENTS)) strips = ceil_div(N, 16 * SEGMENTS);
+    return strips < 1 ? 1 : strips;
 }
 
 // Widest access of at most `most` elements that all addresses and strides allow.
@@ -363,7 +370,8 @@ int launch_taps(Kind kind, const ConvArgs& a, int taps, hipStream_t s) {
         default: return launch<T, VEC, 8>(kind, a, s);
     }
 }
-// vec: 1, or elements of `bytes` bytes.
+// vec: channels a thread, 4 or 1.  (Eight of a 16-bit type a thread, 16 bytes, were slower:
+// 21.2 us against 18.8 at 32 x 3136 x 192 bf16, fewer waves with more registers each.)
 int dispatch(Kind kind, const ConvArgs& a, int32_t io, int vec, int taps, hipStream_t s) {
     if (io == VH_DTYPE_F32) {
         if (vec == 4) return launch_taps<float, 4>(kind, a, taps, s);
@@ -413,7 +421,7 @@ int vh_causal_conv_forward(const void* x, int64_t x_batch, int64_t x_token, int3
     a.channels = static_cast<int32_t>(C);
     const int e = dtype_bytes(io_dtype), vec = vec_of(C, e, 4 * e, {y, state, new_state}, {a});
     a.groups = static_cast<int32_t>(C / vec);
-    a.segment = static_cast<int32_t>(segment_tokens(B, N, a.groups, FORWARD_WAVES));
+    a.segment = static_cast<int32_t>(segment_tokens(B, N, a.groups));
     a.segments = static_cast<int32_t>(ceil_div(N, a.segment));
     a.threads = B * (a.segments + (new_state != nullptr ? 1 : 0)) * a.groups;
     return dispatch(FORWARD, a, io_dtype, vec, taps, static_cast<hipStream_t>(stream));
@@ -426,7 +434,7 @@ size_t vh_causal_conv_backward_workspace_bytes(int64_t B, int64_t N, int64_t C, 
     int64_t rows = 0;
     size_t sums = 0;
     for (int64_t groups : {C / 4 > 0 ? C / 4 : 1, C}) {
-        const int64_t one = B * ceil_div(ceil_div(N, segment_tokens(B, N, groups, BACKWARD_WAVES)), SEGMENTS);
+        const int64_t one = B * strip_count(B, N, groups);
         const size_t bytes = param_sum_workspace_bytes(one, taps + 1, C);
         rows = one > rows ? one : rows;
         sums = bytes > sums ? bytes : sums;
@@ -465,9 +473,10 @@ int vh_causal_conv_backward(const void* dy, int64_t dy_batch, int64_t dy_token, 
     a.channels = static_cast<int32_t>(C);
     const int e = dtype_bytes(io_dtype), vec = vec_of(C, e, 4 * e, {dx, state, dstate, dnew_state}, {a});
     a.groups = static_cast<int32_t>(C / vec);
-    a.segment = static_cast<int32_t>(segment_tokens(B, N, a.groups, BACKWARD_WAVES));
+    a.strips = static_cast<int32_t>(strip_count(B, N, a.groups));
+    // whole loads of four tokens
+    a.segment = static_cast<int32_t>(ceil_div(ceil_div(N, a.strips * SEGMENTS), 4) * 4);
     a.segments = static_cast<int32_t>(ceil_div(N, a.segment));
-    a.strips = static_cast<int32_t>(ceil_div(a.segments, SEGMENTS));
     a.threads = B * a.strips * ceil_div(a.groups, 16) * 256;
     a.partial = static_cast<float*>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);

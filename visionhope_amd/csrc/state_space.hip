@@ -133,62 +133,76 @@ __global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
 // a zero adjoint behind it and becomes the whole one; the order is reversed and the decay is
 // that of chunk k + 1.  A workgroup takes one state of 64 channels, its waves ranges of the
 // chunks: each folds its range, the ranges' results go through LDS, and each walks its range
-// again from the value before it.  Ranges of up to JOIN slots stand in registers, so each slot
-// is read once, all at the same time.
-constexpr int JOIN = 16;
+// again from the value before it.  Ranges of up to JOIN slots stand in registers and are read
+// once.  The launch is short, so its time is that of fetching its code: both walks share the
+// loop's.
+constexpr int JOIN = 8;
 __global__ __launch_bounds__(1024) void state_space_join_kernel(const SSArgs a, const float* edge, int32_t S,
                                                                 int32_t slots_n, int32_t backward) {
     __shared__ float fold_h[16][64], fold_p[16][64];
-    const int32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int32_t tile = blockIdx.x % a.tiles, n = (blockIdx.x / a.tiles) % S;
-    const int64_t batch = blockIdx.x / (a.tiles * S);
+    const int32_t lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const int32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int32_t rest = blockIdx.x / a.tiles, tile = blockIdx.x - rest * a.tiles;
+    const int32_t batch = rest / S, n = rest - batch * S;
     const int32_t group = tile / a.group_tiles, in_group = (tile - group * a.group_tiles) * 64 + lane;
     // lanes without a channel carry the group's last one, as in the other passes
     const int32_t channel = group * a.group_channels + (in_group < a.group_channels ? in_group : a.group_channels - 1);
-    const int64_t cp = static_cast<int64_t>(a.tiles) * 64, column = static_cast<int64_t>(tile) * 64 + lane;
+    const int64_t cp = static_cast<int64_t>(a.tiles) * 64;
     const float A2 = n < a.states ? a.A[static_cast<int64_t>(channel) * a.states + n] * SS_LOG2E : 0.f;
-    float* slot = a.slots + (batch * slots_n * S + n) * cp + column;
-    const float* sum = a.sums + batch * (slots_n + 1) * cp + column;
     const int32_t per = (slots_n + waves - 1) / waves;
     const int32_t i0 = wave * per, i1 = i0 + per < slots_n ? i0 + per : slots_n;
-    // step i of the walk touches this slot, with the decay of this chunk
-    auto slot_of = [&](int32_t i) { return backward ? slots_n - 1 - i : i; };
-    auto chunk_of = [&](int32_t i) { return backward ? slots_n - i : i; };
+    // Step i touches slot i with the decay of chunk i, or slot slots_n - 1 - i with that of chunk
+    // slots_n - i.  Uniform addresses; the lanes follow each other from there.
+    const int32_t first = i0 < slots_n ? i0 : slots_n - 1;
+    float* slot0 = a.slots + ((static_cast<int64_t>(batch) * slots_n + (backward ? slots_n - 1 - first : first)) * S + n) * cp +
+                   static_cast<int64_t>(tile) * 64;
+    const float* sum0 = a.sums + (static_cast<int64_t>(batch) * (slots_n + 1) + (backward ? slots_n - first : first)) * cp +
+                        static_cast<int64_t>(tile) * 64;
+    const int64_t slot_step = backward ? -S * cp : S * cp, sum_step = backward ? -cp : cp;
+    const uint32_t lane_at = lane * sizeof(float);
     // exp(A sum) h, and nothing from an empty state even where the decay (A > 0) overflows
     auto decayed = [&](float p, float h) { return h == 0.f ? 0.f : h * __builtin_amdgcn_exp2f(A2 * p); };
-    float v[JOIN], p[JOIN];
-    auto read = [&](int32_t from) {   // steps outside the range change nothing
-#pragma unroll
-        for (int i = 0; i < JOIN; ++i) {
-            const bool in = from + i < i1;
-            v[i] = in ? slot[static_cast<int64_t>(slot_of(from + i)) * S * cp] : 0.f;
-            p[i] = in ? sum[chunk_of(from + i) * cp] : 0.f;
+    float v[JOIN], p[JOIN], h = 0.f, ps = 0.f;
+    const int32_t first_walk = waves > 1 ? 0 : 1;
+#pragma nounroll
+    for (int32_t walk = first_walk; walk < 2; ++walk) {
+        if (walk == 1) {
+            if (waves > 1) {
+                fold_h[wave][lane] = h;
+                fold_p[wave][lane] = ps;
+                __syncthreads();
+            }
+            h = edge != nullptr && n < a.states
+                ? edge[(static_cast<int64_t>(batch) * a.channels + channel) * a.states + n] : 0.f;
+#pragma nounroll
+            for (int32_t w = 0; w < wave; ++w) h = decayed(fold_p[w][lane], h) + fold_h[w][lane];
         }
-    };
-    read(i0);
-    float h = 0.f;
-    if (waves > 1) {
-        float ps = 0.f;
+        float* slot = slot0;
+        const float* sum = sum0;
+#pragma nounroll
         for (int32_t from = i0; from < i1; from += JOIN) {
-            if (from != i0) read(from);
+            if (walk == first_walk || per > JOIN) {
+                const float* at = slot;
+                const float* sat = sum;
+#pragma unroll
+                for (int i = 0; i < JOIN; ++i) {   // steps behind the range read its last slot and change nothing
+                    const bool in = from + i < i1;
+                    v[i] = load_at(at, lane_at);
+                    p[i] = load_at(sat, lane_at);
+                    v[i] = in ? v[i] : 0.f;
+                    p[i] = in ? p[i] : 0.f;
+                    at = from + i + 1 < i1 ? at + slot_step : at;
+                    sat = from + i + 1 < i1 ? sat + sum_step : sat;
+                }
+            }
 #pragma unroll
             for (int i = 0; i < JOIN; ++i) {
                 h = decayed(p[i], h) + v[i];
                 ps += p[i];
+                if (walk == 1 && from + i < i1) store_at<float>(slot, i * slot_step, lane_at, h);
             }
-        }
-        fold_h[wave][lane] = h;
-        fold_p[wave][lane] = ps;
-        __syncthreads();
-    }
-    h = edge != nullptr && n < a.states ? edge[(batch * a.channels + channel) * a.states + n] : 0.f;
-    for (int32_t w = 0; w < wave; ++w) h = decayed(fold_p[w][lane], h) + fold_h[w][lane];
-    for (int32_t from = i0; from < i1; from += JOIN) {
-        if (per > JOIN) read(from);
-#pragma unroll
-        for (int i = 0; i < JOIN; ++i) {
-            h = decayed(p[i], h) + v[i];
-            if (from + i < i1) slot[static_cast<int64_t>(slot_of(from + i)) * S * cp] = h;
+            slot += JOIN * slot_step;
+            sum += JOIN * sum_step;
         }
     }
 }
@@ -282,26 +296,28 @@ __global__ __launch_bounds__(256) void state_space_step_kernel(const StepArgs a)
 }
 
 // Tokens a chunk.  A line stays whole where sequences and channels alone give every SIMD a
-// wave (1024 SIMDs); otherwise the count of chunks is the one whose passes take the least time
-// by what a wave costs: a SIMD issues a vector instruction every 7.2, 5.3, 4.9, 4.6, 4.5
-// cycles with 1, 2, 3, 4, 5 and more waves (measured), every chunk spends about 8 tokens'
-// time around its loop, and chunks are whole blocks of 16 tokens.
+// wave (1024 SIMDs).  Otherwise the chunk is the one (in whole blocks of 16 tokens) whose
+// passes take the least time by what was measured at 16 states: about 118 vector instructions
+// a token, of which a SIMD issues one every 9, 6, 5, 4.6, 4.5 cycles with 1, 2, 3, 4, 5 and
+// more waves; 1.8 passes; 8 tokens' time around a chunk's loop; and 5 ns for every chunk of 64
+// channels whose states go through the join.  (Lines of 3136 tokens, 96 tiles: 80 tokens 166 us
+// for both passes, against 183 at 96, where some SIMDs have four waves and others three.)
 int64_t forward_chunk(int64_t B, int64_t N, int64_t tiles) {
     const int64_t blocks = ss_ceil(N, SS_BLOCK), lines = B * tiles;
-    static const double issue[] = {0., 7.2, 5.3, 4.9, 4.6, 4.5, 4.5};
+    static const double issue[] = {0., 9., 6., 5., 4.6, 4.5, 4.5};
     if (lines >= 1024 || blocks < 3) return blocks * SS_BLOCK;
     int64_t best = blocks;
     double least = 0.;
-    for (int64_t waves = 1; waves <= 6; ++waves) {
-        int64_t chunks = waves * 1024 / lines;
-        chunks = chunks < 2 ? 2 : chunks > blocks ? blocks : chunks;
-        const int64_t per = ss_ceil(blocks, chunks);
-        const int64_t each = ss_ceil(ss_ceil(blocks, per) * lines, 1024);
-        const double time = static_cast<double>(per * SS_BLOCK + 8) * each * issue[each < 6 ? each : 6];
+    const int64_t most = ss_ceil(blocks * lines, 1024) + 1;   // blocks a chunk with one wave a SIMD
+    for (int64_t per = ss_ceil(most, 8); per <= most && per < blocks; ++per) {
+        const int64_t chunks = ss_ceil(blocks, per), each = ss_ceil(chunks * lines, 1024);
+        const double time = static_cast<double>(per * SS_BLOCK + 8) * each * issue[each < 6 ? each : 6] * 1.8 * 118 / 2300 +
+                            5e-3 * chunks * lines;
         if (least == 0. || time < least) {
             least = time;
             best = per;
         }
+        if (per - ss_ceil(most, 8) >= 256) break;
     }
     return best * SS_BLOCK;
 }
