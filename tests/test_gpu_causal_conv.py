@@ -246,3 +246,30 @@ def test_refusals(device):
     grad, = torch.autograd.grad(visionhope_causal_conv(leaf, weight).sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         grad.sum().backward()
+
+
+def test_forward_mode_is_refused_and_saved_tensors_may_change_strides(device):
+    from torch.autograd import forward_ad
+
+    from visionhope_amd.utils.causal_conv import visionhope_causal_conv
+
+    leaves = [t.to(device).requires_grad_() for t in _inputs(2, 30, 8, 4, torch.float32, seed=95)]
+    dy = randn(2, 30, 8, seed=96).to(device)
+
+    def call(x, weight, bias, state):
+        return visionhope_causal_conv(x, weight, bias, silu=True, state=state)
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            with pytest.raises(NotImplementedError):
+                call(forward_ad.make_dual(leaves[0].detach(), torch.ones_like(leaves[0])), *leaves[1:])
+    want = torch.autograd.grad(call(*leaves), leaves, dy)
+
+    def spread(t):   # the same values, every other element of a wider tensor
+        wide = torch.zeros(*t.shape, 2, device=t.device, dtype=t.dtype)
+        wide[..., 0] = t
+        return wide[..., 0]
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread):
+        got = torch.autograd.grad(call(*leaves), leaves, dy)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

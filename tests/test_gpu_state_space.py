@@ -345,3 +345,29 @@ def test_refusals(device):
         visionhope_state_space_step(*tokens, t["state"].transpose(0, 1).contiguous().transpose(0, 1))
     with pytest.raises(TypeError, match="state"):
         visionhope_state_space_step(*tokens, t["state"].half())
+
+
+def test_forward_mode_is_refused_and_saved_tensors_may_change_strides(device):
+    from torch.autograd import forward_ad
+
+    inputs = _inputs(2, 40, 24, 16, 2, torch.float32, seed=140)
+    leaves = [inputs[n].to(device).requires_grad_() for n in NAMES]
+    dy = randn(2, 40, 24, seed=141).to(device)
+
+    def call(*tensors):
+        return _own(tensors, True, None)[0]
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            with pytest.raises(NotImplementedError):
+                call(forward_ad.make_dual(leaves[0].detach(), torch.ones_like(leaves[0])), *leaves[1:])
+    want = torch.autograd.grad(call(*leaves), leaves, dy)
+
+    def spread(t):   # the same values, every other element of a wider tensor
+        wide = torch.zeros(*t.shape, 2, device=t.device, dtype=t.dtype)
+        wide[..., 0] = t
+        return wide[..., 0]
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread):
+        got = torch.autograd.grad(call(*leaves), leaves, dy)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

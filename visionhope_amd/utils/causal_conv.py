@@ -14,8 +14,8 @@ from torch.autograd.function import once_differentiable
 
 from . import hip
 from .cuda import on_tensor_device
-from .token_lines import (address, check_io, check_like, check_param, dense_channels, fp32_param, line_lengths,
-                          refuse_gradients)
+from .token_lines import (address, check_io, check_like, check_param, dense_channels, differentiated,
+                          fp32_param, line_lengths, refuse_gradients)
 
 MAX_TAPS = 8
 
@@ -57,6 +57,9 @@ class _CausalConvFunction(Function):
     def _gradients(x, weight, bias, state, lengths, ctx, dy, dnew_state):
         if dy is None and dnew_state is None:
             return (None,) * 7
+        # saved-tensor hooks may return other strides than were saved
+        x, weight = dense_channels(x), weight.contiguous()
+        bias, state, lengths = (None if t is None else t.contiguous() for t in (bias, state, lengths))
         batch, length, channels = x.shape
         taps = weight.shape[1]
         dy = torch.zeros_like(x, memory_format=torch.contiguous_format) if dy is None else dense_channels(dy.to(x.dtype))
@@ -113,7 +116,7 @@ def visionhope_causal_conv(x, weight, bias=None, *, silu=False, state=None, leng
         state = state.contiguous()
     lengths = line_lengths(name, lengths, batch, x.device)
     x = dense_channels(x)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, state)):
+    if differentiated(x, weight, bias, state):
         return _CausalConvFunction.apply(x, weight, bias, state, bool(silu), lengths, bool(return_state))
     y, new_state = _no_grad_forward(x, weight, bias, silu, state, lengths, return_state)
     return (y, new_state) if return_state else y

@@ -13,7 +13,7 @@ from torch.autograd.function import once_differentiable
 
 from . import hip
 from .cuda import on_tensor_device
-from .token_lines import IO_DTYPES, address, check_like, check_param, fp32_param
+from .token_lines import IO_DTYPES, address, check_like, check_param, differentiated, fp32_param
 
 MAX_CHANNELS = 8192
 
@@ -22,6 +22,8 @@ def _rows(t):
     """``t`` as rows a fixed number of elements apart: ``(tensor, stride)``.  Leading dimensions
     that do not fold into one are copied."""
     channels = t.shape[-1]
+    if t.is_contiguous():
+        return t, channels
     if t.ndim == 1:
         t = t[None]
     if t.stride(-1) != 1 and channels > 1:
@@ -49,14 +51,16 @@ def _forward(x, weight, bias, gate, eps, keep):
     if gate is not None:
         gate, gate_row = _rows(gate)
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    mean = rstd = None
+    stats, mean, rstd = None, None, None   # mean of every row, then rstd of every row
     if keep:
-        mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32).unbind(0)
+        stats = torch.empty((2, rows), device=x.device, dtype=torch.float32)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
     hip.check(hip.load_library().vh_gated_layernorm_forward(
         address(x), x_row, address(gate), gate_row, hip.dtype_code(x.dtype), address(weight), address(bias),
-        address(y), address(mean), address(rstd), rows, channels, float(eps), hip.stream_of(x)),
+        address(y), mean, rstd, rows, channels, float(eps), hip.stream_of(x)),
         "vh_gated_layernorm_forward")
-    return y, mean, rstd
+    return y, stats
 
 
 class _GatedLayerNormFunction(Function):
@@ -64,8 +68,8 @@ class _GatedLayerNormFunction(Function):
     @on_tensor_device
     def forward(ctx, x, weight, bias, gate, eps):
         weight32, bias32 = fp32_param(weight), fp32_param(bias)
-        y, mean, rstd = _forward(x, weight32, bias32, gate, eps, True)
-        ctx.save_for_backward(x, weight32, bias32, gate, mean, rstd)
+        y, stats = _forward(x, weight32, bias32, gate, eps, True)
+        ctx.save_for_backward(x, weight32, bias32, gate, stats)
         ctx.param_dtypes = (weight.dtype, bias.dtype)
         return y.view(x.shape)
 
@@ -76,9 +80,11 @@ class _GatedLayerNormFunction(Function):
 
     @staticmethod
     @on_tensor_device
-    def _gradients(x, weight, bias, gate, mean, rstd, ctx, dy):
+    def _gradients(x, weight, bias, gate, stats, ctx, dy):
         shape, channels = x.shape, x.shape[-1]
         rows = x.numel() // channels
+        # saved-tensor hooks may return other strides than were saved
+        weight, bias, stats = weight.contiguous(), bias.contiguous(), stats.contiguous()
         need = ctx.needs_input_grad
         x, x_row = _rows(x)
         dy, dy_row = _rows(dy.to(x.dtype))
@@ -93,7 +99,7 @@ class _GatedLayerNormFunction(Function):
         ws = hip.workspace(lib.vh_gated_layernorm_backward_workspace_bytes(rows, channels), x.device)
         hip.check(lib.vh_gated_layernorm_backward(
             address(dy), dy_row, address(x), x_row, address(gate), gate_row, hip.dtype_code(x.dtype), address(weight),
-            address(bias), address(mean), address(rstd), address(dx), address(dgate), address(dweight), address(dbias),
+            address(bias), stats.data_ptr(), stats.data_ptr() + 4 * rows, address(dx), address(dgate), address(dweight), address(dbias),
             rows, channels, address(ws), ws.numel() * 4, hip.stream_of(x)), "vh_gated_layernorm_backward")
         return (dx, dweight.to(ctx.param_dtypes[0]) if need[1] else None,
                 dbias.to(ctx.param_dtypes[1]) if need[2] else None, dgate, None)
@@ -117,7 +123,7 @@ def visionhope_gated_layernorm(x, weight, bias, eps=1e-6, *, gate=None):
     check_param(name, "bias", bias, (channels,), x.device)
     if gate is not None:
         check_like(name, "gate", gate, x.shape, x.dtype, x.device)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, gate)):
+    if differentiated(x, weight, bias, gate):
         return _GatedLayerNormFunction.apply(x, weight, bias, gate, float(eps))
     return _no_grad_forward(x, weight, bias, gate, eps)
 

@@ -18,8 +18,8 @@ from torch.autograd.function import once_differentiable
 
 from . import hip
 from .cuda import on_tensor_device
-from .token_lines import (address, check_io, check_like, check_param, dense_channels, fp32_param, line_lengths,
-                          refuse_gradients, rows_of)
+from .token_lines import (address, check_io, check_like, check_param, dense_channels, differentiated,
+                          fp32_param, line_lengths, refuse_gradients, rows_of)
 
 MAX_STATES = 32
 
@@ -55,7 +55,8 @@ class _StateSpaceScanFunction(Function):
     @on_tensor_device
     def forward(ctx, x, dt, A, b, c, D, gate, dt_bias, state, softplus, lengths, return_state):
         A32, D32, bias32 = fp32_param(A), fp32_param(D), fp32_param(dt_bias)
-        y, new_state, kept = _forward(x, dt, A32, b, c, D32, gate, bias32, state, softplus, lengths, return_state, True)
+        y, new_state, kept = _forward(x, dt, A32, b, c, D32, gate, bias32, state, softplus, lengths, return_state,
+                                      any(ctx.needs_input_grad))
         ctx.save_for_backward(x, dt, A32, b, c, D32, gate, bias32, lengths, kept)
         ctx.softplus = softplus
         ctx.param_dtypes = tuple(None if t is None else t.dtype for t in (A, D, dt_bias))
@@ -72,6 +73,10 @@ class _StateSpaceScanFunction(Function):
     def _gradients(x, dt, A, b, c, D, gate, dt_bias, lengths, kept, ctx, dy, dnew_state):
         if dy is None and dnew_state is None:
             return (None,) * 12
+        # saved-tensor hooks may return other strides than were saved
+        x, dt, b, c = dense_channels(x), dense_channels(dt), _dense_maps(b), _dense_maps(c)
+        gate = None if gate is None else dense_channels(gate)
+        A, D, dt_bias, lengths, kept = (None if t is None else t.contiguous() for t in (A, D, dt_bias, lengths, kept))
         shape, device, dtype = x.shape, x.device, x.dtype
         sizes = (*shape, b.shape[2], A.shape[1])
         need = ctx.needs_input_grad
@@ -151,8 +156,7 @@ def visionhope_state_space_scan(x, dt, A, B, C, D=None, *, gate=None, dt_bias=No
     x, dt, B, C = dense_channels(x), dense_channels(dt), _dense_maps(B), _dense_maps(C)
     gate = None if gate is None else dense_channels(gate)
     state = None if state is None else state.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, dt, A, B, C, D, gate, dt_bias, state)):
+    if differentiated(x, dt, A, B, C, D, gate, dt_bias, state):
         return _StateSpaceScanFunction.apply(x, dt, A, B, C, D, gate, dt_bias, state, int(bool(softplus)), lengths,
                                              bool(return_state))
     return _no_grad_forward(x, dt, A, B, C, D, gate, dt_bias, state, int(bool(softplus)), lengths, return_state)

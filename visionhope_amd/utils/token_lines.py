@@ -1,6 +1,7 @@
 """Argument handling shared by the operators of token lines ``[B, N, C]``."""
 
 import torch
+from torch.autograd import forward_ad
 
 IO_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -74,7 +75,19 @@ def rows_of(t):
     return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
 
 
+def differentiated(*tensors):
+    """Whether a call goes through its autograd Function: gradients are recorded for one of the
+    tensors, or a forward-mode level is open (the Function then refuses tangents, which no
+    kernel carries)."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def refuse_gradients(name, *tensors):
-    """Single-token calls write states in place and record no graph."""
+    """Single-token calls write states in place and record no derivatives of either mode."""
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} is for inference; call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
