@@ -71,16 +71,16 @@ __device__ __forceinline__ SSPlace ss_place(const SSArgs& a) {
     p.t1 = a.tokens - p.t0 < a.chunk ? a.tokens : p.t0 + a.chunk;
     int32_t len = a.tokens;
     if (a.lengths != nullptr) {
-        len = a.lengths[p.batch];
+        len = __builtin_amdgcn_readfirstlane(a.lengths[p.batch]);
         len = len < 0 ? 0 : len > a.tokens ? a.tokens : len;
     }
     p.te = len < p.t0 ? p.t0 : len > p.t1 ? p.t1 : len;
     return p;
 }
 
-// An element `offset` bytes behind a uniform address.  The offset passes through a register the
-// compiler cannot see behind, or it would keep a 64-bit address a lane for every tensor in
-// vector registers over the whole walk.
+// An element `offset` bytes behind a uniform address.  `opaque` hides a lane's offset from the
+// compiler, which would otherwise add it to the tensor's address once and keep (and step) a
+// 64-bit address a lane for every tensor in vector registers.
 __device__ __forceinline__ uint32_t opaque(uint32_t v) {
     asm volatile("" : "+v"(v));
     return v;

@@ -373,9 +373,9 @@ int check_sizes(int64_t B, int64_t N, int64_t C, int32_t groups) {
     return VH_OK;
 }
 
-// The scalar unit reads whole words.
+// The scalar unit reads whole words; the backward's offsets over a few rows are 32 bits wide.
 bool whole_words(const SSTokens& t, int64_t e) {
-    return reinterpret_cast<uintptr_t>(t.data) % 4 == 0 && t.bs * e % 4 == 0 && t.ts * e % 4 == 0;
+    return reinterpret_cast<uintptr_t>(t.data) % 4 == 0 && t.bs * e % 4 == 0 && t.ts * e % 4 == 0 && t.ts < (1 << 24);
 }
 
 }  // namespace
@@ -386,6 +386,8 @@ int ss_fill(SSArgs& a, int32_t io_dtype, int64_t B, int64_t N, int64_t C, int32_
     VH_REQUIRE(states >= 1 && states <= 32, VH_ERR_SHAPE, "states must be 1 to 32, got %d", states);
     VH_REQUIRE(a.x.data != nullptr && a.dt.data != nullptr && a.b.data != nullptr && a.c.data != nullptr &&
                    a.A != nullptr, VH_ERR_ARG, "x, dt, B, C and A must not be null");
+    VH_REQUIRE(static_cast<int64_t>(groups) * ss_padded(states) < (1 << 24), VH_ERR_SHAPE,
+               "state space scan: too many groups (%d)", groups);
     a.states = states;
     a.groups = groups;
     a.batches = static_cast<int32_t>(B);

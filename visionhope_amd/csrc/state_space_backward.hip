@@ -83,34 +83,47 @@ __global__ __launch_bounds__(64) void state_space_adjoint_kernel(const SSArgs a)
     a.sums[(static_cast<int64_t>(p.batch) * a.chunks + p.chunk) * cp + p.column] = total;
 }
 
-// Sum over lane bits 1 .. 5 above the LANES lanes of a channel, of 2 SPL values a lane: the row
-// swaps halve the values (lanes 32 .. 63 end with the second half, odd rows of 16 with the
-// second quarter), the bits inside a row are added up in every lane.
-template <int LANES, int SPL>
-__device__ __forceinline__ void channel_sums(float (&v)[2 * SPL]) {
-#pragma unroll
-    for (int i = 0; i < SPL; ++i) {
-        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + SPL]), false, false);
-        v[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-    }
-#pragma unroll
-    for (int i = 0; i < SPL / 2; ++i) {
-        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + SPL / 2]), false, false);
-        v[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-    }
-#pragma unroll
-    for (int i = 0; i < SPL / 2; ++i) {
-        v[i] += ln_dpp<0x128>(v[i]);                        // row_ror 8
-        v[i] += ln_dpp<0x124>(v[i]);                        // row_ror 4
-        if constexpr (LANES == 2) v[i] += ln_dpp<0x4E>(v[i]);   // lanes (2, 3, 0, 1)
-    }
+// The sums over lanes of four tokens' values, so that no lane holds a value twice before it must:
+// exchanging one lane bit of two registers and adding leaves the sum of the first in the lanes
+// with the bit clear, that of the second in the others.
+__device__ __forceinline__ float fold32(float a, float b) {   // lane bit 5
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
-// Sum over the LANES lanes of a channel.
+__device__ __forceinline__ float fold16(float a, float b) {   // lane bit 4
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ float fold_quad(float a, float b, bool upper) {   // a bit within four lanes
+    const float first = a + ln_dpp<CTRL>(a), second = b + ln_dpp<CTRL>(b);
+    return upper ? second : first;
+}
+// Sum over the channels inside a row of 16 lanes, in every lane.
 template <int LANES>
-__device__ __forceinline__ float state_sum(float v) {
-    v += ln_dpp<0xB1>(v);
-    if constexpr (LANES == 4) v += ln_dpp<0x4E>(v);
+__device__ __forceinline__ float row_channels(float v) {
+    v += ln_dpp<0x128>(v);                          // row_ror 8
+    v += ln_dpp<0x124>(v);                          // row_ror 4
+    if constexpr (LANES == 2) v += ln_dpp<0x4E>(v); // lanes (2, 3, 0, 1)
     return v;
+}
+
+// An element `offset` bytes behind a uniform address, through a buffer descriptor made of it.
+// (Plain loads cost more here: 415 vector instructions in part 3. below against 301, and 24
+// registers; in the forward's loop it is the other way round, 107 us against 117.)  Offsets stay
+// below the descriptor's 4 GiB: channels < 2^24 and at most 2^26 of them a token row.
+template <typename T>
+__device__ __forceinline__ T row_load(const T* base, uint32_t offset) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, -1, 0x00027000);
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rsrc, offset, 0, 0));
+    else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(rsrc, offset, 0, 0));
+}
+template <typename T>
+__device__ __forceinline__ void row_store(void* base, int64_t element, uint32_t offset, float v) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(static_cast<T*>(base) + element, 0, -1, 0x00027000);
+    const T out = from_f32<T>(v);
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, out), rsrc, offset, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, out), rsrc, offset, 0, 0);
 }
 
 // Waves a SIMD that the registers of the gradients' pass allow.
@@ -132,7 +145,8 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
     constexpr int TOKENS = SS_BLOCK * CHANNELS / 256;   // of a thread in 1. and 3.
     __shared__ float4 tok[SS_BLOCK][CHANNELS];
     __shared__ float maps[SS_BLOCK][2 * S];             // C, then B
-    __shared__ float parts[4][SS_BLOCK][2 * S];
+    __shared__ float parts[4][SS_BLOCK][2 * S + 4];    // (+ 4: the rows that a wave writes together in other banks)
+    __shared__ float starts[SUBS - 1][SPL][256];        // states before the sub-blocks but the last, a lane's own
 
     const uint32_t bid = xcd_remap_any(blockIdx.x, gridDim.x);
     const uint32_t rest = bid / static_cast<uint32_t>(a.wide_tiles);
@@ -143,7 +157,7 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
     const int32_t first = (tile - group * tiles_of_group) * CHANNELS;   // in the group
     const int32_t t0 = chunk * a.chunk, t1 = a.tokens - t0 < a.chunk ? a.tokens : t0 + a.chunk;
     int32_t te = a.tokens;
-    if (a.lengths != nullptr) te = a.lengths[batch];
+    if (a.lengths != nullptr) te = __builtin_amdgcn_readfirstlane(a.lengths[batch]);
     te = te < t0 ? t0 : te > t1 ? t1 : te;
     const int32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t cp = static_cast<int64_t>(a.tiles) * 64;
@@ -184,35 +198,41 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
     const T* x = static_cast<const T*>(a.x.data) + batch * a.x.bs;
     const T* dt = static_cast<const T*>(a.dt.data) + batch * a.dt.bs;
     const T* dy = static_cast<const T*>(a.dy.data) + batch * a.dy.bs;
-    const T* gate = a.gate.data != nullptr
-        ? static_cast<const T*>(a.gate.data) + batch * a.gate.bs : nullptr;
+    const bool gated = a.gate.data != nullptr, soft = a.softplus != 0;
+    const T* gate = gated ? static_cast<const T*>(a.gate.data) + batch * a.gate.bs : dy;
+    const int64_t gate_ts = gated ? a.gate.ts : a.dy.ts;
+    const uint32_t lane_at = static_cast<uint32_t>(tchannel) * sizeof(T);
     const BCT* bmap = static_cast<const BCT*>(a.b.data) + batch * a.b.bs + static_cast<int64_t>(group) * S;
     const BCT* cmap = static_cast<const BCT*>(a.c.data) + batch * a.c.bs + static_cast<int64_t>(group) * S;
     const int64_t out0 = static_cast<int64_t>(batch) * a.tokens * a.channels;
     float* bc = a.bc_partial + (static_cast<int64_t>(tile) * a.batches + batch) * a.tokens * (2 * S);
     float dD = 0.f, dbias = 0.f;
 
-    constexpr int MAPS = (SS_BLOCK * 2 * S + 255) / 256;   // values of B and C a thread brings
+    constexpr int MAPS = SS_BLOCK * 2 * S / 256;   // values of B and C a thread brings
     struct Raw { T x[TOKENS], dt[TOKENS], dy[TOKENS], gate[TOKENS]; };
     Raw next;
     float next_maps[MAPS];
     auto fetch = [&](int32_t tb) {
-        const uint32_t at = opaque(static_cast<uint32_t>(tchannel) * sizeof(T));
 #pragma unroll
         for (int i = 0; i < TOKENS; ++i) {
             const int64_t t = tb + tr + i < te ? tb + tr + i : te - 1;   // a token of the sequence
-            next.x[i] = load_at(x + t * a.x.ts, at);
-            next.dt[i] = load_at(dt + t * a.dt.ts, at);
-            next.dy[i] = load_at(dy + t * a.dy.ts, at);
-            if (gate != nullptr) next.gate[i] = load_at(gate + t * a.gate.ts, at);
+            next.x[i] = row_load(x + t * a.x.ts, lane_at);
+            next.dt[i] = row_load(dt + t * a.dt.ts, lane_at);
+            next.dy[i] = row_load(dy + t * a.dy.ts, lane_at);
+            next.gate[i] = row_load(gate + t * gate_ts, lane_at);
         }
-        const int32_t tid = opaque(threadIdx.x);
+        // a wave's values of one load are of C or of B and of rows that follow each other
+        const int32_t lane = threadIdx.x & 63;
 #pragma unroll
         for (int i = 0; i < MAPS; ++i) {
-            const int32_t v = tid + i * 256, r = v / (2 * S), n = v % (2 * S);
-            const int64_t t = tb + r;
-            next_maps[i] = v < SS_BLOCK * 2 * S && t < te
-                ? to_f32(n < S ? cmap[t * a.c.ts + n] : bmap[t * a.b.ts + n - S]) : 0.f;
+            const int32_t first = wave * 64 + i * 256;
+            const bool second = first >= SS_BLOCK * S;
+            const int32_t row = tb + (first - (second ? SS_BLOCK * S : 0)) / S, down = lane / S;
+            const int32_t from = row < te ? row : te - 1, left = te - 1 - from;
+            const int64_t ts = second ? a.b.ts : a.c.ts;
+            const uint32_t at = static_cast<uint32_t>(down < left ? down : left) * static_cast<uint32_t>(ts) + lane % S;
+            const float value = to_f32(row_load((second ? bmap : cmap) + from * ts, at * static_cast<uint32_t>(sizeof(BCT))));
+            next_maps[i] = row + down < te ? value : 0.f;
         }
     };
 
@@ -224,35 +244,33 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
         float h[SPL];
         {
             const float* from = a.kept + (static_cast<int64_t>(batch) * a.blocks + tb / SS_BLOCK) * S * cp;
-            const uint32_t at = opaque(static_cast<uint32_t>((part * SPL * cp + column) * sizeof(float)));
+            const uint32_t at = static_cast<uint32_t>((part * SPL * cp + column) * sizeof(float));
 #pragma unroll
-            for (int j = 0; j < SPL; ++j) h[j] = live ? load_at(from + j * cp, at) : 0.f;
+            for (int j = 0; j < SPL; ++j) h[j] = live ? row_load(from + j * cp, at) : 0.f;
         }
         // 1.  Tokens behind the sequence decay by one and add nothing.
 #pragma unroll
         for (int i = 0; i < TOKENS; ++i) {
             const bool in = tb + tr + i < te;
-            float step = to_f32(raw.dt[i]) + bias;
-            if (a.softplus) step = ss_softplus(step);
-            float dz = to_f32(raw.dy[i]);
-            if (gate != nullptr) {
-                const float z = to_f32(raw.gate[i]);
-                dz *= z * sigmoid_fast(z);
-            }
+            const float v = to_f32(raw.dt[i]) + bias, plus = ss_softplus(v), step = soft ? plus : v;
+            const float z = to_f32(raw.gate[i]), silu = z * sigmoid_fast(z);
+            const float dz = to_f32(raw.dy[i]) * (gated ? silu : 1.f);
             const float dtx = step * to_f32(raw.x[i]);
             tok[tr + i][tc] = make_float4(in ? step : 0.f, in && tlive ? dtx : 0.f, in && tlive ? dz : 0.f, 0.f);
         }
 #pragma unroll
         for (int i = 0; i < MAPS; ++i)
-            if (tid + i * 256 < SS_BLOCK * 2 * S) (&maps[0][0])[tid + i * 256] = next_maps[i];
+        {
+            const int32_t first = wave * 64 + i * 256, lane = tid & 63;
+            const bool second = first >= SS_BLOCK * S;
+            maps[(first - (second ? SS_BLOCK * S : 0)) / S + lane / S][(second ? S : 0) + lane % S] = next_maps[i];
+        }
         __syncthreads();
         // 2.
-        float start[SUBS][SPL];
 #pragma unroll
-        for (int sub = 0; sub < SUBS; ++sub) {
+        for (int sub = 0; sub < SUBS - 1; ++sub) {
 #pragma unroll
-            for (int j = 0; j < SPL; ++j) start[sub][j] = h[j];
-            if (sub == SUBS - 1) break;
+            for (int j = 0; j < SPL; ++j) starts[sub][j][tid] = h[j];
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
                 const float4 k = tok[sub * SUB + u][mine];
@@ -267,8 +285,10 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
             float decay[SUB][SPL], q[SUB][SPL];
             // the tokens' entries are read again from LDS in each walk, not kept from the last
             asm volatile("" ::: "memory");
+            if (sub < SUBS - 1) {
 #pragma unroll
-            for (int j = 0; j < SPL; ++j) h[j] = start[sub][j];
+                for (int j = 0; j < SPL; ++j) h[j] = starts[sub][j][tid];
+            }
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
                 const float4 k = tok[sub * SUB + u][mine];
@@ -282,79 +302,97 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
                 if (u % 2) __builtin_amdgcn_sched_barrier(0);
             }
             asm volatile("" ::: "memory");
-#pragma unroll
-            for (int u = SUB - 1; u >= 0; --u) {
+            // the adjoints, from the last token: each token's sums over states (y, g B, g A q)
+            // and the parts of dC and dB of each of its states
+            auto token = [&](int u, float (&v)[2 * SPL], float (&sum)[3]) {
                 const int32_t t = sub * SUB + u;
                 const float4 k = tok[t][mine];
                 const float* c = &maps[t][part * SPL];
                 const float* b = &maps[t][S + part * SPL];
-                float y = 0.f, gb = 0.f, ga = 0.f, v[2 * SPL];
+                sum[0] = sum[1] = sum[2] = 0.f;
 #pragma unroll
                 for (int j = 0; j < SPL; ++j) {
                     const float hj = fmaf(k.y, b[j], q[u][j]);
                     const float g = fmaf(c[j], k.z, carry[j]);
-                    y = fmaf(c[j], hj, y);
-                    gb = fmaf(g, b[j], gb);
+                    sum[0] = fmaf(c[j], hj, sum[0]);
+                    sum[1] = fmaf(g, b[j], sum[1]);
                     const float gq = g * q[u][j];
-                    ga = fmaf(gq, A2[j], ga);
+                    sum[2] = fmaf(gq, A2[j], sum[2]);
                     dA[j] = fmaf(gq, k.x, dA[j]);
                     carry[j] = g * decay[u][j];
                     v[j] = k.z * hj;
                     v[SPL + j] = k.y * g;
+                    // formed here and not put off to the end of the walk, where each token's g q
+                    // would still be needed
+                    asm volatile("" : "+v"(dA[j]));
                 }
-                y = state_sum<LANES>(y);
-                gb = state_sum<LANES>(gb);
-                ga = state_sum<LANES>(ga);
-                // dA's sums are formed here and not put off to the end of the walk, where each
-                // would still need its g q
+            };
+            float v[2][2 * SPL], w[2 * SPL], sum[2][3], late[3];
+            token(3, v[1], sum[1]);
+            token(2, v[0], sum[0]);
 #pragma unroll
-                for (int j = 0; j < SPL; ++j) asm volatile("" : "+v"(dA[j]));
-                // the channel's lanes have read this token's entry: its last use here
-                if (part == 0) tok[t][mine] = make_float4(y, gb, ga, 0.f);
-                channel_sums<LANES, SPL>(v);
-                // lanes 0 .. LANES - 1 of each row of 16: C in rows 0 and 1, B in 2 and 3
-                const int32_t lane = tid & 63, row = lane >> 4;
-                if ((lane & 15) < LANES) {
-                    float* to = &parts[wave][t][(row >> 1) * S + part * SPL + (row & 1) * (SPL / 2)];
+            for (int i = 0; i < 2 * SPL; ++i) w[i] = fold32(v[0][i], v[1][i]);
 #pragma unroll
-                    for (int j = 0; j < SPL / 2; ++j) to[j] = v[j];
-                }
-                if (u % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < 3; ++i) late[i] = fold_quad<0xB1>(sum[0][i], sum[1][i], part & 1);
+            __builtin_amdgcn_sched_barrier(0);
+            token(1, v[1], sum[1]);
+            token(0, v[0], sum[0]);
+#pragma unroll
+            for (int i = 0; i < 2 * SPL; ++i) {
+                // rows of 16 lanes 0 .. 3: tokens 0, 2, 1, 3
+                w[i] = row_channels<LANES>(fold16(fold32(v[0][i], v[1][i]), w[i]));
+                asm volatile("" : "+v"(w[i]));   // the sum is formed in every lane, not again in those that store
             }
+#pragma unroll
+            for (int i = 0; i < 3; ++i) sum[0][i] = fold_quad<0xB1>(sum[0][i], sum[1][i], part & 1);
+            // the channel's lanes have read these tokens' entries for the last time
+            if constexpr (LANES == 4) {
+#pragma unroll
+                for (int i = 0; i < 3; ++i) sum[0][i] = fold_quad<0x4E>(sum[0][i], late[i], part & 2);
+                tok[sub * SUB + part][mine] = make_float4(sum[0][0], sum[0][1], sum[0][2], 0.f);
+            } else {
+                tok[sub * SUB + part][mine] = make_float4(sum[0][0], sum[0][1], sum[0][2], 0.f);
+                tok[sub * SUB + 2 + part][mine] = make_float4(late[0], late[1], late[2], 0.f);
+            }
+            const int32_t lane = tid & 63, row = lane >> 4;
+            if ((lane & 15) < LANES) {
+                float* to = &parts[wave][sub * SUB + (row & 1) * 2 + (row >> 1)][part * SPL];
+#pragma unroll
+                for (int j = 0; j < 2 * SPL; ++j) to[j < SPL ? j : S + j - SPL] = w[j];
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
         // 3.
         if (blk > 0) fetch(tb - SS_BLOCK);
-        const uint32_t lane_at = opaque(static_cast<uint32_t>(tchannel) * sizeof(T));
 #pragma unroll
         for (int i = 0; i < TOKENS; ++i) {
             const int64_t t = tb + tr + i;
             if (t >= te) continue;
             const float4 r = tok[tr + i][tc];   // C h, g B, g A q over the states
-            const float xv = to_f32(raw.x[i]), gy = to_f32(raw.dy[i]), v = to_f32(raw.dt[i]) + bias;
-            const float step = a.softplus ? ss_softplus(v) : v;
-            float dz = gy, dgate = 0.f;
-            if (gate != nullptr) {
-                const float z = to_f32(raw.gate[i]), sig = sigmoid_fast(z);
-                dz *= z * sig;
-                dgate = gy * fmaf(D, xv, r.x) * (sig * fmaf(z, 1.f - sig, 1.f));
-            }
+            float xv = to_f32(raw.x[i]), gy = to_f32(raw.dy[i]), v = to_f32(raw.dt[i]) + bias;
+            float z = to_f32(raw.gate[i]);
+            // formed again rather than kept in registers through 2.
+            asm volatile("" : "+v"(v), "+v"(z), "+v"(gy), "+v"(xv));
+            const float plus = ss_softplus(v), step = soft ? plus : v, sig = sigmoid_fast(z);
+            const float dz = gy * (gated ? z * sig : 1.f);
+            const float dgate = gy * fmaf(D, xv, r.x) * (sig * fmaf(z, 1.f - sig, 1.f));
             // A2 is A log2(e)
-            float ddt = fmaf(xv, r.y, r.z * 0.6931471805599453f);
-            if (a.softplus) ddt *= sigmoid_fast(v);
+            const float ddt = fmaf(xv, r.y, r.z * 0.6931471805599453f) * (soft ? sigmoid_fast(v) : 1.f);
             dD = fmaf(dz, xv, dD);
             dbias += ddt;
             if (tlive) {
                 const int64_t at = out0 + t * a.channels;
-                store_at<T>(a.dx, at, lane_at, fmaf(step, r.y, D * dz));
-                store_at<T>(a.ddt, at, lane_at, ddt);
-                if (gate != nullptr) store_at<T>(a.dgate, at, lane_at, dgate);
+                row_store<T>(a.dx, at, lane_at, fmaf(step, r.y, D * dz));
+                row_store<T>(a.ddt, at, lane_at, ddt);
+                if (gated) row_store<T>(a.dgate, at, lane_at, dgate);
             }
         }
-        for (int32_t v = opaque(tid); v < SS_BLOCK * 2 * S; v += 256) {
-            const int32_t r = v / (2 * S), n = v % (2 * S);
-            if (tb + r < te)
-                bc[static_cast<int64_t>(tb) * (2 * S) + v] = (parts[0][r][n] + parts[1][r][n]) + (parts[2][r][n] + parts[3][r][n]);
+        for (uint32_t v = threadIdx.x; v < SS_BLOCK * 2 * S; v += 256) {
+            const uint32_t r = v / (2 * S), n = v % (2 * S);
+            if (tb + static_cast<int32_t>(r) < te)
+                row_store<float>(bc, static_cast<int64_t>(tb) * (2 * S), v * static_cast<uint32_t>(sizeof(float)),
+                                (parts[0][r][n] + parts[1][r][n]) + (parts[2][r][n] + parts[3][r][n]));
         }
     }
     // behind the sequence's end
@@ -363,7 +401,7 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
         const int64_t at = out0 + t * a.channels + tchannel;
         static_cast<T*>(a.dx)[at] = from_f32<T>(0.f);
         static_cast<T*>(a.ddt)[at] = from_f32<T>(0.f);
-        if (gate != nullptr) static_cast<T*>(a.dgate)[at] = from_f32<T>(0.f);
+        if (gated) static_cast<T*>(a.dgate)[at] = from_f32<T>(0.f);
     }
     for (int64_t v = static_cast<int64_t>(te) * (2 * S) + tid; v < static_cast<int64_t>(t1) * (2 * S); v += 256) bc[v] = 0.f;
 
