@@ -58,6 +58,7 @@ REFUSED = [
     ("vh_state_space_forward", SCAN, dict(states=0), hip.VH_ERR_SHAPE, "states"),
     ("vh_state_space_forward", SCAN, dict(states=33), hip.VH_ERR_SHAPE, "states"),
     ("vh_state_space_forward", SCAN, dict(groups=3), hip.VH_ERR_SHAPE, "groups"),
+    ("vh_state_space_forward", SCAN, dict(C=1 << 16, groups=1 << 16), hip.VH_ERR_SHAPE, "groups"),
     ("vh_state_space_forward", SCAN, dict(b=None), hip.VH_ERR_ARG, "null"),
     ("vh_state_space_forward", SCAN, dict(A=None), hip.VH_ERR_ARG, "null"),
     ("vh_state_space_forward", SCAN, dict(N=4096, wsn=16), hip.VH_ERR_WORKSPACE, "workspace"),

@@ -216,6 +216,17 @@ def test_gradients_only_where_asked(device):
         assert not visionhope_causal_conv(leaf, weight).requires_grad
 
 
+def test_step_marks_the_state_as_changed(device):
+    """A graph that saved the state refuses to run its backward with the moved-on one."""
+    from visionhope_amd.utils.causal_conv import visionhope_causal_conv, visionhope_causal_conv_step
+
+    x, weight, bias, state = (t.to(device) for t in _inputs(2, 9, 8, 4, torch.float32, seed=75))
+    y = visionhope_causal_conv(x, weight.clone().requires_grad_(), state=state)
+    visionhope_causal_conv_step(x[:, 0], state, weight)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_refusals(device):
     from visionhope_amd.utils.causal_conv import visionhope_causal_conv, visionhope_causal_conv_step
 

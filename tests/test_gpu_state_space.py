@@ -312,6 +312,41 @@ def test_gradients_only_where_asked(device):
     assert half.grad.dtype == torch.bfloat16
 
 
+def test_step_marks_the_state_as_changed(device):
+    from visionhope_amd.utils.state_space import visionhope_state_space_step
+
+    t = {k: v.to(device) for k, v in _inputs(2, 3, 24, 5, 1, torch.float32, seed=125).items()}
+    before = t["state"]._version
+    visionhope_state_space_step(t["x"][:, 0], t["dt"][:, 0], t["A"], t["B"][:, 0], t["C"][:, 0], t["state"])
+    assert t["state"]._version == before + 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_two_streams_at_once(device, dtype):
+    """Two training steps that overlap on two streams give what they give alone."""
+    runs = []
+    for seed in (150, 160):
+        inputs = _inputs(2, 600, 96, 16, 1, dtype, seed=seed)
+        leaves = [inputs[n].to(device).requires_grad_() for n in NAMES]
+        dy = randn(2, 600, 96, seed=seed + 10).to(device, dtype)
+
+        def step(leaves=leaves, dy=dy):
+            y, state = _own(leaves, True, None)
+            return [y.detach(), state.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+        runs.append((step, step(), torch.cuda.Stream(device)))
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(4):
+        for step, _, stream in runs:
+            with torch.cuda.stream(stream):
+                results.append(step())
+    torch.cuda.synchronize()
+    for i, got in enumerate(results):
+        for a, b in zip(got, runs[i % 2][1]):
+            assert torch.equal(a, b)
+
+
 def test_refusals(device):
     from visionhope_amd.utils.state_space import visionhope_state_space_scan, visionhope_state_space_step
 

@@ -121,6 +121,18 @@ def test_serving_prompt_then_tokens(device, dtype, norm):
             assert not out[i, n:].any()
 
 
+def test_inference_mode(device):
+    mixer = _mixer(True).to(device).eval()
+    x = randn(2, 9, 48, seed=6).to(device)
+    with torch.no_grad():
+        want = mixer(x)
+    with torch.inference_mode():
+        out, state = mixer(x[:, :8], return_state=True)
+        last = mixer.step(x[:, 8], state)
+    tol = 2 * tolerance(torch.float32, 9 + 4 * 96)
+    compare(torch.cat((out, last[:, None]), 1), want.double().cpu(), tol, "inference mode")
+
+
 def test_module_surface(device):
     from visionhope_amd.models import StateSpaceMixer
 

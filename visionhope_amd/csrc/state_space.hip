@@ -386,8 +386,7 @@ int ss_fill(SSArgs& a, int32_t io_dtype, int64_t B, int64_t N, int64_t C, int32_
     VH_REQUIRE(states >= 1 && states <= 32, VH_ERR_SHAPE, "states must be 1 to 32, got %d", states);
     VH_REQUIRE(a.x.data != nullptr && a.dt.data != nullptr && a.b.data != nullptr && a.c.data != nullptr &&
                    a.A != nullptr, VH_ERR_ARG, "x, dt, B, C and A must not be null");
-    VH_REQUIRE(static_cast<int64_t>(groups) * ss_padded(states) < (1 << 24), VH_ERR_SHAPE,
-               "state space scan: too many groups (%d)", groups);
+    VH_REQUIRE(groups <= 32768, VH_ERR_SHAPE, "state space scan: at most 32768 groups, got %d", groups);
     a.states = states;
     a.groups = groups;
     a.batches = static_cast<int32_t>(B);

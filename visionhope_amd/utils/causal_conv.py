@@ -15,7 +15,7 @@ from torch.autograd.function import once_differentiable
 from . import hip
 from .cuda import on_tensor_device
 from .token_lines import (address, check_io, check_like, check_param, dense_channels, differentiated,
-                          fp32_param, line_lengths, refuse_gradients)
+                          fp32_param, line_lengths, moved_on, refuse_gradients)
 
 MAX_TAPS = 8
 
@@ -152,4 +152,5 @@ def visionhope_causal_conv_step(x, state, weight, bias=None, *, silu=False, new_
     hip.check(hip.load_library().vh_causal_conv_step(
         address(x), x.stride(0), hip.dtype_code(x.dtype), address(weight), address(bias), int(silu), address(state),
         address(new_state), address(y), batch, channels, taps, hip.stream_of(x)), "vh_causal_conv_step")
+    moved_on(new_state)
     return y

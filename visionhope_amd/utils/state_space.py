@@ -19,7 +19,7 @@ from torch.autograd.function import once_differentiable
 from . import hip
 from .cuda import on_tensor_device
 from .token_lines import (address, check_io, check_like, check_param, dense_channels, differentiated,
-                          fp32_param, line_lengths, refuse_gradients, rows_of)
+                          fp32_param, line_lengths, moved_on, refuse_gradients, rows_of)
 
 MAX_STATES = 32
 
@@ -198,4 +198,5 @@ def visionhope_state_space_step(x, dt, A, B, C, state, D=None, *, gate=None, dt_
         hip.dtype_code(x.dtype), B.data_ptr(), B.stride(0), C.data_ptr(), C.stride(0), A.data_ptr(), address(D),
         address(dt_bias), int(bool(softplus)), state.data_ptr(), new_state.data_ptr(), y.data_ptr(), batch, channels,
         groups, states, hip.stream_of(x)), "vh_state_space_step")
+    moved_on(new_state)
     return y

@@ -2,6 +2,7 @@
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 IO_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -18,6 +19,8 @@ def check_io(name, x, ndim):
 
 def check_like(name, what, t, shape, dtype, device):
     """``t`` has exactly this shape, dtype and device."""
+    if isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == dtype and t.device == device:
+        return
     if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape):
         got = tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__
         raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {got}")
@@ -29,6 +32,8 @@ def check_like(name, what, t, shape, dtype, device):
 
 def check_param(name, what, t, shape, device):
     """A floating-point parameter of this shape on this device."""
+    if isinstance(t, torch.Tensor) and t.shape == shape and t.is_floating_point() and t.device == device:
+        return
     if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape):
         got = tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__
         raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {got}")
@@ -82,6 +87,13 @@ def differentiated(*tensors):
     if forward_ad._current_level >= 0:
         return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def moved_on(state):
+    """Marks a state that a kernel wrote as changed, so that a graph that saved it refuses to use
+    what stands there now (inference tensors keep no such mark)."""
+    if not state.is_inference():
+        increment_version(state)
 
 
 def refuse_gradients(name, *tensors):
