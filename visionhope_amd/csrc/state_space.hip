@@ -295,29 +295,31 @@ __global__ __launch_bounds__(256) void state_space_step_kernel(const StepArgs a)
     }
 }
 
-// Tokens a chunk.  A line stays whole where sequences and channels alone give every SIMD a
-// wave (1024 SIMDs).  Otherwise the chunk is the one (in whole blocks of 16 tokens) whose
-// passes take the least time by what was measured at 16 states: about 118 vector instructions
-// a token, of which a SIMD issues one every 9, 6, 5, 4.6, 4.5 cycles with 1, 2, 3, 4, 5 and
-// more waves; 1.8 passes; 8 tokens' time around a chunk's loop; and 5 ns for every chunk of 64
-// channels whose states go through the join.  (Lines of 3136 tokens, 96 tiles: 80 tokens 166 us
-// for both passes, against 183 at 96, where some SIMDs have four waves and others three.)
+// Tokens a chunk: whole lines, or the chunk (in whole blocks of 16 tokens) whose passes take
+// the least time by what was measured at 16 states: about 118 vector instructions a token, of
+// which a SIMD (of 1024) issues one every 9, 6, 5, 4.6, 4.5 cycles with 1, 2, 3, 4, 5 and more
+// waves; one pass for whole lines, 1.8 for chunks; 8 tokens' time around a chunk's loop; 5 ns
+// for every chunk of 64 channels whose states go through the join; and 10 us for the two
+// launches more.  (Lines of 3136 tokens, 96 tiles: 80 tokens 183 us for both passes, against
+// 204 at 96, where some SIMDs have four waves and others three.)
 int64_t forward_chunk(int64_t B, int64_t N, int64_t tiles) {
     const int64_t blocks = ss_ceil(N, SS_BLOCK), lines = B * tiles;
     static const double issue[] = {0., 9., 6., 5., 4.6, 4.5, 4.5};
-    if (lines >= 1024 || blocks < 3) return blocks * SS_BLOCK;
+    auto pass = [&](int64_t per, int64_t waves) {   // us, `waves` waves of `per` blocks
+        const int64_t each = ss_ceil(waves, 1024);
+        return static_cast<double>(per * SS_BLOCK + 8) * each * issue[each < 6 ? each : 6] * 118 / 2300;
+    };
     int64_t best = blocks;
-    double least = 0.;
+    double least = pass(blocks, lines);
     const int64_t most = ss_ceil(blocks * lines, 1024) + 1;   // blocks a chunk with one wave a SIMD
-    for (int64_t per = ss_ceil(most, 8); per <= most && per < blocks; ++per) {
-        const int64_t chunks = ss_ceil(blocks, per), each = ss_ceil(chunks * lines, 1024);
-        const double time = static_cast<double>(per * SS_BLOCK + 8) * each * issue[each < 6 ? each : 6] * 1.8 * 118 / 2300 +
-                            5e-3 * chunks * lines;
-        if (least == 0. || time < least) {
+    const int64_t first = ss_ceil(most, 8);
+    for (int64_t per = first; per <= most && per < blocks && per < first + 256; ++per) {
+        const int64_t chunks = ss_ceil(blocks, per);
+        const double time = 1.8 * pass(per, chunks * lines) + 5e-3 * chunks * lines + 10.;
+        if (time < least) {
             least = time;
             best = per;
         }
-        if (per - ss_ceil(most, 8) >= 256) break;
     }
     return best * SS_BLOCK;
 }

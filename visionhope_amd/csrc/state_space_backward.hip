@@ -480,7 +480,7 @@ Cut make_cut(int64_t B, int64_t N, int64_t C, int32_t groups, int32_t states) {
     c.wide_tiles = ss_ceil(C / groups, states <= 8 ? 128 : 64) * groups;
     const int64_t blocks = ss_ceil(N, SS_BLOCK);
     int64_t chunks = CUS * backward_waves(states) / (B * c.wide_tiles);
-    chunks = chunks < 1 ? 1 : chunks > blocks ? blocks : chunks;
+    chunks = chunks < 1 || blocks <= 4 ? 1 : chunks > blocks ? blocks : chunks;   // few blocks: no adjoints' pass
     const int64_t per = ss_ceil(blocks, chunks);             // blocks a chunk
     c.chunk = per * SS_BLOCK;
     c.chunks = ss_ceil(N, c.chunk);

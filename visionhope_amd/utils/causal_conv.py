@@ -138,8 +138,8 @@ def visionhope_causal_conv_step(x, state, weight, bias=None, *, silu=False, new_
     check_io(name, x, 2)
     batch, channels = x.shape
     taps = _check_weight(name, weight, bias, channels, x.device)
-    refuse_gradients(name, x, state, weight, bias)
     check_like(name, "state", state, (batch, taps - 1, channels), x.dtype, x.device)
+    refuse_gradients(name, x, state, weight, bias)
     if new_state is None:
         new_state = state
     else:
@@ -147,7 +147,7 @@ def visionhope_causal_conv_step(x, state, weight, bias=None, *, silu=False, new_
     if not state.is_contiguous() or not new_state.is_contiguous():
         raise ValueError(f"{name}: states must be contiguous")
     x = dense_channels(x)
-    weight, bias = fp32_param(weight).reshape(channels, -1), fp32_param(bias)
+    weight, bias = fp32_param(weight), fp32_param(bias)   # [C, K] and [C, 1, K] are the same memory
     y = torch.empty((batch, channels), device=x.device, dtype=x.dtype)
     hip.check(hip.load_library().vh_causal_conv_step(
         address(x), x.stride(0), hip.dtype_code(x.dtype), address(weight), address(bias), int(silu), address(state),

@@ -9,12 +9,13 @@ IO_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 def check_io(name, x, ndim):
     """``x`` is a CUDA tensor of a supported type with ``ndim`` nonempty dimensions."""
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in IO_DTYPES and x.ndim == ndim and x.numel():
+        return
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError(f"{name} expects CUDA tensors")
     if x.dtype not in IO_DTYPES:
         raise TypeError(f"{name} supports FP16, BF16 and FP32 tensors, got {x.dtype}")
-    if x.ndim != ndim or min(x.shape) <= 0:
-        raise ValueError(f"{name} expects a nonempty tensor of {ndim} dimensions, got shape {tuple(x.shape)}")
+    raise ValueError(f"{name} expects a nonempty tensor of {ndim} dimensions, got shape {tuple(x.shape)}")
 
 
 def check_like(name, what, t, shape, dtype, device):
@@ -98,8 +99,11 @@ def moved_on(state):
 
 def refuse_gradients(name, *tensors):
     """Single-token calls write states in place and record no derivatives of either mode."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} is for inference; call it under torch.no_grad() or on detached tensors")
-    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
-                                              for t in tensors):
-        raise NotImplementedError(f"{name} has no forward-mode derivative")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} is for inference; call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} has no forward-mode derivative")
