@@ -112,3 +112,41 @@ def test_cpu_tensors_are_refused():
                  lambda: visionhope_gated_layernorm(x, torch.ones(8), torch.zeros(8))):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+def test_captured_backward_refuses_leaves_of_a_living_default_stream_graph():
+    """The capture itself is played: the Function's two calls get the stream and the state."""
+    import torch
+
+    from visionhope_amd.utils.token_lines import mark_leaves, refuse_marked_leaves
+
+    class Double(torch.autograd.Function):
+        stream, capturing = 0, False
+
+        @staticmethod
+        def forward(ctx, x, weight):
+            mark_leaves(ctx, Double.stream)
+            return x * weight
+
+        @staticmethod
+        def backward(ctx, dy):
+            refuse_marked_leaves("double", ctx, Double.capturing)
+            return dy, dy
+
+    x, weight = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
+
+    def run(stream, capturing, inputs):
+        Double.stream, Double.capturing = stream, capturing
+        y = Double.apply(*inputs)
+        y.sum().backward()
+        return y
+
+    alive = run(0, False, (x, weight))
+    for inputs in ((x, weight), (x * 2, weight), (x, weight.detach())):
+        with pytest.raises(RuntimeError, match="still alive"):
+            run(7, True, inputs)
+    run(7, False, (x, weight))               # not a capture
+    run(7, True, (x.detach() * 2, weight.clone().detach().requires_grad_()))
+    del alive
+    alive = run(7, True, (x, weight))        # the graph is gone; one of another stream may live
+    run(8, True, (x, weight))

@@ -90,6 +90,28 @@ def differentiated(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+_LeafNode = type(torch.autograd.graph.get_gradient_edge(torch.empty(0, requires_grad=True)).node)
+
+
+def mark_leaves(ctx, stream):
+    """Called by a Function's forward: marks the nodes that accumulate its leaves' gradients when
+    it is recorded on the default stream.  Such a node keeps that stream for as long as any
+    graph over the leaf lives."""
+    if stream == 0:
+        for node, _ in ctx.next_functions:
+            if type(node) is _LeafNode:
+                node.metadata["visionhope_default_stream"] = True
+
+
+def refuse_marked_leaves(name, ctx, capturing):
+    """Called by a Function's backward: a captured backward must not reach a node of the default
+    stream, which cannot take part in a capture (the process would end there)."""
+    if capturing and any(type(node) is _LeafNode and "visionhope_default_stream" in node.metadata
+                         for node, _ in ctx.next_functions):
+        raise RuntimeError(f"{name}: cannot capture this backward pass: an autograd graph that was recorded over the "
+                           "same leaves on the default stream is still alive; drop its outputs before the capture")
+
+
 def moved_on(state):
     """Marks a state that a kernel wrote as changed, so that a graph that saved it refuses to use
     what stands there now (inference tensors keep no such mark)."""
