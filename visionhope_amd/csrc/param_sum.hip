@@ -2,7 +2,8 @@
 //
 // A workgroup takes 64 columns, its 16 waves interleaved rows, four loads in flight each; LDS
 // joins the waves.  With few columns and many rows the rows are also split over workgroups
-// and a second launch of the same kernel adds the parts.
+// and a second launch of the same kernel adds the parts.  3 to 5 us a launch: mostly the
+// launch's own time (1024 rows of 192 sums: 4.8 + 3.9 us).
 #include "param_sum.h"
 
 namespace vh {

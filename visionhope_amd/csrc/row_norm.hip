@@ -5,13 +5,14 @@
 // A row stays in registers between the statistics and the output: 2^lg lanes take it in
 // vectors of 16 bytes (2 or 1 elements where sizes or alignment ask for it), a whole
 // workgroup takes rows of more than 64 lanes' worth.  A workgroup walks several rows with
-// weight and bias in registers.  Bound by the bytes of the activations.
+// weight and bias in registers.  Bound by the bytes of the activations: 53.7 us for 401,408
+// rows of 96 bf16, 231 MB at 4.3 TB/s (a large copy reaches 4.84); 6.8 us for 64 rows of 1024.
 //
 // Backward, with g = dy silu(gate), gw = g w:
 //   dx = rstd (gw - mean(gw) - xhat mean(gw xhat)),  dw = sum g xhat,  db = sum g,
 //   dgate = dy (xhat w + b) silu'(gate)
 // with the statistics of the forward; the sums of dw and db stay in registers over a
-// workgroup's rows and are joined by param_sum.
+// workgroup's rows and are joined by param_sum.  91.4 us for the same rows, 389 MB at 4.3 TB/s.
 #include "param_sum.h"
 
 namespace vh {
