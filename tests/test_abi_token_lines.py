@@ -118,19 +118,19 @@ def test_captured_backward_refuses_leaves_of_a_living_default_stream_graph():
     """The capture itself is played: the Function's two calls get the stream and the state."""
     import torch
 
-    from visionhope_amd.utils.token_lines import mark_leaves, refuse_marked_leaves
+    from visionhope_amd.utils.token_lines import note_stream, refuse_held_leaves
 
     class Double(torch.autograd.Function):
         stream, capturing = 0, False
 
         @staticmethod
         def forward(ctx, x, weight):
-            mark_leaves(ctx, Double.stream)
+            note_stream(ctx, Double.stream)
             return x * weight
 
         @staticmethod
         def backward(ctx, dy):
-            refuse_marked_leaves("double", ctx, Double.capturing)
+            refuse_held_leaves("double", ctx, Double.capturing)
             return dy, dy
 
     x, weight = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)

@@ -15,7 +15,7 @@ from torch.autograd.function import once_differentiable
 from . import hip
 from .cuda import on_tensor_device
 from .token_lines import (address, check_io, check_like, check_param, dense_channels, differentiated,
-                          fp32_param, line_lengths, mark_leaves, moved_on, refuse_gradients, refuse_marked_leaves)
+                          fp32_param, line_lengths, moved_on, note_stream, refuse_gradients, refuse_held_leaves)
 
 MAX_TAPS = 8
 
@@ -39,7 +39,7 @@ class _CausalConvFunction(Function):
     def forward(ctx, x, weight, bias, state, silu, lengths, return_state):
         weight32, bias32 = fp32_param(weight).reshape(x.shape[-1], -1), fp32_param(bias)
         y, new_state = _forward(x, weight32, bias32, silu, state, lengths, return_state)
-        mark_leaves(ctx, hip.stream_of(x))
+        note_stream(ctx, hip.stream_of(x))
         ctx.save_for_backward(x, weight32, bias32, state, lengths)
         ctx.silu = silu
         ctx.weight_like = (weight.shape, weight.dtype)
@@ -56,7 +56,7 @@ class _CausalConvFunction(Function):
     @staticmethod
     @on_tensor_device
     def _gradients(x, weight, bias, state, lengths, ctx, dy, dnew_state):
-        refuse_marked_leaves("visionhope_causal_conv", ctx, torch.cuda.is_current_stream_capturing())
+        refuse_held_leaves("visionhope_causal_conv", ctx, torch.cuda.is_current_stream_capturing())
         if dy is None and dnew_state is None:
             return (None,) * 7
         # saved-tensor hooks may return other strides than were saved

@@ -13,8 +13,8 @@ from torch.autograd.function import once_differentiable
 
 from . import hip
 from .cuda import on_tensor_device
-from .token_lines import (IO_DTYPES, address, check_like, check_param, differentiated, fp32_param, mark_leaves,
-                          refuse_marked_leaves)
+from .token_lines import (IO_DTYPES, address, check_like, check_param, differentiated, fp32_param, note_stream,
+                          refuse_held_leaves)
 
 MAX_CHANNELS = 8192
 
@@ -70,7 +70,7 @@ class _GatedLayerNormFunction(Function):
     def forward(ctx, x, weight, bias, gate, eps):
         weight32, bias32 = fp32_param(weight), fp32_param(bias)
         y, stats = _forward(x, weight32, bias32, gate, eps, True)
-        mark_leaves(ctx, hip.stream_of(x))
+        note_stream(ctx, hip.stream_of(x))
         ctx.save_for_backward(x, weight32, bias32, gate, stats)
         ctx.param_dtypes = (weight.dtype, bias.dtype)
         return y.view(x.shape)
@@ -83,7 +83,7 @@ class _GatedLayerNormFunction(Function):
     @staticmethod
     @on_tensor_device
     def _gradients(x, weight, bias, gate, stats, ctx, dy):
-        refuse_marked_leaves("visionhope_gated_layernorm", ctx, torch.cuda.is_current_stream_capturing())
+        refuse_held_leaves("visionhope_gated_layernorm", ctx, torch.cuda.is_current_stream_capturing())
         shape, channels = x.shape, x.shape[-1]
         rows = x.numel() // channels
         # saved-tensor hooks may return other strides than were saved

@@ -19,7 +19,7 @@ from torch.autograd.function import once_differentiable
 from . import hip
 from .cuda import on_tensor_device
 from .token_lines import (address, check_io, check_like, check_param, dense_channels, differentiated,
-                          fp32_param, line_lengths, mark_leaves, moved_on, refuse_gradients, refuse_marked_leaves,
+                          fp32_param, line_lengths, moved_on, note_stream, refuse_gradients, refuse_held_leaves,
                           rows_of)
 
 MAX_STATES = 32
@@ -58,7 +58,7 @@ class _StateSpaceScanFunction(Function):
         A32, D32, bias32 = fp32_param(A), fp32_param(D), fp32_param(dt_bias)
         y, new_state, kept = _forward(x, dt, A32, b, c, D32, gate, bias32, state, softplus, lengths, return_state,
                                       any(ctx.needs_input_grad))
-        mark_leaves(ctx, hip.stream_of(x))
+        note_stream(ctx, hip.stream_of(x))
         ctx.save_for_backward(x, dt, A32, b, c, D32, gate, bias32, lengths, kept)
         ctx.softplus = softplus
         ctx.param_dtypes = tuple(None if t is None else t.dtype for t in (A, D, dt_bias))
@@ -73,7 +73,7 @@ class _StateSpaceScanFunction(Function):
     @staticmethod
     @on_tensor_device
     def _gradients(x, dt, A, b, c, D, gate, dt_bias, lengths, kept, ctx, dy, dnew_state):
-        refuse_marked_leaves("visionhope_state_space_scan", ctx, torch.cuda.is_current_stream_capturing())
+        refuse_held_leaves("visionhope_state_space_scan", ctx, torch.cuda.is_current_stream_capturing())
         if dy is None and dnew_state is None:
             return (None,) * 12
         # saved-tensor hooks may return other strides than were saved

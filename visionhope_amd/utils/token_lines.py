@@ -1,5 +1,7 @@
 """Argument handling shared by the operators of token lines ``[B, N, C]``."""
 
+from weakref import WeakValueDictionary
+
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
@@ -91,25 +93,33 @@ def differentiated(*tensors):
 
 
 _LeafNode = type(torch.autograd.graph.get_gradient_edge(torch.empty(0, requires_grad=True)).node)
+_DEFAULT_STREAM_GRAPHS = WeakValueDictionary()   # living nodes of Functions, by id
 
 
-def mark_leaves(ctx, stream):
-    """Called by a Function's forward: marks the nodes that accumulate its leaves' gradients when
-    it is recorded on the default stream.  Such a node keeps that stream for as long as any
-    graph over the leaf lives."""
+def note_stream(ctx, stream):
+    """Called by a Function's forward: keeps in mind, for as long as its graph lives, that it was
+    recorded on the default stream.  The nodes that accumulate its leaves' gradients keep that
+    stream as long."""
     if stream == 0:
-        for node, _ in ctx.next_functions:
-            if type(node) is _LeafNode:
-                node.metadata["visionhope_default_stream"] = True
+        _DEFAULT_STREAM_GRAPHS[id(ctx)] = ctx
 
 
-def refuse_marked_leaves(name, ctx, capturing):
+def _leaf_nodes(ctx):
+    return {node for node, _ in ctx.next_functions if type(node) is _LeafNode}
+
+
+def refuse_held_leaves(name, ctx, capturing):
     """Called by a Function's backward: a captured backward must not reach a node of the default
     stream, which cannot take part in a capture (the process would end there)."""
-    if capturing and any(type(node) is _LeafNode and "visionhope_default_stream" in node.metadata
-                         for node, _ in ctx.next_functions):
-        raise RuntimeError(f"{name}: cannot capture this backward pass: an autograd graph that was recorded over the "
-                           "same leaves on the default stream is still alive; drop its outputs before the capture")
+    if not capturing:
+        return
+    leaves = _leaf_nodes(ctx)
+    for other in _DEFAULT_STREAM_GRAPHS.valuerefs():
+        other = other()
+        if other is not None and not leaves.isdisjoint(_leaf_nodes(other)):
+            raise RuntimeError(f"{name}: cannot capture this backward pass: an autograd graph that was recorded over "
+                               "the same leaves on the default stream is still alive; drop its outputs before the "
+                               "capture")
 
 
 def moved_on(state):
