@@ -53,6 +53,9 @@ REFUSED = [
     ("vh_causal_conv_backward", CONV_BACK, dict(wsn=16), hip.VH_ERR_WORKSPACE, "workspace"),
     ("vh_causal_conv_backward", CONV_BACK, dict(dx=None), hip.VH_ERR_ARG, "null"),
     ("vh_causal_conv_step", CONV_STEP, dict(state=None), hip.VH_ERR_ARG, "null"),
+    ("vh_causal_conv_forward", CONV, dict(state=P, new_state=P), hip.VH_ERR_ARG, "overlap"),
+    ("vh_causal_conv_step", CONV_STEP, dict(new_state=P + 2 * 3 * 8 * 4 - 4), hip.VH_ERR_ARG, "overlap"),
+    ("vh_causal_conv_step", CONV_STEP, dict(state=P + 4), hip.VH_ERR_ARG, "overlap"),
     ("vh_causal_conv_step", CONV_STEP, dict(taps=0), hip.VH_ERR_SHAPE, "taps"),
     ("vh_state_space_forward", SCAN, dict(io=-1), hip.VH_ERR_DTYPE, "io_dtype"),
     ("vh_state_space_forward", SCAN, dict(states=0), hip.VH_ERR_SHAPE, "states"),
@@ -67,6 +70,8 @@ REFUSED = [
     ("vh_state_space_backward", SCAN_BACK, dict(gate=P), hip.VH_ERR_ARG, "dgate"),
     ("vh_state_space_backward", SCAN_BACK, dict(ws=P + 4), hip.VH_ERR_WORKSPACE, "aligned"),
     ("vh_state_space_backward", SCAN_BACK, dict(wsn=16), hip.VH_ERR_WORKSPACE, "workspace"),
+    ("vh_state_space_forward", SCAN, dict(state=P, new_state=P + 16), hip.VH_ERR_ARG, "overlap"),
+    ("vh_state_space_step", SCAN_STEP, dict(new_state=P + 2 * 8 * 16 * 4 - 4), hip.VH_ERR_ARG, "overlap"),
     ("vh_state_space_step", SCAN_STEP, dict(states=33), hip.VH_ERR_SHAPE, "states"),
     ("vh_state_space_step", SCAN_STEP, dict(B=0), hip.VH_ERR_SHAPE, "nonempty"),
     ("vh_state_space_step", SCAN_STEP, dict(state=None), hip.VH_ERR_ARG, "null"),

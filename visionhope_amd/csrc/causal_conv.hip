@@ -410,6 +410,8 @@ int vh_causal_conv_forward(const void* x, int64_t x_batch, int64_t x_token, int3
     using namespace vh;
     if (int rc = check_sizes(io_dtype, B, N, C, taps)) return rc;
     VH_REQUIRE(x != nullptr && weight != nullptr && y != nullptr, VH_ERR_ARG, "x, weight and y must not be null");
+    VH_REQUIRE(!overlapping(state, new_state, B * (taps - 1) * C * dtype_bytes(io_dtype)), VH_ERR_ARG,
+               "state and new_state must not overlap");
     ConvArgs a{};
     a.x = x;
     a.x_bs = x_batch;
@@ -503,6 +505,8 @@ int vh_causal_conv_step(const void* x, int64_t x_batch, int32_t io_dtype, const 
     if (int rc = check_sizes(io_dtype, B, 1, C, taps)) return rc;
     VH_REQUIRE(x != nullptr && weight != nullptr && state != nullptr && new_state != nullptr && y != nullptr, VH_ERR_ARG,
                "x, weight, state, new_state and y must not be null");
+    VH_REQUIRE(state == new_state || !overlapping(state, new_state, B * (taps - 1) * C * dtype_bytes(io_dtype)),
+               VH_ERR_ARG, "state and new_state must be the same memory or not overlap");
     ConvArgs a{};
     a.x = x;
     a.x_bs = x_batch;

@@ -492,6 +492,7 @@ int vh_state_space_forward(
     a.kept = kept;
     if (int rc = ss_fill(a, io_dtype, B, N, C, groups, states)) return rc;
     VH_REQUIRE(y != nullptr, VH_ERR_ARG, "y must not be null");
+    VH_REQUIRE(!overlapping(state, new_state, B * C * states * 4), VH_ERR_ARG, "state and new_state must not overlap");
     const int32_t S = ss_padded(states);
     a.chunk = static_cast<int32_t>(forward_chunk(B, N, a.tiles));
     a.chunks = static_cast<int32_t>(ss_ceil(N, a.chunk));
@@ -518,6 +519,8 @@ int vh_state_space_step(
     VH_REQUIRE(x != nullptr && dt != nullptr && b != nullptr && c != nullptr && A != nullptr && state != nullptr &&
                    new_state != nullptr && y != nullptr, VH_ERR_ARG,
                "x, dt, B, C, A, state, new_state and y must not be null");
+    VH_REQUIRE(state == new_state || !overlapping(state, new_state, B * C * states * 4), VH_ERR_ARG,
+               "state and new_state must be the same memory or not overlap");
     StepArgs a{};
     a.x = x;
     a.x_bs = x_batch;

@@ -171,6 +171,12 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
 // Element size of an io dtype code.
 inline int dtype_bytes(int t) { return t == VH_DTYPE_F32 ? 4 : 2; }
 
+// Whether two buffers of the same size share memory (null shares none).
+inline bool overlapping(const void* a, const void* b, int64_t bytes) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+    return a != nullptr && b != nullptr && (p > q ? p - q : q - p) < static_cast<uintptr_t>(bytes);
+}
+
 // ---------------------------------------------------------------------------
 // Scan-order maps of the four-direction operator (models/operator.py:79-86;
 // restoration in models/srnl_core/csrc/parallel_line.cuh:16-23).
