@@ -72,7 +72,9 @@ __global__ __launch_bounds__(64) void state_space_adjoint_kernel(const SSArgs a)
         fetch(t);
         cn.load(a.c.data, c0 + t * a.c.ts);
     }
+    SSTurns turns(count);
     for (; t >= SS_UNROLL - 1; t -= SS_UNROLL) {
+        turns.left(t);
         T dr[SS_UNROLL], yr[SS_UNROLL], gr[SS_UNROLL];
 #pragma unroll
         for (int u = 0; u < SS_UNROLL; ++u) { dr[u] = dn[u]; yr[u] = yn[u]; gr[u] = gn[u]; }
@@ -244,7 +246,9 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
 
     const int32_t blocks = (te - t0 + SS_BLOCK - 1) / SS_BLOCK;
     if (blocks > 0) fetch(t0 + (blocks - 1) * SS_BLOCK);
+    SSTurns turns(blocks);
     for (int32_t blk = blocks - 1; blk >= 0; --blk) {
+        turns.left(blk);
         const int32_t tb = t0 + blk * SS_BLOCK;
         const Raw raw = next;
         float h[SPL];
