@@ -155,7 +155,10 @@ __global__ __launch_bounds__(1024) void state_space_join_kernel(const SSArgs a, 
     __shared__ float fold_h[16][64], fold_p[16][64];
     const int32_t lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     const int32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int32_t rest = blockIdx.x / a.tiles, tile = blockIdx.x - rest * a.tiles;
+    // contiguous ranges of workgroups to each XCD: the states of a sequence share its sums there
+    // (7 sequences of 448 channels, 49 chunks: 14.8 -> 12.0 us)
+    const uint32_t bid = xcd_remap_any(blockIdx.x, gridDim.x);
+    const int32_t rest = static_cast<int32_t>(bid / static_cast<uint32_t>(a.tiles)), tile = static_cast<int32_t>(bid) - rest * a.tiles;
     const int32_t batch = rest / S, n = rest - batch * S;
     const int32_t group = tile / a.group_tiles, in_group = (tile - group * a.group_tiles) * 64 + lane;
     // lanes without a channel carry the group's last one, as in the other passes
