@@ -135,25 +135,6 @@ __device__ __forceinline__ float ss_softplus(float v) {
     return fmaf(s + s, p, fmaxf(v, 0.f));
 }
 
-// Turns of the waves of a SIMD.  Of equal priorities the oldest wave issues first, so waves of
-// equal work end one after the other and the last runs nearly alone, at two thirds of the rate
-// of four.  With a priority that falls when a half, a quarter and an eighth of its work is left
-// to a wave, they end together (1 x 16384 x 1024, 16 states: 81.4 -> 73 us for the output pass;
-// backward at 32 x 3136 x 192: 317 -> 297.  Even quarters 304, marks inside the backward's
-// blocks 316).
-struct SSTurns {
-    int32_t mark, level;
-    __device__ __forceinline__ explicit SSTurns(int32_t work) : mark(work >> 1), level(3) { __builtin_amdgcn_s_setprio(3); }
-    __device__ __forceinline__ void left(int32_t work) {
-        if (work > mark) return;
-        if (level == 3) __builtin_amdgcn_s_setprio(2);
-        else if (level == 2) __builtin_amdgcn_s_setprio(1);
-        else __builtin_amdgcn_s_setprio(0);
-        level -= 1;
-        mark = level > 0 ? mark >> 1 : -1;
-    }
-};
-
 inline int64_t ss_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // A channel's decay rates times log2(e), zero for the padding (whose states stay zero, as B and

@@ -103,7 +103,7 @@ __global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
         if (AHEAD) rows(0);
     }
     int32_t t = 0;
-    SSTurns turns(count);
+    WaveTurns turns(count);
     for (; t < count; t += SS_UNROLL) {
         turns.left(count - t);
         if (OUT && a.kept != nullptr && t % SS_BLOCK == 0) {

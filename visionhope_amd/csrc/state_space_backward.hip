@@ -72,7 +72,7 @@ __global__ __launch_bounds__(64) void state_space_adjoint_kernel(const SSArgs a)
         fetch(t);
         cn.load(a.c.data, c0 + t * a.c.ts);
     }
-    SSTurns turns(count);
+    WaveTurns turns(count);
     for (; t >= SS_UNROLL - 1; t -= SS_UNROLL) {
         turns.left(t);
         T dr[SS_UNROLL], yr[SS_UNROLL], gr[SS_UNROLL];
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
 
     const int32_t blocks = (te - t0 + SS_BLOCK - 1) / SS_BLOCK;
     if (blocks > 0) fetch(t0 + (blocks - 1) * SS_BLOCK);
-    SSTurns turns(blocks);
+    WaveTurns turns(blocks);
     for (int32_t blk = blocks - 1; blk >= 0; --blk) {
         turns.left(blk);
         const int32_t tb = t0 + blk * SS_BLOCK;
