@@ -314,14 +314,14 @@ __global__ __launch_bounds__(256) void state_space_step_kernel(const StepArgs a)
 
 // Tokens a chunk: whole lines, or the chunk (in whole blocks of 16 tokens) whose passes take
 // the least time by what was measured at 16 states: about 118 vector instructions a token, of
-// which a SIMD (of 1024) issues one every 9, 6, 5, 4.6, 4.5 cycles with 1, 2, 3, 4, 5 and more
-// waves; one pass for whole lines, 1.8 for chunks; 8 tokens' time around a chunk's loop; 5 ns
-// for every chunk of 64 channels whose states go through the join; and 10 us for the two
-// launches more.  (Lines of 3136 tokens, 96 tiles: 80 tokens 183 us for both passes, against
-// 204 at 96, where some SIMDs have four waves and others three.)
+// which a SIMD (of 1024) issues one every 9.5, 5.8, 5.2, 4.9, 4.5 cycles with 1, 2, 3, 4, 5 and
+// more waves; one pass for whole lines, 1.8 for chunks; 8 tokens' time around a chunk's loop;
+// 1.6 ns for every chunk of 64 channels whose states go through the join; and 10 us for the two
+// launches more.  (All passes at 64 and 80 tokens a chunk: 173 and 185 us for 32 x 3136 x 192
+// in training, 139 and 162 for 1 x 16384 x 1024; at 16 and 32: 43 and 45 for 7 x 785 x 448.)
 int64_t forward_chunk(int64_t B, int64_t N, int64_t tiles) {
     const int64_t blocks = ss_ceil(N, SS_BLOCK), lines = B * tiles;
-    static const double issue[] = {0., 9., 6., 5., 4.6, 4.5, 4.5};
+    static const double issue[] = {0., 9.5, 5.8, 5.2, 4.9, 4.5, 4.5};
     auto pass = [&](int64_t per, int64_t waves) {   // us, `waves` waves of `per` blocks
         const int64_t each = ss_ceil(waves, 1024);
         return static_cast<double>(per * SS_BLOCK + 8) * each * issue[each < 6 ? each : 6] * 118 / 2300;
@@ -332,7 +332,7 @@ int64_t forward_chunk(int64_t B, int64_t N, int64_t tiles) {
     const int64_t first = ss_ceil(most, 8);
     for (int64_t per = first; per <= most && per < blocks && per < first + 256; ++per) {
         const int64_t chunks = ss_ceil(blocks, per);
-        const double time = 1.8 * pass(per, chunks * lines) + 5e-3 * chunks * lines + 10.;
+        const double time = 1.8 * pass(per, chunks * lines) + 1.6e-3 * chunks * lines + 10.;
         if (time < least) {
             least = time;
             best = per;
