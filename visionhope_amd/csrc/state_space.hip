@@ -13,9 +13,9 @@
 // Bound by the issue of vector instructions.  A state of a token takes an exponential and four
 // products or sums (the output pass; three in the first), so 16 states take about 75 of the
 // output pass's 118 instructions a token and wave; softplus, SiLU and the conversions take the
-// rest.  A prompt of 1 x 16384 x 1024, 16 states, bf16: 61 + 13 + 84 us where the bytes need 28;
-// the vector unit is active for 76 and 72 % of the passes.  In training, which also writes the
-// kept states: 81 + 12 + 109 us at 32 x 3136 x 192 (bytes 48).
+// rest.  A prompt of 1 x 16384 x 1024, 16 states, bf16: 54 + 13 + 72 us where the bytes need 28;
+// the vector unit is active for 87 and 83 % of the passes.  In training, which also writes the
+// kept states: 66 + 15 + 95 us at 32 x 3136 x 192 (bytes 48).
 #include "state_space.h"
 
 namespace vh {
@@ -23,8 +23,8 @@ namespace {
 
 // OUT: the output pass; otherwise the pass for the chunks' own states.  One lane a channel: a
 // token's B and C stand in scalar registers and its sum over the states needs no other lane.
-// (At 1 x 16384 x 1024 the second takes 84 us; without the exponentials it would take 68,
-// without softplus and SiLU 73, with B and C of one token throughout 78.)
+// (Of the second's time at 1 x 16384 x 1024 the exponentials are a fifth, softplus
+// and SiLU an eighth.)
 template <typename T, typename BCT, int S, bool OUT>
 __global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
     const SSPlace p = ss_place(a);
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(64) void state_space_chunk_kernel(const SSArgs a) {
 // chunks: each folds its range, the ranges' results go through LDS, and each walks its range
 // again from the value before it.  Ranges of up to JOIN slots stand in registers and are read
 // once.  The launch is short, so its time is that of fetching its code: both walks share the
-// loop's.  12.4 us with 40 chunks (32 sequences of 192 channels, 16 states), 13.4 with 256
+// loop's.  15 us with 49 chunks (32 sequences of 192 channels, 16 states), 13 with 256
 // (one of 1024).
 constexpr int JOIN = 8;
 __global__ __launch_bounds__(1024) void state_space_join_kernel(const SSArgs a, const float* edge, int32_t S,
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(1024) void state_space_join_kernel(const SSArgs a, 
     const int32_t lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     const int32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // contiguous ranges of workgroups to each XCD: the states of a sequence share its sums there
-    // (7 sequences of 448 channels, 49 chunks: 14.8 -> 12.0 us)
+    // (7 sequences of 448 channels, 49 chunks: 14.8 -> 12.7 us)
     const uint32_t bid = xcd_remap_any(blockIdx.x, gridDim.x);
     const int32_t rest = static_cast<int32_t>(bid / static_cast<uint32_t>(a.tiles)), tile = static_cast<int32_t>(bid) - rest * a.tiles;
     const int32_t batch = rest / S, n = rest - batch * S;
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(256) void state_space_maps_kernel(const SSTokens b,
 // One token of every sequence.  Four states a lane; the lanes of a channel stand side by side,
 // so the states are read and written in whole rows of 16 bytes a lane (element by element
 // where the state count or an address does not allow that).  Bound by the states' bytes (FP32,
-// read and written) once the batch is large, by the launch before: 5.7 us for 64 sequences
+// read and written) once the batch is large, by the launch before: 5.8 us for 64 sequences
 // of 1024 channels and 16 states, 9 MB.
 struct StepArgs {
     const void *x, *dt, *gate, *b, *c;

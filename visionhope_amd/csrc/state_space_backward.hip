@@ -12,10 +12,10 @@
 // states inside a block again and then the adjoints, newest token first.  The chunks' adjoints
 // are joined over their boundaries as the forward joins states.
 //
-// At 32 x 3136 x 192, 16 states, bf16: adjoints between chunks 77 us, join 12, gradients 333,
-// dB and dC 9, parameters 5, where the bytes need 72.  The gradients' pass is bound by the
+// At 32 x 3136 x 192, 16 states, bf16: adjoints between chunks 68 us, join 15, gradients 294,
+// dB and dC 10, parameters 5, where the bytes need 72.  The gradients' pass is bound by the
 // issue of vector instructions: 111 a token for a wave's 16 channels, the vector unit active
-// for 76 % of the time, the rest two barriers a block and LDS.  (One lane a channel, as in the
+// for 87 % of the time.  (One lane a channel, as in the
 // forward, spills its states: 681 us for the pass.)
 #include "param_sum.h"
 #include "state_space.h"
