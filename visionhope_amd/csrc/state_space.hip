@@ -267,7 +267,10 @@ __global__ __launch_bounds__(256) void state_space_step_kernel(const StepArgs a)
     const T* b = static_cast<const T*>(a.b) + batch * a.b_bs + static_cast<int64_t>(group) * a.states + part;
     const T* c = static_cast<const T*>(a.c) + batch * a.c_bs + static_cast<int64_t>(group) * a.states + part;
     float h[4], A[4], bv[4], cv[4];
-    if (a.wide) {
+    // of 12, 20, 24 and 28 states the last lanes have none, and the memory there is the next
+    // channel's
+    const bool wide = a.wide && part < a.states;
+    if (wide) {
         const float4 h4 = *reinterpret_cast<const float4*>(state), A4 = *reinterpret_cast<const float4*>(rates);
         h[0] = h4.x; h[1] = h4.y; h[2] = h4.z; h[3] = h4.w;
         A[0] = A4.x; A[1] = A4.y; A[2] = A4.z; A[3] = A4.w;
@@ -277,7 +280,7 @@ __global__ __launch_bounds__(256) void state_space_step_kernel(const StepArgs a)
         const bool in = part + n < a.states;
         bv[n] = in ? to_f32(b[n]) : 0.f;
         cv[n] = in ? to_f32(c[n]) : 0.f;
-        if (!a.wide) {
+        if (!wide) {
             h[n] = in ? state[n] : 0.f;
             A[n] = in ? rates[n] : 0.f;
         }
@@ -294,7 +297,7 @@ __global__ __launch_bounds__(256) void state_space_step_kernel(const StepArgs a)
         acc = fmaf(cv[n], h[n], acc);
     }
     float* next = a.new_state + row * a.states + part;
-    if (a.wide) {
+    if (wide) {
         *reinterpret_cast<float4*>(next) = make_float4(h[0], h[1], h[2], h[3]);
     } else {
 #pragma unroll
