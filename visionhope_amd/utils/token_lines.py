@@ -92,7 +92,7 @@ def differentiated(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-_LeafNode = type(torch.autograd.graph.get_gradient_edge(torch.empty(0, requires_grad=True)).node)
+_LEAF_NODE = "torch::autograd::AccumulateGrad"
 _DEFAULT_STREAM_GRAPHS = WeakValueDictionary()   # living nodes of Functions, by id
 
 
@@ -105,7 +105,7 @@ def note_stream(ctx, stream):
 
 
 def _leaf_nodes(ctx):
-    return {node for node, _ in ctx.next_functions if type(node) is _LeafNode}
+    return {node for node, _ in ctx.next_functions if node is not None and node.name() == _LEAF_NODE}
 
 
 def refuse_held_leaves(name, ctx, capturing):
