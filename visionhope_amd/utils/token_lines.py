@@ -104,8 +104,26 @@ def note_stream(ctx, stream):
         _DEFAULT_STREAM_GRAPHS[id(ctx)] = ctx
 
 
-def _leaf_nodes(ctx):
-    return {node for node, _ in ctx.next_functions if node is not None and node.name() == _LEAF_NODE}
+def _leaf_nodes(roots, among=lambda node: True):
+    """The nodes that accumulate leaves' gradients behind these ones: their own inputs', and those
+    behind any operations between."""
+    leaves, seen, stack = set(), set(roots), list(roots)
+    while stack:
+        for node, _ in stack.pop().next_functions:
+            if node is None or node in seen or not among(node):
+                continue
+            seen.add(node)
+            (leaves.add if node.name() == _LEAF_NODE else stack.append)(node)
+    return leaves
+
+
+def _runs(node):
+    """Whether the backward pass under way goes to a node (asked about a leaf whose gradient is
+    returned and not accumulated, which it does go to, autograd raises)."""
+    try:
+        return torch._C._will_engine_execute_node(node)
+    except RuntimeError:
+        return True
 
 
 def refuse_held_leaves(name, ctx, capturing):
@@ -113,13 +131,11 @@ def refuse_held_leaves(name, ctx, capturing):
     stream, which cannot take part in a capture (the process would end there)."""
     if not capturing:
         return
-    leaves = _leaf_nodes(ctx)
-    for other in _DEFAULT_STREAM_GRAPHS.valuerefs():
-        other = other()
-        if other is not None and not leaves.isdisjoint(_leaf_nodes(other)):
-            raise RuntimeError(f"{name}: cannot capture this backward pass: an autograd graph that was recorded over "
-                               "the same leaves on the default stream is still alive; drop its outputs before the "
-                               "capture")
+    held = [other for other in (ref() for ref in _DEFAULT_STREAM_GRAPHS.valuerefs()) if other is not None]
+    if held and not _leaf_nodes([ctx], _runs).isdisjoint(_leaf_nodes(held)):
+        raise RuntimeError(f"{name}: cannot capture this backward pass: an autograd graph that was recorded over "
+                           "the same leaves on the default stream is still alive; drop its outputs before the "
+                           "capture")
 
 
 def moved_on(state):
