@@ -138,7 +138,7 @@ __global__ __launch_bounds__(256) void row_norm_kernel(const NormArgs a) {
 
 template <typename T, int VEC, int CPL>
 __global__ __launch_bounds__(256) void row_norm_backward_kernel(const NormArgs a) {
-    __shared__ float slots[2][4];
+    __shared__ float slots[3][4];
     __shared__ float joined[256 * VEC];
     const int32_t lanes = 1 << a.lg, sub = threadIdx.x & (lanes - 1), slot = threadIdx.x >> a.lg;
     const int32_t per_block = 256 >> a.lg;
@@ -172,37 +172,45 @@ __global__ __launch_bounds__(256) void row_norm_backward_kernel(const NormArgs a
                 if (gate != nullptr) load_vec<T, VEC>(gate + row * a.gate_ts + c, z[j]);
             }
         }
-        float s1 = 0.f, s2 = 0.f;
+        // The rounding of `mean` leaves the centred values a common offset, which the forward takes
+        // off once more; here it is summed beside the other two sums and enters behind them.
+        float off = 0.f, s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < CPL; ++j) {
-            const int32_t c = (j * lanes + sub) * VEC;
-            const bool mine = live && c < a.channels;
-            float dz[VEC];
+            const bool mine = live && (j * lanes + sub) * VEC < a.channels;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 xhat[j][i] = mine ? (xhat[j][i] - mean) * rstd : 0.f;
-                if (gate != nullptr) {
+                off += xhat[j][i];
+                if (gate != nullptr) {   // z becomes dy silu'(z)
                     const float zv = z[j][i], sig = sigmoid_fast(zv);
-                    dz[i] = g[j][i] * fmaf(xhat[j][i], w[j][i], b[j][i]) * (sig * fmaf(zv, 1.f - sig, 1.f));
+                    z[j][i] = g[j][i] * (sig * fmaf(zv, 1.f - sig, 1.f));
                     g[j][i] *= zv * sig;
                 }
-                dw[j][i] = fmaf(g[j][i], xhat[j][i], dw[j][i]);
-                db[j][i] += g[j][i];
-                g[j][i] *= w[j][i];
-                s1 += g[j][i];
-                s2 = fmaf(g[j][i], xhat[j][i], s2);
+                const float gw = g[j][i] * w[j][i];
+                s1 += gw;
+                s2 = fmaf(gw, xhat[j][i], s2);
             }
-            if (mine && gate != nullptr) store_vec<T, VEC>(static_cast<T*>(a.dgate) + row * a.channels + c, dz);
         }
-        s1 = row_sum(s1, a.lg, slots[0]) * inv;
-        s2 = row_sum(s2, a.lg, slots[1]) * inv;
+        off = row_sum(off, a.lg, slots[0]) * inv;
+        s1 = row_sum(s1, a.lg, slots[1]) * inv;
+        s2 = row_sum(s2, a.lg, slots[2]) * inv - off * s1;
 #pragma unroll
         for (int j = 0; j < CPL; ++j) {
             const int32_t c = (j * lanes + sub) * VEC;
-            float out[VEC];
+            float out[VEC], dz[VEC];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) out[i] = rstd * (g[j][i] - fmaf(xhat[j][i], s2, s1));
-            if (live && c < a.channels) store_vec<T, VEC>(static_cast<T*>(a.dx) + row * a.channels + c, out);
+            for (int i = 0; i < VEC; ++i) {
+                const float xh = xhat[j][i] - off;
+                dw[j][i] = fmaf(g[j][i], xh, dw[j][i]);
+                db[j][i] += g[j][i];
+                out[i] = rstd * (fmaf(g[j][i], w[j][i], -fmaf(xh, s2, s1)));
+                dz[i] = z[j][i] * fmaf(xh, w[j][i], b[j][i]);
+            }
+            if (live && c < a.channels) {
+                store_vec<T, VEC>(static_cast<T*>(a.dx) + row * a.channels + c, out);
+                if (gate != nullptr) store_vec<T, VEC>(static_cast<T*>(a.dgate) + row * a.channels + c, dz);
+            }
         }
     }
     // the row slots' sums, in order
