@@ -137,6 +137,15 @@ __device__ __forceinline__ float ss_softplus(float v) {
 
 inline int64_t ss_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// A decay rate as an exponent of two a unit step: the rate times log2(e), kept finite, since a
+// step of zero (a token behind a sequence's end, a chunk's sum of none) must decay by one and
+// zero times an infinite rate has no value.  A NaN stays one.
+__device__ __forceinline__ float ss_rate(float rate) {
+    constexpr float most = 3.4028234664e38f;
+    const float v = rate * SS_LOG2E;
+    return v < -most ? -most : v > most ? most : v;
+}
+
 // A channel's decay rates times log2(e), zero for the padding (whose states stay zero, as B and
 // C are zero there).
 template <int S>
@@ -153,7 +162,7 @@ __device__ __forceinline__ void ss_rates(const SSArgs& a, int32_t channel, float
         for (int n = 0; n < S; ++n) A2[n] = n < a.states ? from[n] : 0.f;
     }
 #pragma unroll
-    for (int n = 0; n < S; ++n) A2[n] *= SS_LOG2E;
+    for (int n = 0; n < S; ++n) A2[n] = ss_rate(A2[n]);
 }
 
 // State count that the kernels are built for.

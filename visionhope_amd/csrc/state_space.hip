@@ -164,7 +164,7 @@ __global__ __launch_bounds__(1024) void state_space_join_kernel(const SSArgs a, 
     // lanes without a channel carry the group's last one, as in the other passes
     const int32_t channel = group * a.group_channels + (in_group < a.group_channels ? in_group : a.group_channels - 1);
     const int64_t cp = static_cast<int64_t>(a.tiles) * 64;
-    const float A2 = n < a.states ? a.A[static_cast<int64_t>(channel) * a.states + n] * SS_LOG2E : 0.f;
+    const float A2 = n < a.states ? ss_rate(a.A[static_cast<int64_t>(channel) * a.states + n]) : 0.f;
     const int32_t per = (slots_n + waves - 1) / waves;
     const int32_t i0 = wave * per, i1 = i0 + per < slots_n ? i0 + per : slots_n;
     // Step i touches slot i with the decay of chunk i, or slot slots_n - 1 - i with that of chunk
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(256) void state_space_step_kernel(const StepArgs a)
     float acc = 0.f;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-        h[n] = fmaf(dtx, bv[n], h[n] * __builtin_amdgcn_exp2f(step * (A[n] * SS_LOG2E)));
+        h[n] = fmaf(dtx, bv[n], h[n] * __builtin_amdgcn_exp2f(step * ss_rate(A[n])));
         acc = fmaf(cv[n], h[n], acc);
     }
     float* next = a.new_state + row * a.states + part;

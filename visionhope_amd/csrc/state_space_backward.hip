@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256, backward_waves(LANES * SPL)) void state_space_
 #pragma unroll
     for (int j = 0; j < SPL; ++j) {
         const int32_t n = part * SPL + j;
-        A2[j] = n < a.states ? a.A[static_cast<int64_t>(channel) * a.states + n] * SS_LOG2E : 0.f;
+        A2[j] = n < a.states ? ss_rate(a.A[static_cast<int64_t>(channel) * a.states + n]) : 0.f;
         dA[j] = 0.f;
     }
     // the adjoint behind the chunk, times the decay of the token behind it
