@@ -17,6 +17,7 @@ from torch.nn.init import trunc_normal_
 from ..utils.causal_conv import visionhope_causal_conv, visionhope_causal_conv_step
 from ..utils.gated_norm import visionhope_gated_layernorm
 from ..utils.state_space import MAX_STATES, visionhope_state_space_scan, visionhope_state_space_step
+from ..utils.token_lines import line_lengths
 
 
 class StateSpaceMixer(nn.Module):
@@ -84,10 +85,16 @@ class StateSpaceMixer(nn.Module):
     def forward(self, x, *, state=None, lengths=None, return_state=False):
         """``[B, N, dim]`` -> ``[B, N, dim]``, or ``(output, state)`` with ``return_state``.
         ``state`` continues earlier tokens; ``lengths`` ``[B]`` ends sequences of a padded batch
-        early (their outputs behind the end are zero)."""
+        early: their outputs and gradients behind the end are zero, whatever stands there."""
         if x.ndim != 3 or x.shape[-1] != self.dim:
             raise ValueError(f"StateSpaceMixer expects [B, N, {self.dim}]")
         conv_state, scan_state = (None, None) if state is None else state
+        live = None
+        if lengths is not None:
+            lengths = line_lengths("StateSpaceMixer", lengths, x.shape[0], x.device)
+            live = (torch.arange(x.shape[1], device=x.device) < lengths[:, None])[..., None]
+            if torch.is_grad_enabled():   # the projections' weight gradients take all rows
+                x = torch.where(live, x, 0.0)
         x, gate = self.in_proj(x).chunk(2, dim=-1)
         x = visionhope_causal_conv(x, self.conv.weight, self.conv.bias, silu=True, state=conv_state, lengths=lengths,
                                    return_state=return_state)
@@ -100,10 +107,9 @@ class StateSpaceMixer(nn.Module):
         if return_state:
             y, scan_state = y
         out = self._output(y, gate)
-        if lengths is not None and self.norm_weight is not None:
-            # the norm gives rows of zeros its bias
-            live = torch.arange(out.shape[1], device=out.device) < lengths[:, None]
-            out = torch.where(live[..., None], out, 0.0)
+        if live is not None and (self.norm_weight is not None or torch.is_grad_enabled()):
+            # the norm does not leave rows of zeros zero, and out's gradient may be anything there
+            out = torch.where(live, out, 0.0)
         return (out, (conv_state, scan_state)) if return_state else out
 
     def step(self, x, state):
