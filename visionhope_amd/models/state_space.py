@@ -14,7 +14,7 @@ from torch import nn
 from torch.nn import functional as F
 from torch.nn.init import trunc_normal_
 
-from ..utils.causal_conv import visionhope_causal_conv, visionhope_causal_conv_step
+from ..utils.causal_conv import MAX_TAPS, visionhope_causal_conv, visionhope_causal_conv_step
 from ..utils.gated_norm import visionhope_gated_layernorm
 from ..utils.state_space import MAX_STATES, visionhope_state_space_scan, visionhope_state_space_step
 from ..utils.token_lines import line_lengths
@@ -34,6 +34,8 @@ class StateSpaceMixer(nn.Module):
             raise ValueError("dim and expand must be positive")
         if not 1 <= state_dim <= MAX_STATES:
             raise ValueError(f"state_dim must be 1 to {MAX_STATES}")
+        if not 2 <= conv_taps <= MAX_TAPS:
+            raise ValueError(f"conv_taps must be 2 to {MAX_TAPS}")
         self.dim, self.inner, self.state_dim, self.eps = int(dim), int(dim * expand), int(state_dim), eps
         self.dt_rank = math.ceil(dim / 16) if dt_rank is None else int(dt_rank)
         self.in_proj = nn.Linear(self.dim, 2 * self.inner, bias=False)
