@@ -141,7 +141,7 @@ def visionhope_causal_conv_step(x, state, weight, bias=None, *, silu=False, new_
     batch, channels = x.shape
     taps = _check_weight(name, weight, bias, channels, x.device)
     check_like(name, "state", state, (batch, taps - 1, channels), x.dtype, x.device)
-    refuse_gradients(name, x, state, weight, bias)
+    refuse_gradients(name, x, state, weight, bias, new_state)
     if new_state is None:
         new_state = state
     else:

@@ -184,7 +184,7 @@ def visionhope_state_space_step(x, dt, A, B, C, state, D=None, *, gate=None, dt_
     batch, channels = x.shape
     states, groups = _check_recurrence(name, x, dt, A, B, C, D, gate, dt_bias)
     check_like(name, "state", state, (batch, channels, states), torch.float32, x.device)
-    refuse_gradients(name, x, dt, A, B, C, state, D, gate, dt_bias)
+    refuse_gradients(name, x, dt, A, B, C, state, D, gate, dt_bias, new_state)
     if new_state is None:
         new_state = state
     else:
