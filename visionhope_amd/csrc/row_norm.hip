@@ -5,14 +5,14 @@
 // A row stays in registers between the statistics and the output: 2^lg lanes take it in
 // vectors of 16 bytes (2 or 1 elements where sizes or alignment ask for it), a whole
 // workgroup takes rows of more than 64 lanes' worth.  A workgroup walks several rows with
-// weight and bias in registers.  Bound by the bytes of the activations: 53.7 us for 401,408
-// rows of 96 bf16, 231 MB at 4.3 TB/s (a large copy reaches 4.84); 6.8 us for 64 rows of 1024.
+// weight and bias in registers.  Bound by the bytes of the activations: 54.6 us for 401,408
+// rows of 96 bf16, 231 MB at 4.2 TB/s (a large copy reaches 4.90); 6.8 us for 64 rows of 1024.
 //
 // Backward, with g = dy silu(gate), gw = g w:
 //   dx = rstd (gw - mean(gw) - xhat mean(gw xhat)),  dw = sum g xhat,  db = sum g,
 //   dgate = dy (xhat w + b) silu'(gate)
 // with the statistics of the forward; the sums of dw and db stay in registers over a
-// workgroup's rows and are joined by param_sum.  91.4 us for the same rows, 389 MB at 4.3 TB/s.
+// workgroup's rows and are joined by param_sum.  92.2 us for the same rows, 389 MB at 4.2 TB/s.
 #include "param_sum.h"
 
 namespace vh {
@@ -243,8 +243,9 @@ struct Plan {
 // Of the ways to lay a row over lanes, the one that leaves the fewest lanes idle, then the one
 // with the most lanes.  The backward of 16-bit types may also take 8-byte vectors, where that
 // gives a lane 16 elements or fewer: it keeps seven values an element, and 24 elements leave
-// two waves a SIMD (401,408 rows of 96 bf16: 90.6 us with 12 elements a lane against 95.8 with
-// 24; the forward, which keeps four, takes 53.2 us with 24 and 62.0 with 12).  A whole
+// two waves a SIMD (with the parameter sums 96.8 us against 103.3 for 401,408 rows of 96 bf16,
+// 84.9 against 101.2 for 50,000 of 768).  The forward, which keeps four, takes 53.2 us with 24
+// elements of 96 and 62.0 with 12.  A whole
 // workgroup takes a row, and pays barriers for it, only where a wave cannot hold it.
 Plan make_plan(int64_t channels, int widest, bool backward) {
     static const int wide[] = {1, 2, 3, 4, 6, 8}, narrow[] = {1, 2, 4, 8, 16, 32};

@@ -15,7 +15,7 @@
 // output pass's 118 instructions a token and wave; softplus, SiLU and the conversions take the
 // rest.  A prompt of 1 x 16384 x 1024, 16 states, bf16: 54 + 13 + 72 us where the bytes need 28;
 // the vector unit is active for 87 and 83 % of the passes.  In training, which also writes the
-// kept states: 66 + 15 + 95 us at 32 x 3136 x 192 (bytes 48).
+// kept states: 64 + 15 + 93 us at 32 x 3136 x 192 (bytes 48).
 #include "state_space.h"
 
 namespace vh {
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(1024) void state_space_join_kernel(const SSArgs a, 
     const int32_t lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     const int32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // contiguous ranges of workgroups to each XCD: the states of a sequence share its sums there
-    // (7 sequences of 448 channels, 49 chunks: 14.8 -> 12.7 us)
+    // (7 sequences of 448 channels, 49 chunks: 14.8 -> 12.8 us)
     const uint32_t bid = xcd_remap_any(blockIdx.x, gridDim.x);
     const int32_t rest = static_cast<int32_t>(bid / static_cast<uint32_t>(a.tiles)), tile = static_cast<int32_t>(bid) - rest * a.tiles;
     const int32_t batch = rest / S, n = rest - batch * S;
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(256) void state_space_maps_kernel(const SSTokens b,
 // One token of every sequence.  Four states a lane; the lanes of a channel stand side by side,
 // so the states are read and written in whole rows of 16 bytes a lane (element by element
 // where the state count or an address does not allow that).  Bound by the states' bytes (FP32,
-// read and written) once the batch is large, by the launch before: 5.8 us for 64 sequences
+// read and written) once the batch is large, by the launch before: 6.1 us for 64 sequences
 // of 1024 channels and 16 states, 9 MB.
 struct StepArgs {
     const void *x, *dt, *gate, *b, *c;
@@ -316,12 +316,17 @@ __global__ __launch_bounds__(256) void state_space_step_kernel(const StepArgs a)
 }
 
 // Tokens a chunk: whole lines, or the chunk (in whole blocks of 16 tokens) whose passes take
-// the least time by what was measured at 16 states: about 118 vector instructions a token, of
-// which a SIMD (of 1024) issues one every 9.5, 5.8, 5.2, 4.9, 4.5 cycles with 1, 2, 3, 4, 5 and
-// more waves; one pass for whole lines, 1.8 for chunks; 8 tokens' time around a chunk's loop;
-// 1.6 ns for every chunk of 64 channels whose states go through the join; and 10 us for the two
-// launches more.  (All passes at 64 and 80 tokens a chunk: 173 and 185 us for 32 x 3136 x 192
-// in training, 139 and 162 for 1 x 16384 x 1024; at 16 and 32: 43 and 45 for 7 x 785 x 448.)
+// the least time by a model fitted to whole passes of 16 states: about 118 vector instructions
+// a token, of which a SIMD (of 1024) issues one every 9.5, 5.8, 5.2, 4.9, 4.5 cycles with 1, 2,
+// 3, 4, 5 and more waves (its waits included); one pass for whole lines, 1.8 for chunks; 8
+// tokens' time around a chunk's loop; 1.6 ns for every chunk of 64 channels whose states go
+// through the join; and 10 us for the two launches more.  The state count does not enter: more
+// states lengthen the passes and the join alike.
+// Held against other chunks (16 to 128 tokens; 1 x 16384 x 1024, 32 x 3136 x 192, 8 x 784 x 1024
+// and 4 x 4096 x 384, all passes): at 4, 8, 12 and 16 states it takes the best or one 1.5 %
+// behind (the first with 16 states: 127 us at 64 tokens, 137 at 48, 149 at 80), at 20, 24 and 32
+// one up to 5 % behind, but 13 % with 32 states at 32 x 3136 x 192 (64 tokens 303 us in
+// training, 80 tokens 268).
 int64_t forward_chunk(int64_t B, int64_t N, int64_t tiles) {
     const int64_t blocks = ss_ceil(N, SS_BLOCK), lines = B * tiles;
     static const double issue[] = {0., 9.5, 5.8, 5.2, 4.9, 4.5, 4.5};

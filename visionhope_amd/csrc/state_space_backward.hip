@@ -12,7 +12,7 @@
 // states inside a block again and then the adjoints, newest token first.  The chunks' adjoints
 // are joined over their boundaries as the forward joins states.
 //
-// At 32 x 3136 x 192, 16 states, bf16: adjoints between chunks 68 us, join 15, gradients 294,
+// At 32 x 3136 x 192, 16 states, bf16: adjoints between chunks 67 us, join 15, gradients 293,
 // dB and dC 10, parameters 5, where the bytes need 72.  The gradients' pass is bound by the
 // issue of vector instructions: 111 a token for a wave's 16 channels, the vector unit active
 // for 87 % of the time.  (One lane a channel, as in the
@@ -138,8 +138,8 @@ __device__ __forceinline__ void row_store(void* base, int64_t element, uint32_t 
 constexpr int backward_waves(int states) { return states <= 8 ? 3 : states <= 16 ? 4 : 2; }
 
 // The gradients of one chunk.  LANES lanes share a channel, SPL states each, so the decays and
-// states of SUB tokens stand in registers with room for four waves a SIMD (a wave alone issues
-// a vector instruction only every 7 cycles, four together one every 4.6).  A workgroup takes
+// states of SUB tokens stand in registers with room for four waves a SIMD (of independent vector
+// instructions a wave alone issues one every 7 cycles, four together one every 4.6).  A workgroup takes
 // 256 / LANES channels through blocks of SS_BLOCK tokens:
 //   1. by token and channel: step, step x and dz of the block go to LDS, as do B and C;
 //   2. by channel and states: the states before each sub-block from the kept ones, then from
