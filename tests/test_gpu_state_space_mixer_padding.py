@@ -5,6 +5,7 @@ import torch
 
 from tests.helpers import randn
 from tests.test_gpu_state_space_mixer import _mixer
+from tests.token_lines import compare, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +41,37 @@ def test_lengths_are_checked(device):
     for lengths in (torch.ones(3, dtype=torch.int32, device=device), torch.ones(2, dtype=torch.int32)):
         with pytest.raises(ValueError, match="lengths"):
             mixer(x, lengths=lengths)
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_captured_training_step(device, norm, ragged):
+    """Forward and backward of the whole module in one graph, replayed with new inputs."""
+    mixer = _mixer(norm).to(device)
+    lengths = torch.tensor([40, 0, 17, 1], dtype=torch.int32, device=device) if ragged else None
+    x, dout = randn(4, 40, 48, seed=5).to(device), randn(4, 40, 48, seed=6).to(device)
+    live = x.clone().requires_grad_()
+
+    def step():
+        out = mixer(live, lengths=lengths)
+        return [out.detach(), *torch.autograd.grad(out, [live, *mixer.parameters()], dout)]
+
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(side):
+        step()   # the library's products choose their kernels outside the capture
+    torch.cuda.current_stream(device).wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for replay in range(3):
+        with torch.no_grad():
+            live.copy_(x * (replay + 1))
+        want = step()
+        for t in captured:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for name, a, b in zip(("out", "x", *(n for n, _ in mixer.named_parameters())), captured, want):
+            compare(a, b.double().cpu(), tolerance(torch.float32, 4 * 40 + 96), f"replay {replay} {name}")

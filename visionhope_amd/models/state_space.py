@@ -17,7 +17,7 @@ from torch.nn.init import trunc_normal_
 from ..utils.causal_conv import MAX_TAPS, visionhope_causal_conv, visionhope_causal_conv_step
 from ..utils.gated_norm import visionhope_gated_layernorm
 from ..utils.state_space import MAX_STATES, visionhope_state_space_scan, visionhope_state_space_step
-from ..utils.token_lines import line_lengths
+from ..utils.token_lines import guarded, line_lengths
 
 
 class StateSpaceMixer(nn.Module):
@@ -112,6 +112,7 @@ class StateSpaceMixer(nn.Module):
         if live is not None and (self.norm_weight is not None or torch.is_grad_enabled()):
             # the norm does not leave rows of zeros zero, and out's gradient may be anything there
             out = torch.where(live, out, 0.0)
+        out = guarded("StateSpaceMixer", out)
         return (out, (conv_state, scan_state)) if return_state else out
 
     def step(self, x, state):

@@ -6,6 +6,8 @@ import torch
 from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
+from .cuda import on_tensor_device
+
 IO_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
@@ -136,6 +138,27 @@ def refuse_held_leaves(name, ctx, capturing):
         raise RuntimeError(f"{name}: cannot capture this backward pass: an autograd graph that was recorded over "
                            "the same leaves on the default stream is still alive; drop its outputs before the "
                            "capture")
+
+
+class _GuardFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, out, name):
+        ctx.name = name
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, dy):
+        refuse_held_leaves(ctx.name, ctx, torch.cuda.is_current_stream_capturing())
+        return dy, None
+
+
+@on_tensor_device
+def guarded(name, out):
+    """Called by a module on its output: in a capture its backward refuses held leaves here, before
+    the pass comes to those of the module's operations behind the last operator."""
+    if out.requires_grad and torch.cuda.is_current_stream_capturing():
+        return _GuardFunction.apply(out, name)
+    return out
 
 
 def moved_on(state):
