@@ -637,6 +637,43 @@ int vh_gated_layernorm_backward(const void* dy, int64_t dy_row, const void* x, i
                                 float* dbias, int64_t rows, int64_t channels, void* workspace, size_t workspace_bytes,
                                 void* stream);
 
+/* Linear attention of token lines with a decay for each head, states [key_dim, value_dim] FP32:
+ *   S[t] = exp(log_decay) S[t-1] + k[t] v[t]^T,   o[t] = scale q[t]^T S[t]
+ * q, k [B, N, heads, key_dim] and v [B, N, heads, value_dim] in io_dtype with the element strides
+ * of a sequence, a token and a head (0: shared), heads of 1..128; log_decay [heads] fp32; state and
+ * new_state [B, heads, key_dim, value_dim] fp32 (or NULL), not overlapping; out [B, N, heads,
+ * value_dim].  Workspaces from the queries, 16-byte aligned (NULL where a query says 0). */
+size_t vh_linear_attention_workspace_bytes(int64_t B, int64_t N, int64_t heads, int64_t key_dim, int64_t value_dim,
+                                           int32_t io_dtype);
+int vh_linear_attention_forward(
+    const void* q, int64_t q_batch, int64_t q_token, int64_t q_head, const void* k, int64_t k_batch, int64_t k_token,
+    int64_t k_head, const void* v, int64_t v_batch, int64_t v_token, int64_t v_head, int32_t io_dtype,
+    const float* log_decay, float scale, const float* state, const int32_t* lengths, void* out, float* new_state,
+    int64_t B, int64_t N, int64_t heads, int64_t key_dim, int64_t value_dim, void* workspace, size_t workspace_bytes,
+    void* stream);
+
+/* Gradients of vh_linear_attention_forward: dq, dk [B, N, heads, key_dim] and dv [B, N, heads,
+ * value_dim] in io_dtype, dense; dstate (or NULL) like state, dlog_decay [heads] (or NULL; the
+ * workspace query's `decay`) fp32; dnew_state (or NULL) is the gradient of new_state.  Sums run in
+ * a fixed order. */
+size_t vh_linear_attention_backward_workspace_bytes(int64_t B, int64_t N, int64_t heads, int64_t key_dim,
+                                                    int64_t value_dim, int32_t io_dtype, int32_t decay);
+int vh_linear_attention_backward(
+    const void* dout, int64_t dout_batch, int64_t dout_token, int64_t dout_head, const void* q, int64_t q_batch,
+    int64_t q_token, int64_t q_head, const void* k, int64_t k_batch, int64_t k_token, int64_t k_head, const void* v,
+    int64_t v_batch, int64_t v_token, int64_t v_head, int32_t io_dtype, const float* log_decay, float scale,
+    const float* state, const int32_t* lengths, const float* dnew_state, void* dq, void* dk, void* dv, float* dstate,
+    float* dlog_decay, int64_t B, int64_t N, int64_t heads, int64_t key_dim, int64_t value_dim, void* workspace,
+    size_t workspace_bytes, void* stream);
+
+/* One token of every sequence: q, k [B, heads, key_dim] and v [B, heads, value_dim], strides of a
+ * sequence and a head; state and new_state [B, heads, key_dim, value_dim] fp32 (may be the same
+ * memory, must not overlap otherwise); out [B, heads, value_dim]. */
+int vh_linear_attention_step(
+    const void* q, int64_t q_batch, int64_t q_head, const void* k, int64_t k_batch, int64_t k_head, const void* v,
+    int64_t v_batch, int64_t v_head, int32_t io_dtype, const float* log_decay, float scale, const float* state,
+    float* new_state, void* out, int64_t B, int64_t heads, int64_t key_dim, int64_t value_dim, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -222,3 +222,21 @@ def gated_layernorm_torch(x, weight, bias, eps, gate=None):
     var = ((x - mean) ** 2).mean(-1, keepdim=True)
     y = (x - mean) / torch.sqrt(var + eps) * weight + bias
     return y if gate is None else y * torch.nn.functional.silu(gate)
+
+
+def linear_attention_torch(q, k, v, log_decay, scale=None, state=None, lengths=None):
+    """Token by token: S = exp(log_decay) S + k v^T, o = scale q^T S over q, k [B, N, H, K] and
+    v [B, N, H, V]; returns (o, last state of every sequence)."""
+    batch, length, heads, key_dim = q.shape
+    live = _before(lengths, length)[..., None]
+    none = torch.zeros((), dtype=q.dtype)
+    q, k, v = (torch.where(live, t, none) for t in (q, k, v))
+    scale = key_dim ** -0.5 if scale is None else scale
+    s = torch.zeros(batch, heads, key_dim, v.shape[-1], dtype=q.dtype) if state is None else state
+    decay = torch.exp(log_decay)[:, None, None]
+    rows = []
+    for t in range(length):
+        moved = decay * s + k[:, t, :, :, None] * v[:, t, :, None, :]
+        s = moved if lengths is None else torch.where(live[:, t, ..., None], moved, s)
+        rows.append((q[:, t, :, :, None] * s).sum(-2) * scale)
+    return torch.where(live, torch.stack(rows, 1), none), s

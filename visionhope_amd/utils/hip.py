@@ -46,6 +46,8 @@ EXPORTED_SYMBOLS = (
     "vh_causal_conv_step", "vh_state_space_workspace_bytes", "vh_state_space_kept_bytes", "vh_state_space_forward",
     "vh_state_space_backward_workspace_bytes", "vh_state_space_backward", "vh_state_space_step",
     "vh_gated_layernorm_forward", "vh_gated_layernorm_backward_workspace_bytes", "vh_gated_layernorm_backward",
+    "vh_linear_attention_workspace_bytes", "vh_linear_attention_forward",
+    "vh_linear_attention_backward_workspace_bytes", "vh_linear_attention_backward", "vh_linear_attention_step",
 )
 
 
@@ -181,6 +183,16 @@ _SIGNATURES = {
     "vh_gated_layernorm_backward_workspace_bytes": (_sz, [_i64, _i64]),
     "vh_gated_layernorm_backward": (ctypes.c_int, [
         _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz, _vp]),
+    "vh_linear_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32]),
+    "vh_linear_attention_forward": (ctypes.c_int, [
+        _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _f32, _vp, _vp, _vp, _vp,
+        _i64, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "vh_linear_attention_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32, _i32]),
+    "vh_linear_attention_backward": (ctypes.c_int, [
+        _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _f32,
+        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "vh_linear_attention_step": (ctypes.c_int, [
+        _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _f32, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
 }
 
 _LIB = None
