@@ -674,6 +674,25 @@ int vh_linear_attention_step(
     int64_t v_batch, int64_t v_head, int32_t io_dtype, const float* log_decay, float scale, const float* state,
     float* new_state, void* out, int64_t B, int64_t heads, int64_t key_dim, int64_t value_dim, void* stream);
 
+/* Group norm of dense channels-last maps [B, pixels, C] (io_dtype) in `groups` equal runs of at most
+ * 1024 channels, then an activation (0: none, 1: SiLU, 2: exact GELU): mean and biased variance over
+ * a group's channels and all pixels of an image; weight and bias [C] fp32.  stats [3, B, groups]
+ * fp32 (or NULL) receives mean, the rest that rounding left of it, and rstd for the backward.
+ * Workspaces from the queries, 16-byte aligned.  No counterpart in the reference's native code (its
+ * models/layers.py offers nn.GroupNorm). */
+size_t vh_group_norm_workspace_bytes(int64_t B, int64_t pixels, int64_t channels, int64_t groups, int32_t io_dtype);
+int vh_group_norm_forward(const void* x, int32_t io_dtype, const float* weight, const float* bias, int32_t activation,
+                          void* y, float* stats, int64_t B, int64_t pixels, int64_t channels, int64_t groups, float eps,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of vh_group_norm_forward: dx in io_dtype, dweight and dbias [C] fp32 (each may be NULL),
+ * summed in a fixed order. */
+size_t vh_group_norm_backward_workspace_bytes(int64_t B, int64_t pixels, int64_t channels, int64_t groups, int32_t io_dtype);
+int vh_group_norm_backward(const void* dy, const void* x, int32_t io_dtype, const float* weight, const float* bias,
+                           int32_t activation, const float* stats, void* dx, float* dweight, float* dbias, int64_t B,
+                           int64_t pixels, int64_t channels, int64_t groups, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -240,3 +240,16 @@ def linear_attention_torch(q, k, v, log_decay, scale=None, state=None, lengths=N
         s = moved if lengths is None else torch.where(live[:, t, ..., None], moved, s)
         rows.append((q[:, t, :, :, None] * s).sum(-2) * scale)
     return torch.where(live, torch.stack(rows, 1), none), s
+
+
+def group_norm_torch(x, groups, weight, bias, eps, activation=None):
+    """Group norm of [B, C, H, W] (biased variance), then SiLU or the exact GELU."""
+    batch, channels = x.shape[:2]
+    grouped = x.reshape(batch, groups, -1)
+    mean = grouped.mean(-1, keepdim=True)
+    var = ((grouped - mean) ** 2).mean(-1, keepdim=True)
+    y = ((grouped - mean) / torch.sqrt(var + eps)).reshape(x.shape)
+    y = y * weight.reshape(1, channels, 1, 1) + bias.reshape(1, channels, 1, 1)
+    if activation == "silu":
+        return y * torch.sigmoid(y)
+    return y * 0.5 * torch.special.erfc(-y * 0.5 ** 0.5) if activation == "gelu" else y

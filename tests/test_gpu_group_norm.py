@@ -1,0 +1,260 @@
+"""Group norm of channels-last maps with an activation on the GPU against the float64 oracle."""
+
+import pytest
+import torch
+
+from oracle.oracle_torch import group_norm_torch
+from tests.helpers import randn
+from tests.token_lines import DTYPES, compare, gradients, tolerance
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-5
+ACTIVATIONS = (None, "silu", "gelu")
+
+
+def _inputs(shape, dtype, seed=0):
+    channels = shape[1]
+    x = randn(*shape, seed=seed + 1) * torch.exp(0.3 * randn(1, channels, 1, 1, seed=seed + 2)) + randn(1, channels, 1, 1, seed=seed + 3)
+    return x.to(dtype), 1 + 0.2 * randn(channels, seed=seed + 4), 0.2 * randn(channels, seed=seed + 5)
+
+
+def _last(t):
+    return t.contiguous(memory_format=torch.channels_last)
+
+
+def _run(leaves, groups, activation, dy):
+    from visionhope_amd.utils.group_norm import visionhope_group_norm
+
+    y = visionhope_group_norm(leaves[0], groups, *leaves[1:], EPS, activation=activation)
+    return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+
+def _check(device, shape, groups, dtype, activation, what, x=None, extra=0.0):
+    made, weight, bias = _inputs(shape, dtype)
+    x = made if x is None else x
+    dy = randn(*shape, seed=9).to(dtype)
+    want, grads = gradients(lambda *a: group_norm_torch(a[0], groups, a[1], a[2], EPS, activation), (x, weight, bias), (dy,))
+    leaves = [t.to(device).requires_grad_() for t in (_last(x), weight, bias)]
+    got = _run(leaves, groups, activation, _last(dy.to(device)))
+    assert got[0].dtype == dtype and got[0].is_contiguous(memory_format=torch.channels_last)
+    values, rows = x.numel() // (shape[0] * groups), x.numel() // shape[1]
+    compare(got[0], want[0], tolerance(dtype, values) + extra, f"{what} y")
+    compare(got[1], grads[0], tolerance(dtype, values) + extra, f"{what} dx")
+    for name, a, b in zip(("dweight", "dbias"), got[2:], grads[1:]):
+        compare(a, b, tolerance(torch.float32, rows + values) + extra, f"{what} {name}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("shape, groups", [((1, 16, 1, 1), 1), ((2, 32, 7, 7), 2), ((3, 30, 5, 9), 5), ((2, 33, 6, 4), 3),
+                                           ((2, 96, 56, 56), 6), ((1, 640, 7, 7), 40), ((2, 12, 31, 17), 3), ((1, 257, 3, 5), 1),
+                                           ((5, 64, 1, 3), 1), ((1, 1024, 2, 3), 1), ((1, 2046, 4, 4), 2), ((2, 48, 130, 70), 1),
+                                           ((1, 7, 4, 100), 7)])
+def test_maps_and_gradients(device, dtype, activation, shape, groups):
+    _check(device, shape, groups, dtype, activation, f"{shape} {groups} {dtype} {activation}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_maps_far_from_zero(device, dtype):
+    """An offset of 1000 (FP32) or 64 (16 bits) beside a spread of 1: what the input's rounding leaves is
+    normalised as exactly as values around zero."""
+    offset = 1000.0 if dtype == torch.float32 else 64.0
+    x = (randn(2, 32, 40, 40, seed=20) + offset).to(dtype)
+    _check(device, (2, 32, 40, 40), 2, dtype, "silu", "offset", x=x, extra=offset * 2.0 ** -40)
+
+
+def test_one_value_far_from_the_others(device):
+    """The first value, which threads sum about, is 10^4 times the spread."""
+    x = randn(1, 16, 30, 30, seed=25)
+    x[0, 0, 0, 0] = 1e4
+    # its share of the squares is 1, and their sum is rounded as every other
+    _check(device, (1, 16, 30, 30), 1, torch.float32, None, "outlier", x=x)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_constant_maps(device, dtype):
+    from visionhope_amd.utils.group_norm import visionhope_group_norm
+
+    x = torch.zeros(2, 16, 9, 9)
+    x[:, :8], x[1, 8:] = 3.0, -200.0
+    weight, bias = randn(16, seed=30).to(device), randn(16, seed=31).to(device)
+    y = visionhope_group_norm(_last(x.to(device, dtype)), 2, weight, bias, EPS)
+    # x - mean is zero but for the mean's rounding of the sum of squares' weights: nothing
+    want = bias.to(dtype).reshape(1, 16, 1, 1).expand_as(y)
+    assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+def test_activations_over_their_range(device, activation):
+    """Outputs from deep in the activation's tail to far above it (FP32, the norm made the identity)."""
+    from visionhope_amd.utils.group_norm import visionhope_group_norm
+
+    n = 4096
+    x = torch.linspace(-9, 9, n).reshape(1, 1, 64, 64)
+    scale = (x.double().var(unbiased=False) + EPS).sqrt().float().reshape(1)
+    x = _last(x.to(device)).requires_grad_()
+    y = visionhope_group_norm(x, 1, scale.to(device), torch.zeros(1, device=device), EPS, activation=activation)
+    want = group_norm_torch(x.detach().double().cpu(), 1, scale.double(), torch.zeros(1).double(), EPS, activation)
+    diff = (y.detach().double().cpu() - want).abs()
+    # z (9 at most) is off by some 2^-22 of itself; an activation's slope is at most 1.13, and its
+    # relative slope in the tail |z|: 9 * 9 * 2^-22.  The tail's fit adds 9e-8, its exponent 2^-24 * 9^2 / 2.
+    assert (diff <= 1.13 * 9 * 2.0 ** -22 + want.abs() * (81 * 2.0 ** -22 + 9e-8 + 41 * 2.0 ** -24)).all()
+    small = want.abs() < 1e-3
+    assert (diff[small] <= 2.0 ** -100 + want.abs()[small] * 81 * 2.0 ** -20).all() or activation is None
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layouts_and_odd_addresses(device, dtype):
+    x, weight, bias = (t.to(device) for t in _inputs((2, 32, 12, 10), dtype, seed=40))
+    dy = randn(2, 32, 12, 10, seed=41).to(device, dtype)
+    x, dy = _last(x), _last(dy)
+
+    def both(view):
+        leaves = [view(x).detach().requires_grad_(), weight.clone().requires_grad_(), bias.clone().requires_grad_()]
+        return _run(leaves, 2, "gelu", view(dy))
+
+    def planes(t):
+        return t.contiguous()
+
+    def channels_of_a_wider_map(t):
+        w = torch.full((2, 40, 12, 10), float("nan"), device=device, dtype=dtype).contiguous(memory_format=torch.channels_last)
+        w[:, 4:36] = t
+        return w[:, 4:36]
+
+    def odd(t):
+        return torch.empty(t.numel() + 1, device=device, dtype=dtype)[1:].view(2, 12, 10, 32).permute(0, 3, 1, 2).copy_(t)
+
+    want = both(lambda t: t)
+    for view in (planes, channels_of_a_wider_map):
+        for a, b in zip(both(view), want):
+            assert torch.equal(a, b), view.__name__
+    for a, b in zip(both(odd), want):   # other vectors sum in another order
+        compare(a, b.double().cpu(), 2 * tolerance(a.dtype, 16 * 120), "odd")
+    ones = torch.ones((), device=device, dtype=dtype).expand(2, 32, 12, 10)
+    leaves = [t.clone().requires_grad_() for t in (x, weight, bias)]
+    for a, b in zip(_run(leaves, 2, "silu", ones), _run(leaves, 2, "silu", ones.contiguous())):
+        assert torch.equal(a, b)
+
+
+def test_parameters_of_other_types_and_unwanted_gradients(device):
+    from visionhope_amd.utils.group_norm import visionhope_group_norm
+
+    x, weight, bias = (t.to(device) for t in _inputs((2, 16, 8, 8), torch.bfloat16, seed=50))
+    x, dy = _last(x), _last(randn(2, 16, 8, 8, seed=51).to(device, torch.bfloat16))
+    half = weight.bfloat16().requires_grad_()
+    y = visionhope_group_norm(x, 2, half, bias, EPS, activation="silu")
+    (got,) = torch.autograd.grad(y, half, dy)
+    full = half.detach().float().requires_grad_()
+    want_y = visionhope_group_norm(x, 2, full, bias, EPS, activation="silu")
+    (want,) = torch.autograd.grad(want_y, full, dy)
+    assert got.dtype == torch.bfloat16 and torch.equal(y, want_y) and torch.equal(got, want.bfloat16())
+    with torch.no_grad():
+        assert torch.equal(visionhope_group_norm(x, 2, half, bias, EPS, activation="silu"), y)
+
+
+def test_repeats_bit_by_bit_on_any_stream_and_in_a_graph(device):
+    x, weight, bias = (t.to(device) for t in _inputs((6, 96, 40, 40), torch.bfloat16, seed=60))
+    x, dy = _last(x), _last(randn(6, 96, 40, 40, seed=61).to(device, torch.bfloat16))
+    leaves = [t.clone().requires_grad_() for t in (x, weight, bias)]
+
+    def step():
+        return _run(leaves, 6, "gelu", dy)
+
+    want = step()
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(side):
+        other = step()
+    torch.cuda.current_stream(device).wait_stream(side)
+    torch.cuda.synchronize()
+    for a, b in zip(want, other):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for round_ in range(3):
+        with torch.no_grad():
+            leaves[0].copy_(x * (round_ + 1) + round_)
+        want = step()
+        for t in captured:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, captured):
+            assert torch.equal(a, b), f"replay {round_}"
+
+
+def test_gradients_against_differences(device):
+    from visionhope_amd.utils.group_norm import visionhope_group_norm
+
+    x, weight, bias = (t.to(device) for t in _inputs((2, 24, 6, 5), torch.float32, seed=70))
+    dy = randn(2, 24, 6, 5, seed=71).to(device)
+    for activation in ACTIVATIONS:
+        leaves = [t.clone().requires_grad_() for t in (_last(x), weight, bias)]
+
+        def total(tensors):
+            return (visionhope_group_norm(tensors[0], 3, *tensors[1:], EPS, activation=activation).double() * dy).sum()
+
+        grads = torch.autograd.grad(total(leaves), leaves)
+        with torch.no_grad():
+            for at, grad in enumerate(grads):
+                direction, step = randn(*grad.shape, seed=72 + at).to(device), 2.0 ** -7
+                values = []
+                for sign in (1, -1):
+                    other = list(leaves)
+                    other[at] = leaves[at] + sign * step * direction
+                    values.append(total(other))
+                slope = ((values[0] - values[1]) / (2 * step)).item()
+                expected = (grad.double() * direction).sum().item()
+                # third derivatives of order one: step^2 = 6e-5 of the terms; outputs round at 2^-24 of
+                # themselves, over the step 1e-5
+                assert abs(slope - expected) <= 1e-3 * (grad.double() * direction).norm().item() + 1e-4 * abs(expected)
+
+
+def test_refusals(device):
+    from visionhope_amd.utils.group_norm import visionhope_group_norm as norm
+
+    x, weight, bias = (t.to(device) for t in _inputs((2, 16, 3, 3), torch.float32, seed=80))
+    wide = torch.zeros(1, 2050, 1, 1, device=device)
+    many = torch.zeros(2050, device=device)
+    bad = [
+        (ValueError, "CUDA", lambda: norm(x.cpu(), 2, weight, bias)),
+        (TypeError, "FP16, BF16 and FP32", lambda: norm(x.double(), 2, weight, bias)),
+        (ValueError, "4 dimensions", lambda: norm(x[0], 2, weight, bias)),
+        (ValueError, "nonempty", lambda: norm(x[:0], 2, weight, bias)),
+        (ValueError, "groups", lambda: norm(x, 3, weight, bias)),
+        (ValueError, "groups", lambda: norm(x, 0, weight, bias)),
+        (ValueError, "1024", lambda: norm(wide, 1, many, many)),
+        (ValueError, "activation", lambda: norm(x, 2, weight, bias, activation="relu")),
+        (ValueError, "weight", lambda: norm(x, 2, weight[:4], bias)),
+        (ValueError, "bias", lambda: norm(x, 2, weight, None)),
+        (TypeError, "weight", lambda: norm(x, 2, weight.int(), bias)),
+    ]
+    for error, match, call in bad:
+        with pytest.raises(error, match=match):
+            call()
+
+
+def test_forward_mode_is_refused_and_saved_tensors_may_change_strides(device):
+    from torch.autograd import forward_ad
+
+    from visionhope_amd.utils.group_norm import visionhope_group_norm
+
+    leaves = [t.to(device).requires_grad_() for t in _inputs((2, 16, 5, 5), torch.float32, seed=90)]
+    dy = randn(2, 16, 5, 5, seed=91).to(device)
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            with pytest.raises(NotImplementedError):
+                visionhope_group_norm(forward_ad.make_dual(leaves[0].detach(), torch.ones_like(leaves[0])), 2, *leaves[1:])
+    want = _run(leaves, 2, "silu", dy)
+
+    def spread(t):   # the same values, every other element of a wider tensor
+        wide = torch.zeros(*t.shape, 2, device=t.device, dtype=t.dtype)
+        wide[..., 0] = t
+        return wide[..., 0]
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread):
+        got = _run(leaves, 2, "silu", dy)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

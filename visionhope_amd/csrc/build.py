@@ -21,7 +21,7 @@ LIB_NAME = "libvisionhope_hip.so"
 SOURCES = ("vh_common.hip", "srnl.hip", "elementwise.hip", "dwconv.hip", "pointwise.hip", "conv3x3.hip", "srnl_backward.hip",
            "srnl_backward_blocks.hip", "linear_train.hip", "tail_backward.hip", "srnl_noalloc.hip", "srnl_wide.hip", "srnl_ut.hip", "srnl_utw.hip",
            "srnl_utw32.hip", "causal_conv.hip", "state_space.hip", "state_space_backward.hip", "row_norm.hip", "param_sum.hip",
-           "linear_attention.hip", "linear_attention_backward.hip")
+           "linear_attention.hip", "linear_attention_backward.hip", "group_norm.hip")
 ARCH = os.environ.get("VISIONHOPE_OFFLOAD_ARCH", "gfx950")
 
 # Packed-fp32 VALU ops are disabled for all device code (hipcc's host pass

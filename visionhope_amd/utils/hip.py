@@ -48,6 +48,8 @@ EXPORTED_SYMBOLS = (
     "vh_gated_layernorm_forward", "vh_gated_layernorm_backward_workspace_bytes", "vh_gated_layernorm_backward",
     "vh_linear_attention_workspace_bytes", "vh_linear_attention_forward",
     "vh_linear_attention_backward_workspace_bytes", "vh_linear_attention_backward", "vh_linear_attention_step",
+    "vh_group_norm_workspace_bytes", "vh_group_norm_forward", "vh_group_norm_backward_workspace_bytes",
+    "vh_group_norm_backward",
 )
 
 
@@ -193,6 +195,12 @@ _SIGNATURES = {
         _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
     "vh_linear_attention_step": (ctypes.c_int, [
         _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _f32, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "vh_group_norm_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32]),
+    "vh_group_norm_forward": (ctypes.c_int, [
+        _vp, _i32, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _vp, _sz, _vp]),
+    "vh_group_norm_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32]),
+    "vh_group_norm_backward": (ctypes.c_int, [
+        _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
 }
 
 _LIB = None
