@@ -10,6 +10,8 @@
 // a 16x16x32 tile where the FP32 matrix instructions take 256.
 #pragma once
 
+#include <initializer_list>
+
 #include "vh_common.h"
 
 namespace vh {
@@ -109,69 +111,81 @@ struct LADecay {
     }
 };
 
-// Four values of a tensor as loaded.
-template <typename T> struct LAQuad { uint2 u; };
-template <> struct LAQuad<float> { float4 f; };
+// Eight values of a tensor's row as loaded.
+template <typename T> struct LAOct { uint4 u; };
+template <> struct LAOct<float> { float4 a, b; };
 
-// Values col .. col + 3 of a row of `dim`, zeros behind it; `wide`: one load (dim and addresses are
-// multiples of four elements).
+// Values col .. col + 7 of a row of `dim`, zeros behind it.  `vec`: elements that one load may take
+// (8, 4 or 1), by dim, strides and addresses.
 template <typename T>
-__device__ __forceinline__ LAQuad<T> la_load(const T* row, int32_t col, int32_t dim, bool wide, bool live) {
-    LAQuad<T> r{};
-    if (!live || col >= dim) return r;
-    if (wide) {
-        if constexpr (sizeof(T) == 4) r.f = *reinterpret_cast<const float4*>(row + col);
-        else r.u = *reinterpret_cast<const uint2*>(row + col);
+__device__ __forceinline__ LAOct<T> la_load(const T* row, int32_t col, int32_t dim, int32_t vec) {
+    LAOct<T> r{};
+    if (col >= dim) return r;
+    if (vec == 8) {
+        if constexpr (sizeof(T) == 4) {
+            r.a = *reinterpret_cast<const float4*>(row);
+            r.b = *reinterpret_cast<const float4*>(row + 4);
+        } else {
+            r.u = *reinterpret_cast<const uint4*>(row);
+        }
         return r;
     }
+    if (vec == 4) {
+        if constexpr (sizeof(T) == 4) {
+            r.a = *reinterpret_cast<const float4*>(row);
+            if (col + 4 < dim) r.b = *reinterpret_cast<const float4*>(row + 4);
+        } else {
+            const uint2 lo = *reinterpret_cast<const uint2*>(row);
+            uint2 hi = make_uint2(0, 0);
+            if (col + 4 < dim) hi = *reinterpret_cast<const uint2*>(row + 4);
+            r.u = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+        return r;
+    }
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < dim ? row[i] : T{};
     if constexpr (sizeof(T) == 4) {
-        r.f.x = row[col];
-        if (col + 1 < dim) r.f.y = row[col + 1];
-        if (col + 2 < dim) r.f.z = row[col + 2];
-        if (col + 3 < dim) r.f.w = row[col + 3];
+        r.a = make_float4(v[0], v[1], v[2], v[3]);
+        r.b = make_float4(v[4], v[5], v[6], v[7]);
     } else {
-        r.u.x = row[col].bits;
-        if (col + 1 < dim) r.u.x |= static_cast<uint32_t>(row[col + 1].bits) << 16;
-        if (col + 2 < dim) r.u.y = row[col + 2].bits;
-        if (col + 3 < dim) r.u.y |= static_cast<uint32_t>(row[col + 3].bits) << 16;
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = v[2 * i].bits | static_cast<uint32_t>(v[2 * i + 1].bits) << 16;
+        r.u = make_uint4(w[0], w[1], w[2], w[3]);
     }
     return r;
 }
 
-// A quad as limbs: words (0, 1) and (2, 3) of each.
+// The eight values as limbs.
 template <typename T>
-__device__ __forceinline__ void la_limbs(const LAQuad<T>& q, uint2 (&out)[LAType<T>::raw]) {
+__device__ __forceinline__ void la_limbs(const LAOct<T>& q, uint4 (&out)[LAType<T>::raw]) {
     if constexpr (std::is_same<T, bf16_t>::value) {
         out[0] = q.u;
     } else {
-        float v[4];
+        float v[8];
         if constexpr (sizeof(T) == 4) {
-            v[0] = q.f.x; v[1] = q.f.y; v[2] = q.f.z; v[3] = q.f.w;
+            v[0] = q.a.x; v[1] = q.a.y; v[2] = q.a.z; v[3] = q.a.w;
+            v[4] = q.b.x; v[5] = q.b.y; v[6] = q.b.z; v[7] = q.b.w;
         } else {
-            v[0] = to_f32(T{static_cast<uint16_t>(q.u.x & 0xffffu)});
-            v[1] = to_f32(T{static_cast<uint16_t>(q.u.x >> 16)});
-            v[2] = to_f32(T{static_cast<uint16_t>(q.u.y & 0xffffu)});
-            v[3] = to_f32(T{static_cast<uint16_t>(q.u.y >> 16)});
-        }
-        uint32_t a[LAType<T>::raw], b[LAType<T>::raw];
-        la_split<LAType<T>::raw>(v[0], v[1], a);
-        la_split<LAType<T>::raw>(v[2], v[3], b);
+            const uint32_t w[4] = {q.u.x, q.u.y, q.u.z, q.u.w};
 #pragma unroll
-        for (int l = 0; l < LAType<T>::raw; ++l) out[l] = make_uint2(a[l], b[l]);
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = to_f32(T{static_cast<uint16_t>(w[i] & 0xffffu)});
+                v[2 * i + 1] = to_f32(T{static_cast<uint16_t>(w[i] >> 16)});
+            }
+        }
+        la_split8<LAType<T>::raw>(v, out);
     }
 }
 
-// The low (high) halves of two words as one.
-__device__ __forceinline__ uint32_t la_lows(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
-__device__ __forceinline__ uint32_t la_highs(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
-
-// Stores four values of a row.
+// Stores values col .. col + 3 of a row of `dim` at `row`; `wide`: as one.
 template <typename T>
 __device__ __forceinline__ void la_store(T* row, int32_t col, int32_t dim, bool wide, const float (&v)[4]) {
     if (wide) {
         if (col >= dim) return;
         if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4*>(row + col) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(row) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
             uint2 w;
             if constexpr (std::is_same<T, bf16_t>::value) {
@@ -180,61 +194,73 @@ __device__ __forceinline__ void la_store(T* row, int32_t col, int32_t dim, bool 
                 w.x = from_f32<T>(v[0]).bits | static_cast<uint32_t>(from_f32<T>(v[1]).bits) << 16;
                 w.y = from_f32<T>(v[2]).bits | static_cast<uint32_t>(from_f32<T>(v[3]).bits) << 16;
             }
-            *reinterpret_cast<uint2*>(row + col) = w;
+            *reinterpret_cast<uint2*>(row) = w;
         }
         return;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (col + i < dim) row[col + i] = from_f32<T>(v[i]);
+        if (col + i < dim) row[i] = from_f32<T>(v[i]);
 }
 
-// Tiles of a chunk in LDS, for heads padded to D.
+// Tiles of a chunk in LDS, for heads padded to D: rows of tokens, eight values longer than they
+// need, so that the 16-byte reads of 16 rows spread over all banks.
 template <typename T, int D>
 struct LAShape {
     static constexpr int R = LAType<T>::raw, F = LAType<T>::formed, C = LAType<T>::tokens;
-    static constexpr int waves = D / 16, threads = 64 * waves;
-    // rows of LDS tiles, eight values longer than they need: 16 rows' 16-byte reads spread over all banks
+    static constexpr int waves = D / 16, threads = 64 * waves, units = C / 32;   // units: of eight values a thread
     static constexpr int row_d = D + 8, row_c = C + 8;
-    static constexpr int tokens_tile = C * row_d, turned_tile = D * row_c, weights_tile = C * row_c;
-    static constexpr int state_lds = (2 * R * turned_tile) * 2 + 512;
-    static constexpr int lds = state_lds + (2 * R * tokens_tile + F * weights_tile) * 2;
+    static constexpr int tile = C * row_d, weights = C * row_c;   // one limb
+    static constexpr int head = 512;                              // bytes of small tables
+    static constexpr int state_lds = head + 2 * R * tile * 2;
+    static constexpr int lds = head + (3 * R * tile + F * weights) * 2;
 };
 
-// Four columns 4 cu .. + 3 of C / 16 tokens (the tu-th such run) into `rows` (tokens' rows; the index
-// 32 x + 16 h + 4 y + r stands at 32 x + 8 y + 4 h + r, the order in which two tiles of accumulators
-// have it) and into `turned` (columns' rows); either may be null.
-template <typename T, int D>
-__device__ __forceinline__ void la_stage(const LAQuad<T> (&raw)[LAShape<T, D>::C / 16], uint16_t* rows, uint16_t* turned,
-                                         int32_t cu, int32_t tu) {
+// Where value d of a row stands that a product with the state contracts over: d = 32 x + 16 h + 4 y + r
+// at 32 x + 8 y + 4 h + r, the order in which two tiles of accumulators have it.
+__device__ __forceinline__ int32_t la_place(int32_t d) {
+    return (d & ~31) + ((d & 15) >> 2) * 8 + ((d >> 4) & 1) * 4 + (d & 3);
+}
+
+// Eight values col .. col + 7 of token i into a tile; PLACED: in the order above.
+template <typename T, int D, bool PLACED>
+__device__ __forceinline__ void la_stage(const LAOct<T>& raw, uint16_t* tile, int32_t col, int32_t i) {
     using P = LAShape<T, D>;
-    constexpr int UNIT = P::C / 16;
-    const int32_t in = (4 * cu) & 31, place = ((4 * cu) & ~31) + ((in & 15) >> 2) * 8 + (in >> 4) * 4;
-    uint2 limbs[UNIT][P::R];
-#pragma unroll
-    for (int u = 0; u < UNIT; ++u) la_limbs<T>(raw[u], limbs[u]);
+    uint4 limbs[P::R];
+    la_limbs<T>(raw, limbs);
 #pragma unroll
     for (int l = 0; l < P::R; ++l) {
-        if (rows != nullptr) {
-#pragma unroll
-            for (int u = 0; u < UNIT; ++u)
-                *reinterpret_cast<uint2*>(rows + l * P::tokens_tile + (tu * UNIT + u) * P::row_d + place) = limbs[u][l];
+        uint16_t* row = tile + l * P::tile + i * P::row_d;
+        if constexpr (PLACED) {
+            *reinterpret_cast<uint2*>(row + la_place(col)) = make_uint2(limbs[l].x, limbs[l].y);
+            *reinterpret_cast<uint2*>(row + la_place(col + 4)) = make_uint2(limbs[l].z, limbs[l].w);
+        } else {
+            *reinterpret_cast<uint4*>(row + col) = limbs[l];
         }
-        if (turned != nullptr) {
-            uint16_t* to = turned + l * P::turned_tile + 4 * cu * P::row_c + tu * UNIT;
+    }
+}
+
+typedef short la_i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) la_i16x4 la_lds_i16x4;
+
+// A column of a tile over eight tokens, of every limb: lane l gets column 16 m + l % 16 at tokens
+// 32 x + 8 (l / 16) .. + 7.  The transposing read takes four tokens' rows from the four quarters of
+// a 16-lane group and gives each lane one column of them.  `at`: la_column<PLACED>.
+template <bool PLACED>
+__device__ __forceinline__ int32_t la_column(int32_t lane, int32_t row_d) {
+    return (8 * (lane >> 4) + ((lane & 15) >> 2)) * row_d + (lane & 3) * (PLACED ? 8 : 4);
+}
+template <typename T, int D, bool PLACED>
+__device__ __forceinline__ void la_turned(const uint16_t* tile, int32_t at, int32_t x, int32_t m, uint4 (&out)[LAShape<T, D>::R]) {
+    using P = LAShape<T, D>;
+    const int32_t of_tile = PLACED ? 32 * (m >> 1) + 4 * (m & 1) : 16 * m;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t w[UNIT / 2];
-#pragma unroll
-                for (int u = 0; u < UNIT / 2; ++u) {
-                    const uint32_t x = c < 2 ? limbs[2 * u][l].x : limbs[2 * u][l].y;
-                    const uint32_t y = c < 2 ? limbs[2 * u + 1][l].x : limbs[2 * u + 1][l].y;
-                    w[u] = c & 1 ? la_highs(x, y) : la_lows(x, y);
-                }
-                if constexpr (UNIT == 4) *reinterpret_cast<uint2*>(to + c * P::row_c) = make_uint2(w[0], w[UNIT / 2 - 1]);
-                else *reinterpret_cast<uint32_t*>(to + c * P::row_c) = w[0];
-            }
-        }
+    for (int l = 0; l < P::R; ++l) {
+        const uint16_t* from = tile + l * P::tile + at + 32 * x * P::row_d + of_tile;
+        const la_i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_i16x4*)from);
+        const la_i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_i16x4*)(from + 4 * P::row_d));
+        const uint2 ua = __builtin_bit_cast(uint2, a), ub = __builtin_bit_cast(uint2, b);
+        out[l] = make_uint4(ua.x, ua.y, ub.x, ub.y);
     }
 }
 
@@ -258,7 +284,8 @@ struct LAPass {
     const int32_t* lengths;
     float* slots;            // [B, heads, segments - 1, D * D]: states between the segments
     int32_t batches, tokens, heads, kdim, vdim, segments, chunks_per_segment, chunk, reversed;
-    bool wide_q, wide_k, wide_v, wide_out;
+    int32_t vec_q, vec_k, vec_v;   // elements of one load
+    bool wide_out;
 };
 
 // Tokens of a sequence.
@@ -276,6 +303,7 @@ struct LACut {   // segments of a line, and chunks of each (the last may have fe
 LACut la_cut(int64_t heads, int64_t N, int32_t padded, int32_t io_dtype);
 size_t la_slots_bytes(int64_t heads, const LACut& cut, int32_t padded);
 int la_check_sizes(int32_t io_dtype, int64_t B, int64_t N, int64_t heads, int64_t key_dim, int64_t value_dim);
+int la_check_strides(std::initializer_list<int64_t> token_strides);   // below 2^24 elements
 // Runs a pass (sets its widths and its chunk itself); la_states: only as far as the states between
 // the segments.
 int la_run(LAPass& a, int32_t io_dtype, hipStream_t stream);
@@ -288,9 +316,14 @@ inline int32_t la_padded(int64_t key_dim, int64_t value_dim) {
     const int64_t d = key_dim > value_dim ? key_dim : value_dim;
     return d <= 32 ? 32 : d <= 64 ? 64 : 128;
 }
-// Whether four elements of a row are one load.
-inline bool la_wide(const LATokens& t, int64_t dim, int64_t e) {
-    return dim % 4 == 0 && reinterpret_cast<uintptr_t>(t.data) % (4 * e) == 0 && t.bs % 4 == 0 && t.ts % 4 == 0 && t.hs % 4 == 0;
+// Elements that one load of a row takes.
+inline int32_t la_vec(const LATokens& t, int64_t dim, int64_t e) {
+    for (int64_t v : {8, 4}) {
+        const uintptr_t bytes = v * e < 16 ? v * e : 16;
+        if (dim % v == 0 && reinterpret_cast<uintptr_t>(t.data) % bytes == 0 && t.bs % v == 0 && t.ts % v == 0 && t.hs % v == 0)
+            return static_cast<int32_t>(v);
+    }
+    return 1;
 }
 inline int32_t la_chunk(int32_t io_dtype) { return io_dtype == VH_DTYPE_BF16 ? 64 : 32; }
 

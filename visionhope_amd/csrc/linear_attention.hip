@@ -21,22 +21,27 @@
 namespace vh {
 namespace {
 
+// A tile (query tile, key tile) of the lower triangle by its number.
+__device__ __forceinline__ void la_triangle(int32_t tile, int32_t& it, int32_t& jt) {
+    it = static_cast<int32_t>((0x3333222110ull >> (4 * tile)) & 15);
+    jt = tile - it * (it + 1) / 2;
+}
+
 // Walks a segment's chunks.  OUT: writes outputs; otherwise the segment's last state only.
 template <typename T, int D, bool OUT>
-__global__ __launch_bounds__(4 * D) void linear_attention_kernel(const LAPass a) {
+__global__ __launch_bounds__(4 * D, D == 128 ? 4 : 3) void linear_attention_kernel(const LAPass a) {
     using P = LAShape<T, D>;
     constexpr int R = P::R, F = P::F, C = P::C, ORDER = LAType<T>::order;
-    constexpr int TILES = C / 16, STEPS_C = C / 32, STEPS_D = D / 32, UNIT = C / 16;
+    constexpr int TILES = C / 16, STEPS_C = C / 32, STEPS_D = D / 32, UNITS = P::units;
     extern __shared__ __align__(16) unsigned char la_lds[];
-    float* powers = reinterpret_cast<float*>(la_lds);                       // [C + 1]
-    uint16_t* kt = reinterpret_cast<uint16_t*>(la_lds + 512);               // [R][D][C]: keys, turned
-    uint16_t* vt = kt + R * P::turned_tile;                                 // [R][D][C]: values, turned
-    uint16_t* qs = vt + R * P::turned_tile;                                 // [R][C][D]: key index in the states' order
-    uint16_t* ks = qs + R * P::tokens_tile;                                 // [R][C][D]: the same
-    uint16_t* ws = ks + R * P::tokens_tile;                                 // [F][C][C]: weights
+    float* entering = reinterpret_cast<float*>(la_lds);                     // [C]: weights of what enters the state
+    uint16_t* ks = reinterpret_cast<uint16_t*>(la_lds + P::head);           // [R][C][D], placed
+    uint16_t* vs = ks + R * P::tile;                                        // [R][C][D]
+    uint16_t* qs = vs + R * P::tile;                                        // [R][C][D], placed
+    uint16_t* ws = qs + R * P::tile;                                        // [F][C][C]: weights of pairs
 
-    const int32_t tid = static_cast<int32_t>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
-    const int32_t n16 = lane & 15, g = lane >> 4;
+    const int32_t tid = static_cast<int32_t>(threadIdx.x), lane = tid & 63;
+    const int32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
     // heads of a token stand side by side in memory: neighbours run on one XCD
     const uint32_t bid = xcd_remap_any(blockIdx.x, gridDim.x);
     const int32_t head = static_cast<int32_t>(bid % static_cast<uint32_t>(a.heads));
@@ -46,16 +51,56 @@ __global__ __launch_bounds__(4 * D) void linear_attention_kernel(const LAPass a)
     // states are wanted of all segments but the walk's last one
     const int32_t segment = static_cast<int32_t>(rest % static_cast<uint32_t>(count)) + (!OUT && a.reversed ? 1 : 0);
     const int64_t bh = static_cast<int64_t>(batch) * a.heads + head;
-    const int32_t end = la_end(a, batch);
+    const int32_t end = __builtin_amdgcn_readfirstlane(la_end(a, batch));
     const int32_t length = a.chunks_per_segment * C;
     const int32_t from = segment * length;
     const int32_t to = a.tokens - from < length ? a.tokens : from + length;      // of all tokens
     const int32_t stop = end < from ? from : end < to ? end : to;                // of the sequence's
     const int32_t last = end > 0 ? (end - 1) / length : 0;                       // segment of the last token
+    const int32_t chunks = (stop - from + C - 1) / C;
+    const int32_t shift = a.reversed ? 1 : 0;
     const LADecay decay(a.log_decay[head]);
-    if (tid <= C) powers[tid] = decay.power(static_cast<float>(tid));
-    if constexpr (OUT) {   // weights of later tokens that share 32 columns with earlier ones stay zero
-        for (int32_t i = tid; i < F * P::weights_tile / 2; i += P::threads) reinterpret_cast<uint32_t*>(ws)[i] = 0;
+
+    // staging: a thread takes eight columns of tokens `row`, row + 32, ... of each tensor
+    const int32_t col = tid % (D / 8) * 8, row = tid / (D / 8);
+    const T* qp = static_cast<const T*>(a.q.data) + batch * a.q.bs + head * a.q.hs;
+    const T* kp = static_cast<const T*>(a.k.data) + batch * a.k.bs + head * a.k.hs;
+    const T* vp = static_cast<const T*>(a.v.data) + batch * a.v.bs + head * a.v.hs;
+    LAOct<T> rq[UNITS], rk[UNITS], rv[UNITS];
+    auto fetch = [&](int32_t chunk) {
+        const int32_t t0 = from + chunk * C, nt = stop - t0 < C ? stop - t0 : C;
+        const T *q = qp + t0 * a.q.ts, *k = kp + t0 * a.k.ts, *v = vp + t0 * a.v.ts;
+        // offsets within a chunk fit 32 bits (token strides below 2^24)
+        const uint32_t qt = static_cast<uint32_t>(a.q.ts), kt = static_cast<uint32_t>(a.k.ts), vt = static_cast<uint32_t>(a.v.ts);
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            const int32_t i = row + 32 * u;
+            const uint32_t t = static_cast<uint32_t>(a.reversed ? nt - 1 - i : i);
+            if (OUT) rq[u] = LAOct<T>{};
+            rk[u] = rv[u] = LAOct<T>{};
+            if (i < nt) {
+                if constexpr (OUT) rq[u] = la_load(q + (t * qt + col), col, a.kdim, a.vec_q);
+                rk[u] = la_load(k + (t * kt + col), col, a.kdim, a.vec_k);
+                rv[u] = la_load(v + (t * vt + col), col, a.vdim, a.vec_v);
+            }
+        }
+    };
+    if (chunks > 0) fetch(a.reversed ? chunks - 1 : 0);
+
+    // powers of the decay that a lane needs in every chunk
+    float diagonal[4], below[4], leaving[TILES];
+    const float p16 = decay.power(16.f), p32 = decay.power(32.f);
+    if constexpr (OUT) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int32_t d = n16 - 4 * g - r;   // of a pair in a tile on the diagonal; 16 more in the next one
+            diagonal[r] = d >= 0 ? decay.power(static_cast<float>(d)) * a.scale_weight : 0.f;
+            below[r] = decay.power(static_cast<float>(d + 16)) * a.scale_weight;
+        }
+#pragma unroll
+        for (int it = 0; it < TILES; ++it) leaving[it] = decay.power(static_cast<float>(16 * it + n16 + 1 - shift)) * a.scale_out;
+        // weights of later tokens that share 32 columns with earlier ones stay zero
+        for (int32_t i = tid; i < F * P::weights / 2; i += P::threads) reinterpret_cast<uint32_t*>(ws)[i] = 0;
     }
 
     // the state: key rows 16 m + 4 g .. + 3, value column 16 wave + n16
@@ -81,62 +126,57 @@ __global__ __launch_bounds__(4 * D) void linear_attention_kernel(const LAPass a)
         for (int m = 0; m < D / 16; ++m) s[m] = at[m * 64];
     }
 
-    // staging: a thread takes four columns of UNIT tokens of each tensor
-    const int32_t cu = tid % (D / 4), tu = tid / (D / 4);
-    const T* qp = static_cast<const T*>(a.q.data) + batch * a.q.bs + head * a.q.hs;
-    const T* kp = static_cast<const T*>(a.k.data) + batch * a.k.bs + head * a.k.hs;
-    const T* vp = static_cast<const T*>(a.v.data) + batch * a.v.bs + head * a.v.hs;
-    LAQuad<T> rq[UNIT], rk[UNIT], rv[UNIT];
-    const int32_t chunks = (stop - from + C - 1) / C;
-    auto fetch = [&](int32_t chunk) {
-        const int32_t t0 = from + chunk * C, nt = stop - t0 < C ? stop - t0 : C;
-#pragma unroll
-        for (int u = 0; u < UNIT; ++u) {
-            const int32_t i = tu * UNIT + u;
-            const int64_t t = a.reversed ? t0 + nt - 1 - i : t0 + i;
-            const bool live = i < nt;
-            if constexpr (OUT) rq[u] = la_load(qp + t * a.q.ts, 4 * cu, a.kdim, a.wide_q, live);
-            rk[u] = la_load(kp + t * a.k.ts, 4 * cu, a.kdim, a.wide_k, live);
-            rv[u] = la_load(vp + t * a.v.ts, 4 * cu, a.vdim, a.wide_v, live);
-        }
-    };
-    if (chunks > 0) fetch(a.reversed ? chunks - 1 : 0);
-    const int32_t shift = a.reversed ? 1 : 0;
+    const int32_t at_row = n16 * P::row_d + 8 * g, at_weights = n16 * P::row_c + 8 * g;
+    const int32_t k_column = la_column<true>(lane, P::row_d), v_column = la_column<false>(lane, P::row_d);
+    int32_t entered = 0;   // the chunk length that `entering` stands for
     for (int32_t step = 0; step < chunks; ++step) {
         const int32_t chunk = a.reversed ? chunks - 1 - step : step;
         const int32_t t0 = from + chunk * C, nt = stop - t0 < C ? stop - t0 : C;
         __syncthreads();   // the last chunk's tiles have been read
-        if constexpr (OUT) la_stage<T, D>(rq, qs, nullptr, cu, tu);
-        la_stage<T, D>(rk, OUT ? ks : nullptr, kt, cu, tu);
-        la_stage<T, D>(rv, nullptr, vt, cu, tu);
+        if (nt != entered) {
+            if (tid < C) entering[tid] = tid < nt ? decay.power(static_cast<float>(nt - 1 - tid + shift)) * a.scale_in : 0.f;
+            entered = nt;
+        }
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            if constexpr (OUT) la_stage<T, D, true>(rq[u], qs, col, row + 32 * u);
+            la_stage<T, D, true>(rk[u], ks, col, row + 32 * u);
+            la_stage<T, D, false>(rv[u], vs, col, row + 32 * u);
+        }
         if (step + 1 < chunks) fetch(a.reversed ? chunk - 1 : chunk + 1);
         __syncthreads();
 
         la_f32x4 o[TILES];
         if constexpr (OUT) {
             // weights of the pairs (query tile it, key tile jt <= it), a tile a wave
-            for (int32_t tile = wave; tile < TILES * (TILES + 1) / 2; tile += P::waves) {
-                int32_t it = 0;
-                while ((it + 1) * (it + 2) / 2 <= tile) ++it;
-                const int32_t jt = tile - it * (it + 1) / 2;
+#pragma unroll
+            for (int32_t first = 0; first < TILES * (TILES + 1) / 2; first += P::waves) {
+                const int32_t tile = first + wave;
+                if (tile >= TILES * (TILES + 1) / 2) break;
+                int32_t it, jt;
+                la_triangle(tile, it, jt);
                 la_f32x4 w = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int x = 0; x < STEPS_D; ++x) {
                     uint4 ka[R], qa[R];
-                    la_read(ks, P::tokens_tile, (16 * jt + n16) * P::row_d + 32 * x + 8 * g, ka);
-                    la_read(qs, P::tokens_tile, (16 * it + n16) * P::row_d + 32 * x + 8 * g, qa);
+                    la_read(ks, P::tile, 16 * jt * P::row_d + at_row + 32 * x, ka);
+                    la_read(qs, P::tile, 16 * it * P::row_d + at_row + 32 * x, qa);
                     w = la_mm<(R == 1 ? 0 : 2)>(ka, qa, w);
                 }
-                const int32_t i = 16 * it + n16, j = 16 * jt + 4 * g;
-                float v[4];
+                if (it == jt) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = j + r <= i ? w[r] * (powers[i - j - r < 0 ? 0 : i - j - r] * a.scale_weight) : 0.f;
+                    for (int r = 0; r < 4; ++r) w[r] = n16 < 4 * g + r ? 0.f : w[r] * diagonal[r];
+                } else {
+                    const float p = it - jt == 1 ? 1.f : it - jt == 2 ? p16 : p32;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) w[r] *= below[r] * p;
+                }
                 uint32_t lo[F], hi[F];
-                la_split<F>(v[0], v[1], lo);
-                la_split<F>(v[2], v[3], hi);
+                la_split<F>(w[0], w[1], lo);
+                la_split<F>(w[2], w[3], hi);
 #pragma unroll
                 for (int l = 0; l < F; ++l)
-                    *reinterpret_cast<uint2*>(ws + l * P::weights_tile + i * P::row_c + j) = make_uint2(lo[l], hi[l]);
+                    *reinterpret_cast<uint2*>(ws + l * P::weights + (16 * it + n16) * P::row_c + 16 * jt + 4 * g) = make_uint2(lo[l], hi[l]);
             }
             // what comes from the state: value rows, token columns
 #pragma unroll
@@ -150,22 +190,20 @@ __global__ __launch_bounds__(4 * D) void linear_attention_kernel(const LAPass a)
 #pragma unroll
                 for (int it = 0; it < TILES; ++it) {
                     uint4 qa[R];
-                    la_read(qs, P::tokens_tile, (16 * it + n16) * P::row_d + 32 * x + 8 * g, qa);
+                    la_read(qs, P::tile, 16 * it * P::row_d + at_row + 32 * x, qa);
                     o[it] = la_mm<ORDER>(sa, qa, o[it]);
                 }
             }
 #pragma unroll
-            for (int it = 0; it < TILES; ++it) {
-                const float p = powers[16 * it + n16 + 1 - shift] * a.scale_out;
+            for (int it = 0; it < TILES; ++it)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[it][r] *= p;
-            }
+                for (int r = 0; r < 4; ++r) o[it][r] *= leaving[it];
         }
         // the state behind the chunk
         uint4 va[STEPS_C][R];
 #pragma unroll
-        for (int x = 0; x < STEPS_C; ++x) la_read(vt, P::turned_tile, column * P::row_c + 32 * x + 8 * g, va[x]);
-        const float whole = powers[nt];
+        for (int x = 0; x < STEPS_C; ++x) la_turned<T, D, false>(vs, v_column, x, wave, va[x]);
+        const float whole = decay.power(static_cast<float>(nt));
 #pragma unroll
         for (int m = 0; m < D / 16; ++m)
 #pragma unroll
@@ -174,17 +212,16 @@ __global__ __launch_bounds__(4 * D) void linear_attention_kernel(const LAPass a)
         for (int x = 0; x < STEPS_C; ++x) {
             float v[8];
             la_join8<R>(va[x], v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int32_t m = nt - 1 - (32 * x + 8 * g + i) + shift;
-                v[i] *= powers[m < 0 ? 0 : m] * a.scale_in;
-            }
+            const float4 e0 = *reinterpret_cast<const float4*>(entering + 32 * x + 8 * g);
+            const float4 e1 = *reinterpret_cast<const float4*>(entering + 32 * x + 8 * g + 4);
+            v[0] *= e0.x; v[1] *= e0.y; v[2] *= e0.z; v[3] *= e0.w;
+            v[4] *= e1.x; v[5] *= e1.y; v[6] *= e1.z; v[7] *= e1.w;
             uint4 vw[LA_STATE_LIMBS];
             la_split8<LA_STATE_LIMBS>(v, vw);
 #pragma unroll
             for (int m = 0; m < D / 16; ++m) {
                 uint4 ka[R];
-                la_read(kt, P::turned_tile, (16 * m + n16) * P::row_c + 32 * x + 8 * g, ka);
+                la_turned<T, D, true>(ks, k_column, x, m, ka);
                 s[m] = la_mm<2>(ka, vw, s[m]);
             }
         }
@@ -196,19 +233,18 @@ __global__ __launch_bounds__(4 * D) void linear_attention_kernel(const LAPass a)
                 for (int x = 0; x < STEPS_C; ++x)
                     if (32 * x < 16 * (it + 1)) {
                         uint4 wa[F];
-#pragma unroll
-                        for (int l = 0; l < F; ++l)
-                            wa[l] = *reinterpret_cast<const uint4*>(ws + l * P::weights_tile + (16 * it + n16) * P::row_c + 32 * x + 8 * g);
+                        la_read(ws, P::weights, 16 * it * P::row_c + at_weights + 32 * x, wa);
                         o[it] = la_mm<ORDER>(va[x], wa, o[it]);
                     }
+            T* out = static_cast<T*>(a.out) + ((batch * static_cast<int64_t>(a.tokens) + t0) * a.heads + head) * a.vdim;
 #pragma unroll
             for (int it = 0; it < TILES; ++it) {
                 const int32_t i = 16 * it + n16;
                 if (i >= nt) continue;
-                const int64_t t = a.reversed ? t0 + nt - 1 - i : t0 + i;
+                const uint32_t t = static_cast<uint32_t>(a.reversed ? nt - 1 - i : i);
                 const float v[4] = {o[it][0], o[it][1], o[it][2], o[it][3]};
-                la_store(static_cast<T*>(a.out) + ((batch * static_cast<int64_t>(a.tokens) + t) * a.heads + head) * a.vdim,
-                         16 * wave + 4 * g, a.vdim, a.wide_out, v);
+                la_store(out + (t * static_cast<uint32_t>(a.heads * a.vdim) + 16 * wave + 4 * g), 16 * wave + 4 * g, a.vdim,
+                         a.wide_out, v);
             }
         }
     }
@@ -220,9 +256,11 @@ __global__ __launch_bounds__(4 * D) void linear_attention_kernel(const LAPass a)
         for (int m = 0; m < D / 16; ++m) at[m * 64] = s[m];
     } else {
         const float zeros[4] = {0.f, 0.f, 0.f, 0.f};   // tokens behind the sequence's end
-        for (int32_t t = stop + tu; t < to; t += 16)
-            la_store(static_cast<T*>(a.out) + ((batch * static_cast<int64_t>(a.tokens) + t) * a.heads + head) * a.vdim, 4 * cu,
-                     a.vdim, a.wide_out, zeros);
+        for (int32_t t = stop + row; t < to; t += 32)
+#pragma unroll
+            for (int c = 0; c < 8; c += 4)
+                la_store(static_cast<T*>(a.out) + ((batch * static_cast<int64_t>(a.tokens) + t) * a.heads + head) * a.vdim + col + c,
+                         col + c, a.vdim, a.wide_out, zeros);
         if (a.new_state != nullptr && (a.reversed ? segment == 0 : segment == last) && column < a.vdim) {
             float* at = a.new_state + bh * a.kdim * a.vdim + column * a.state_col;
 #pragma unroll
@@ -246,19 +284,26 @@ __global__ __launch_bounds__(256) void linear_attention_join_kernel(const LAPass
     const int32_t end = la_end(a, static_cast<int32_t>(bh / a.heads));
     float4* at = reinterpret_cast<float4*>(a.slots) + bh * slots * quads + index % quads;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int32_t i = 0; i < slots; ++i) {
+    constexpr int AHEAD = 8;   // loads in flight: the chain is over them, not over memory
+    for (int32_t i0 = 0; i0 < slots; i0 += AHEAD) {
+        float4 own[AHEAD];
         // slot i belongs to segment i + 1 of a reversed walk and to segment i of the other
-        const int32_t slot = a.reversed ? slots - 1 - i : i;
-        const int32_t first = (a.reversed ? slot + 1 : slot) * tokens;
-        int32_t n = end - first;
-        n = n < 0 ? 0 : n > tokens ? tokens : n;
-        const float p = decay.power(static_cast<float>(n));
-        const float4 own = at[static_cast<int64_t>(slot) * quads];
-        s.x = fmaf(s.x, p, own.x);
-        s.y = fmaf(s.y, p, own.y);
-        s.z = fmaf(s.z, p, own.z);
-        s.w = fmaf(s.w, p, own.w);
-        at[static_cast<int64_t>(slot) * quads] = s;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (i0 + i < slots) own[i] = at[static_cast<int64_t>(a.reversed ? slots - 1 - i0 - i : i0 + i) * quads];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (i0 + i >= slots) break;
+            const int32_t slot = a.reversed ? slots - 1 - i0 - i : i0 + i;
+            int32_t n = end - (a.reversed ? slot + 1 : slot) * tokens;
+            n = n < 0 ? 0 : n > tokens ? tokens : n;
+            const float p = decay.power(static_cast<float>(n));
+            s.x = fmaf(s.x, p, own[i].x);
+            s.y = fmaf(s.y, p, own[i].y);
+            s.z = fmaf(s.z, p, own[i].z);
+            s.w = fmaf(s.w, p, own[i].w);
+            at[static_cast<int64_t>(slot) * quads] = s;
+        }
     }
 }
 
@@ -288,9 +333,9 @@ int launch_typed(const LAPass& a, bool states, hipStream_t stream) {
 
 int run(LAPass& a, int32_t io_dtype, bool states, hipStream_t stream) {
     const int64_t e = dtype_bytes(io_dtype);
-    a.wide_q = la_wide(a.q, a.kdim, e);
-    a.wide_k = la_wide(a.k, a.kdim, e);
-    a.wide_v = la_wide(a.v, a.vdim, e);
+    a.vec_q = la_vec(a.q, a.kdim, e);
+    a.vec_k = la_vec(a.k, a.kdim, e);
+    a.vec_v = la_vec(a.v, a.vdim, e);
     a.wide_out = a.vdim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % (4 * e) == 0;
     a.chunk = la_chunk(io_dtype);
     if (io_dtype == VH_DTYPE_F32) return launch_typed<float>(a, states, stream);
@@ -303,12 +348,12 @@ int la_run(LAPass& a, int32_t io_dtype, hipStream_t stream) { return run(a, io_d
 int la_states(LAPass& a, int32_t io_dtype, hipStream_t stream) { return run(a, io_dtype, true, stream); }
 
 LACut la_cut(int64_t heads, int64_t N, int32_t padded, int32_t io_dtype) {
-    // Workgroups that the card holds at once (LDS: four, two and one a CU), and a half more, so
-    // that ragged segments even out.
-    const int64_t wanted = padded == 32 ? 1536 : padded == 64 ? 768 : 384;
+    // Workgroups that the card holds at once, by registers and LDS: one round of them, since a
+    // segment more than that waits for the end of another.
+    const int64_t held = padded == 32 ? 1024 : padded == 64 ? 768 : io_dtype == VH_DTYPE_F32 ? 256 : 512;
     const int64_t chunks = la_ceil(N, la_chunk(io_dtype));
-    int64_t segments = la_ceil(wanted, heads);
-    segments = segments < chunks ? segments : chunks;
+    int64_t segments = held / heads;
+    segments = segments < 1 ? 1 : segments < chunks ? segments : chunks;
     const int64_t each = la_ceil(chunks, segments);
     return {static_cast<int32_t>(la_ceil(chunks, each)), static_cast<int32_t>(each)};
 }
@@ -329,6 +374,14 @@ int la_check_sizes(int32_t io_dtype, int64_t B, int64_t N, int64_t heads, int64_
     VH_REQUIRE(N < (1ll << 30) && B < (1ll << 24) && heads < (1ll << 24) && B * heads < (1ll << 22), VH_ERR_SHAPE,
                "linear attention: %lld sequences of %lld heads and %lld tokens are out of range", (long long)B,
                (long long)heads, (long long)N);
+    VH_REQUIRE(heads * value_dim < (1ll << 24) && heads * key_dim < (1ll << 24), VH_ERR_SHAPE,
+               "linear attention: a token's %lld heads are out of range", (long long)heads);
+    return VH_OK;
+}
+
+int la_check_strides(std::initializer_list<int64_t> token_strides) {
+    for (int64_t t : token_strides)
+        VH_REQUIRE(t >= 0 && t < (1ll << 24), VH_ERR_SHAPE, "linear attention: a token stride of %lld is out of range", (long long)t);
     return VH_OK;
 }
 
@@ -437,6 +490,7 @@ int vh_linear_attention_forward(
     void* stream) {
     using namespace vh;
     if (int rc = la_check_sizes(io_dtype, B, N, heads, key_dim, value_dim)) return rc;
+    if (int rc = la_check_strides({q_token, k_token, v_token})) return rc;
     VH_REQUIRE(q != nullptr && k != nullptr && v != nullptr && log_decay != nullptr && out != nullptr, VH_ERR_ARG,
                "q, k, v, log_decay and out must not be null");
     VH_REQUIRE(!overlapping(state, new_state, B * heads * key_dim * value_dim * 4), VH_ERR_ARG,

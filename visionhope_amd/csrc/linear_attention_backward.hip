@@ -23,27 +23,18 @@ struct LADecayArgs {
     const int32_t* lengths;
     float scale;
     int32_t tokens, heads, kdim, vdim, chunks;
-    bool wide_q, wide_k, wide_v, wide_dout;
-};
-
-template <typename T, int D>
-struct LADecayShape {
-    using P = LAShape<T, D>;
-    // four tensors one after the other in two row tiles or two turned ones
-    static constexpr int tile = P::tokens_tile > P::turned_tile ? P::tokens_tile : P::turned_tile;
-    static constexpr int lds = 512 + 4 * P::R * tile * 2;
+    int32_t vec_q, vec_k, vec_v, vec_dout;   // elements of one load
 };
 
 // One chunk of one head: the share of a decay's gradient.
 template <typename T, int D>
-__global__ __launch_bounds__(4 * D) void linear_attention_decay_kernel(const LADecayArgs a) {
+__global__ __launch_bounds__(4 * D, 2) void linear_attention_decay_kernel(const LADecayArgs a) {
     using P = LAShape<T, D>;
-    constexpr int R = P::R, C = P::C, TILES = C / 16, STEPS_C = C / 32, STEPS_D = D / 32, UNIT = C / 16;
-    constexpr int TILE = LADecayShape<T, D>::tile * R;
+    constexpr int R = P::R, C = P::C, TILES = C / 16, STEPS_C = C / 32, STEPS_D = D / 32, TILE = P::tile * R;
     extern __shared__ __align__(16) unsigned char la_lds[];
     __shared__ float waves[P::waves];
     float* powers = reinterpret_cast<float*>(la_lds);
-    uint16_t* tiles = reinterpret_cast<uint16_t*>(la_lds + 512);
+    uint16_t* tiles = reinterpret_cast<uint16_t*>(la_lds + P::head);
     const int32_t tid = static_cast<int32_t>(threadIdx.x), lane = tid & 63, wave = tid >> 6, n16 = lane & 15, g = lane >> 4;
     const int32_t chunk = static_cast<int32_t>(blockIdx.x % static_cast<uint32_t>(a.chunks));
     const int64_t bh = blockIdx.x / static_cast<uint32_t>(a.chunks);
@@ -58,19 +49,19 @@ __global__ __launch_bounds__(4 * D) void linear_attention_decay_kernel(const LAD
     }
     const LADecay decay(a.log_decay[head]);
     if (tid <= C) powers[tid] = decay.power(static_cast<float>(tid));
-    const int32_t cu = tid % (D / 4), tu = tid / (D / 4);
-    LAQuad<T> raw[4][UNIT];
+    const int32_t col = tid % (D / 8) * 8, row = tid / (D / 8);
     const LATokens from[4] = {a.q, a.k, a.dout, a.v};
-    const bool wide[4] = {a.wide_q, a.wide_k, a.wide_dout, a.wide_v};
+    const int32_t vec[4] = {a.vec_q, a.vec_k, a.vec_dout, a.vec_v};
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
         const T* p = static_cast<const T*>(from[x].data) + batch * from[x].bs + head * from[x].hs;
 #pragma unroll
-        for (int u = 0; u < UNIT; ++u) {
-            const int32_t i = tu * UNIT + u;
-            raw[x][u] = la_load(p + static_cast<int64_t>(t0 + i) * from[x].ts, 4 * cu, x < 2 ? a.kdim : a.vdim, wide[x], i < nt);
+        for (int u = 0; u < P::units; ++u) {
+            const int32_t i = row + 32 * u;
+            LAOct<T> raw{};
+            if (i < nt) raw = la_load(p + (t0 + i) * from[x].ts + col, col, x < 2 ? a.kdim : a.vdim, vec[x]);
+            la_stage<T, D, false>(raw, tiles + x * TILE, col, i);
         }
-        la_stage<T, D>(raw[x], tiles + x * TILE, nullptr, cu, tu);
     }
     __syncthreads();
     float sum = 0.f;
@@ -84,11 +75,11 @@ __global__ __launch_bounds__(4 * D) void linear_attention_decay_kernel(const LAD
         for (int x = 0; x < STEPS_D; ++x) {
             uint4 m[R], n[R];
             const int32_t of_j = (16 * jt + n16) * P::row_d + 32 * x + 8 * g, of_i = (16 * it + n16) * P::row_d + 32 * x + 8 * g;
-            la_read(tiles + TILE, P::tokens_tile, of_j, m);
-            la_read(tiles, P::tokens_tile, of_i, n);
+            la_read(tiles + TILE, P::tile, of_j, m);
+            la_read(tiles, P::tile, of_i, n);
             w = la_mm<(R == 1 ? 0 : 2)>(m, n, w);
-            la_read(tiles + 3 * TILE, P::tokens_tile, of_j, m);
-            la_read(tiles + 2 * TILE, P::tokens_tile, of_i, n);
+            la_read(tiles + 3 * TILE, P::tile, of_j, m);
+            la_read(tiles + 2 * TILE, P::tile, of_i, n);
             e = la_mm<(R == 1 ? 0 : 2)>(m, n, e);
         }
         const int32_t d = 16 * it + n16 - (16 * jt + 4 * g);
@@ -96,12 +87,8 @@ __global__ __launch_bounds__(4 * D) void linear_attention_decay_kernel(const LAD
         for (int r = 0; r < 4; ++r)
             if (d - r > 0) sum = fmaf(w[r] * e[r], powers[d - r] * (static_cast<float>(d - r) * a.scale), sum);
     }
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < 4; ++x) la_stage<T, D>(raw[x], nullptr, tiles + x * TILE, cu, tu);
-    __syncthreads();
     // the chunk's sums over tokens in the states' layout: key rows 16 m + 4 g .. + 3, a value column
-    const int32_t column = 16 * wave + n16;
+    const int32_t column = 16 * wave + n16, at_column = la_column<false>(lane, P::row_d);
     la_f32x4 before[D / 16], behind[D / 16];
     const int64_t all = a.chunks - 1;
     const int32_t last = (end - 1) / C;
@@ -131,7 +118,7 @@ __global__ __launch_bounds__(4 * D) void linear_attention_decay_kernel(const LAD
 #pragma unroll
         for (int x = 0; x < STEPS_C; ++x) {
             uint4 va[R], vw[LA_STATE_LIMBS];
-            la_read(tiles + (2 + part) * TILE, P::turned_tile, column * P::row_c + 32 * x + 8 * g, va);
+            la_turned<T, D, false>(tiles + (2 + part) * TILE, at_column, x, wave, va);
             float v[8];
             la_join8<R>(va, v);
 #pragma unroll
@@ -143,7 +130,7 @@ __global__ __launch_bounds__(4 * D) void linear_attention_decay_kernel(const LAD
 #pragma unroll
             for (int m = 0; m < D / 16; ++m) {
                 uint4 ka[R];
-                la_read(tiles + part * TILE, P::turned_tile, (16 * m + n16) * P::row_c + 32 * x + 8 * g, ka);
+                la_turned<T, D, false>(tiles + part * TILE, at_column, x, m, ka);
                 acc[m] = la_mm<2>(ka, vw, acc[m]);
             }
         }
@@ -185,7 +172,7 @@ int launch_decay(const LADecayArgs& a, int64_t B, float* out, hipStream_t stream
     const uint32_t grid = static_cast<uint32_t>(B * a.heads * a.chunks);
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        linear_attention_decay_kernel<T, D><<<grid, 4 * D, LADecayShape<T, D>::lds, stream>>>(a);
+        linear_attention_decay_kernel<T, D><<<grid, 4 * D, LAShape<T, D>::head + 4 * LAShape<T, D>::R * LAShape<T, D>::tile * 2, stream>>>(a);
     };
     const int32_t padded = la_padded(a.kdim, a.vdim);
     if (padded == 32) go(std::integral_constant<int, 32>{});
@@ -229,6 +216,7 @@ int vh_linear_attention_backward(
     size_t workspace_bytes, void* stream) {
     using namespace vh;
     if (int rc = la_check_sizes(io_dtype, B, N, heads, key_dim, value_dim)) return rc;
+    if (int rc = la_check_strides({dout_token, q_token, k_token, v_token})) return rc;
     VH_REQUIRE(dout != nullptr && q != nullptr && k != nullptr && v != nullptr && log_decay != nullptr && dq != nullptr &&
                    dk != nullptr && dv != nullptr, VH_ERR_ARG, "dout, q, k, v, log_decay, dq, dk and dv must not be null");
     VH_REQUIRE(!overlapping(dstate, dnew_state, B * heads * key_dim * value_dim * 4), VH_ERR_ARG,
@@ -332,10 +320,10 @@ int vh_linear_attention_backward(
     d.vdim = dv_;
     d.chunks = cut.segments;
     const int64_t e = dtype_bytes(io_dtype);
-    d.wide_q = la_wide(tq, key_dim, e);
-    d.wide_k = la_wide(tk, key_dim, e);
-    d.wide_v = la_wide(tv, value_dim, e);
-    d.wide_dout = la_wide(tdo, value_dim, e);
+    d.vec_q = la_vec(tq, key_dim, e);
+    d.vec_k = la_vec(tk, key_dim, e);
+    d.vec_v = la_vec(tv, value_dim, e);
+    d.vec_dout = la_vec(tdo, value_dim, e);
     if (io_dtype == VH_DTYPE_F32) return launch_decay<float>(d, B, dlog_decay, s);
     return io_dtype == VH_DTYPE_BF16 ? launch_decay<bf16_t>(d, B, dlog_decay, s) : launch_decay<f16_t>(d, B, dlog_decay, s);
 }

@@ -22,9 +22,14 @@ from .token_lines import (address, check_io, check_like, check_param, dense_chan
 MAX_HEAD_DIM = 128
 
 
+def _lines(t):
+    """``t`` with dense heads and tokens less than 2^24 elements apart, as the kernels take it."""
+    return t.contiguous() if t.stride(1) >= 1 << 24 and t.shape[1] > 1 else dense_channels(t)
+
+
 def _heads_of(t):
     """Native arguments of ``[B, N, H, D]``: address and element strides of sequence, token, head."""
-    return t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)
+    return t.data_ptr(), t.stride(0), 0 if t.shape[1] == 1 else t.stride(1), t.stride(2)
 
 
 def _forward(q, k, v, log_decay, scale, state, lengths, return_state):
@@ -67,12 +72,12 @@ class _LinearAttentionFunction(Function):
         if dout is None and dnew_state is None:
             return (None,) * 8
         # saved-tensor hooks may return other strides than were saved
-        q, k, v = dense_channels(q), dense_channels(k), dense_channels(v)
+        q, k, v = _lines(q), _lines(k), _lines(v)
         log_decay, state, lengths = (None if t is None else t.contiguous() for t in (log_decay, state, lengths))
         batch, length, heads, key_dim = q.shape
         value_dim, device, dtype = v.shape[3], q.device, q.dtype
         sizes, need = (batch, length, heads, key_dim, value_dim), ctx.needs_input_grad
-        dout = (torch.zeros(v.shape, device=device, dtype=dtype) if dout is None else dense_channels(dout.to(dtype)))
+        dout = (torch.zeros(v.shape, device=device, dtype=dtype) if dout is None else _lines(dout.to(dtype)))
         if dnew_state is not None:
             dnew_state = dnew_state.float().contiguous()
         dq, dk = (torch.empty(q.shape, device=device, dtype=dtype) for _ in range(2))
@@ -127,7 +132,7 @@ def visionhope_linear_attention(q, k, v, log_decay, *, scale=None, state=None, l
         state = state.contiguous()
     lengths = line_lengths(name, lengths, batch, q.device)
     scale = key_dim ** -0.5 if scale is None else float(scale)
-    q, k, v = dense_channels(q), dense_channels(k), dense_channels(v)
+    q, k, v = _lines(q), _lines(k), _lines(v)
     if differentiated(q, k, v, log_decay, state):
         return _LinearAttentionFunction.apply(q, k, v, log_decay, state, scale, lengths, bool(return_state))
     return _no_grad_forward(q, k, v, log_decay, state, scale, lengths, return_state)
