@@ -654,16 +654,17 @@ int vh_linear_attention_forward(
 
 /* Gradients of vh_linear_attention_forward: dq, dk [B, N, heads, key_dim] and dv [B, N, heads,
  * value_dim] in io_dtype, dense; dstate (or NULL) like state, dlog_decay [heads] (or NULL; the
- * workspace query's `decay`) fp32; dnew_state (or NULL) is the gradient of new_state.  Sums run in
- * a fixed order. */
+ * workspace query's `decay`) fp32; dnew_state (or NULL) is the gradient of new_state.  `kept` is the
+ * forward's workspace as that call left it: the states between its segments (NULL where the
+ * forward needed none).  Sums run in a fixed order. */
 size_t vh_linear_attention_backward_workspace_bytes(int64_t B, int64_t N, int64_t heads, int64_t key_dim,
                                                     int64_t value_dim, int32_t io_dtype, int32_t decay);
 int vh_linear_attention_backward(
     const void* dout, int64_t dout_batch, int64_t dout_token, int64_t dout_head, const void* q, int64_t q_batch,
     int64_t q_token, int64_t q_head, const void* k, int64_t k_batch, int64_t k_token, int64_t k_head, const void* v,
     int64_t v_batch, int64_t v_token, int64_t v_head, int32_t io_dtype, const float* log_decay, float scale,
-    const float* state, const int32_t* lengths, const float* dnew_state, void* dq, void* dk, void* dv, float* dstate,
-    float* dlog_decay, int64_t B, int64_t N, int64_t heads, int64_t key_dim, int64_t value_dim, void* workspace,
+    const float* state, const int32_t* lengths, const float* kept, const float* dnew_state, void* dq, void* dk, void* dv,
+    float* dstate, float* dlog_decay, int64_t B, int64_t N, int64_t heads, int64_t key_dim, int64_t value_dim, void* workspace,
     size_t workspace_bytes, void* stream);
 
 /* One token of every sequence: q, k [B, heads, key_dim] and v [B, heads, value_dim], strides of a

@@ -283,6 +283,7 @@ struct LAPass {
     int64_t state_row, state_col;
     const int32_t* lengths;
     float* slots;            // [B, heads, segments - 1, D * D]: states between the segments
+    bool ready, turned;      // the slots are there already; they hold the states' transposes
     int32_t batches, tokens, heads, kdim, vdim, segments, chunks_per_segment, chunk, reversed;
     int32_t vec_q, vec_k, vec_v;   // elements of one load
     bool wide_out;

@@ -120,10 +120,18 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 4 : 3) void linear_attention_kern
         }
     } else if (OUT && (a.reversed ? segment < last : true)) {
         const int32_t slot = a.reversed ? segment : segment - 1;
-        const la_f32x4* at = reinterpret_cast<const la_f32x4*>(a.slots + (bh * (a.segments - 1) + slot) * D * D) +
-                             wave * (D / 16) * 64 + lane;
+        const float* at = a.slots + (bh * (a.segments - 1) + slot) * D * D;
+        if (a.turned) {   // row 16 m + 4 g + r of this state is the column of that lane there
 #pragma unroll
-        for (int m = 0; m < D / 16; ++m) s[m] = at[m * 64];
+            for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    s[m][r] = at[((m * (D / 16) + wave) * 64 + (n16 >> 2) * 16 + 4 * g + r) * 4 + (n16 & 3)];
+        } else {
+#pragma unroll
+            for (int m = 0; m < D / 16; ++m)
+                s[m] = reinterpret_cast<const la_f32x4*>(at)[(wave * (D / 16) + m) * 64 + lane];
+        }
     }
 
     const int32_t at_row = n16 * P::row_d + 8 * g, at_weights = n16 * P::row_c + 8 * g;
@@ -311,7 +319,7 @@ template <typename T, int D>
 int launch_pass(const LAPass& a, bool states, hipStream_t stream) {
     using P = LAShape<T, D>;
     const int64_t heads = static_cast<int64_t>(a.batches) * a.heads;
-    if (a.segments > 1) {
+    if (a.segments > 1 && !a.ready) {
         linear_attention_kernel<T, D, false><<<static_cast<uint32_t>(heads * (a.segments - 1)), P::threads, P::state_lds, stream>>>(a);
         if (int rc = check_launch("linear_attention states")) return rc;
         const int32_t quads = D * D / 4;

@@ -211,7 +211,7 @@ int vh_linear_attention_backward(
     const void* dout, int64_t dout_batch, int64_t dout_token, int64_t dout_head, const void* q, int64_t q_batch,
     int64_t q_token, int64_t q_head, const void* k, int64_t k_batch, int64_t k_token, int64_t k_head, const void* v,
     int64_t v_batch, int64_t v_token, int64_t v_head, int32_t io_dtype, const float* log_decay, float scale,
-    const float* state, const int32_t* lengths, const float* dnew_state, void* dq, void* dk, void* dv, float* dstate,
+    const float* state, const int32_t* lengths, const float* kept, const float* dnew_state, void* dq, void* dk, void* dv, float* dstate,
     float* dlog_decay, int64_t B, int64_t N, int64_t heads, int64_t key_dim, int64_t value_dim, void* workspace,
     size_t workspace_bytes, void* stream) {
     using namespace vh;
@@ -236,46 +236,50 @@ int vh_linear_attention_backward(
     base.log_decay = log_decay;
     base.scale_weight = scale;
     base.lengths = lengths;
-    base.slots = static_cast<float*>(workspace);
     base.batches = static_cast<int32_t>(B);
     base.tokens = static_cast<int32_t>(N);
     base.heads = static_cast<int32_t>(heads);
     base.segments = cut.segments;
     base.chunks_per_segment = cut.each;
     const int32_t dk_ = static_cast<int32_t>(key_dim), dv_ = static_cast<int32_t>(value_dim);
+    float* const adjoints = static_cast<float*>(workspace);
+    float* const states = decay ? adjoints + la_slots_bytes(B * heads, cut, padded) / sizeof(float) : const_cast<float*>(kept);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    {
-        LAPass a = base;
-        a.q = tdo;
-        a.k = tv;
-        a.v = tk;
-        a.kdim = dv_;
-        a.vdim = dk_;
-        a.out = dq;
-        a.scale_out = scale;
+    LAPass a = base;
+    if (decay) {   // the forward's states are those between its segments
+        a.q = a.k = tk;
+        a.v = tv;
+        a.kdim = dk_;
+        a.vdim = dv_;
         a.scale_in = 1.f;
         a.state = state;
-        a.state_row = 1;
-        a.state_col = value_dim;
-        if (int rc = la_run(a, io_dtype, s)) return rc;
+        a.state_row = value_dim;
+        a.state_col = 1;
+        a.slots = states;
+        if (int rc = la_states(a, io_dtype, s)) return rc;
     }
+    a = base;
+    a.q = tdo;
+    a.k = tv;
+    a.v = tk;
+    a.kdim = dv_;
+    a.vdim = dk_;
+    a.out = dq;
+    a.scale_out = scale;
+    a.scale_in = 1.f;
+    a.state = state;
+    a.state_row = 1;
+    a.state_col = value_dim;
+    a.slots = states;
+    a.ready = a.turned = true;
+    if (int rc = la_run(a, io_dtype, s)) return rc;
+
     base.reversed = 1;
     base.scale_out = 1.f;
     base.scale_in = scale;
     base.state = dnew_state;
-    {
-        LAPass a = base;
-        a.q = tv;
-        a.k = tdo;
-        a.v = tq;
-        a.kdim = dv_;
-        a.vdim = dk_;
-        a.out = dk;
-        a.state_row = 1;
-        a.state_col = value_dim;
-        if (int rc = la_run(a, io_dtype, s)) return rc;
-    }
-    LAPass a = base;
+    base.slots = adjoints;
+    a = base;
     a.q = tk;
     a.k = tq;
     a.v = tdo;
@@ -286,21 +290,19 @@ int vh_linear_attention_backward(
     a.state_col = 1;
     a.new_state = dstate;
     if (int rc = la_run(a, io_dtype, s)) return rc;
+    a = base;
+    a.q = tv;
+    a.k = tdo;
+    a.v = tq;
+    a.kdim = dv_;
+    a.vdim = dk_;
+    a.out = dk;
+    a.state_row = 1;
+    a.state_col = value_dim;
+    a.ready = a.turned = true;
+    if (int rc = la_run(a, io_dtype, s)) return rc;
     if (!decay) return VH_OK;
-    // the last pass left the gradients of the states; the states themselves go behind them
-    float* states = base.slots + la_slots_bytes(B * heads, cut, padded) / sizeof(float);
-    LAPass f = base;
-    f.reversed = 0;
-    f.q = f.k = tk;
-    f.v = tv;
-    f.kdim = dk_;
-    f.vdim = dv_;
-    f.scale_in = 1.f;
-    f.state = state;
-    f.state_row = value_dim;
-    f.state_col = 1;
-    f.slots = states;
-    if (int rc = la_states(f, io_dtype, s)) return rc;
+
     LADecayArgs d{};
     d.q = tq;
     d.k = tk;
@@ -309,7 +311,7 @@ int vh_linear_attention_backward(
     d.log_decay = log_decay;
     d.state = state;
     d.dnew_state = dnew_state;
-    d.adjoints = base.slots;
+    d.adjoints = adjoints;
     d.states = states;
     d.partial = states + la_slots_bytes(B * heads, cut, padded) / sizeof(float);
     d.lengths = lengths;

@@ -192,7 +192,7 @@ _SIGNATURES = {
     "vh_linear_attention_backward_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32, _i32]),
     "vh_linear_attention_backward": (ctypes.c_int, [
         _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _f32,
-        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
+        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
     "vh_linear_attention_step": (ctypes.c_int, [
         _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _f32, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
     "vh_group_norm_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32]),

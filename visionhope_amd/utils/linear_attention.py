@@ -45,7 +45,7 @@ def _forward(q, k, v, log_decay, scale, state, lengths, return_state):
     hip.check(lib.vh_linear_attention_forward(
         *_heads_of(q), *_heads_of(k), *_heads_of(v), code, address(log_decay), scale, address(state), address(lengths),
         address(out), address(new_state), *sizes, address(ws), nbytes, hip.stream_of(q)), "vh_linear_attention_forward")
-    return out, new_state
+    return out, new_state, ws   # the workspace: states that the backward starts from
 
 
 class _LinearAttentionFunction(Function):
@@ -53,9 +53,9 @@ class _LinearAttentionFunction(Function):
     @on_tensor_device
     def forward(ctx, q, k, v, log_decay, state, scale, lengths, return_state):
         decay32 = fp32_param(log_decay)
-        out, new_state = _forward(q, k, v, decay32, scale, state, lengths, return_state)
+        out, new_state, kept = _forward(q, k, v, decay32, scale, state, lengths, return_state)
         note_stream(ctx, hip.stream_of(q))
-        ctx.save_for_backward(q, k, v, decay32, state, lengths)
+        ctx.save_for_backward(q, k, v, decay32, state, lengths, kept)
         ctx.scale, ctx.decay_dtype = scale, log_decay.dtype
         ctx.set_materialize_grads(False)
         return (out, new_state) if return_state else out
@@ -67,13 +67,14 @@ class _LinearAttentionFunction(Function):
 
     @staticmethod
     @on_tensor_device
-    def _gradients(q, k, v, log_decay, state, lengths, ctx, dout, dnew_state):
+    def _gradients(q, k, v, log_decay, state, lengths, kept, ctx, dout, dnew_state):
         refuse_held_leaves("visionhope_linear_attention", ctx, torch.cuda.is_current_stream_capturing())
         if dout is None and dnew_state is None:
             return (None,) * 8
         # saved-tensor hooks may return other strides than were saved
         q, k, v = _lines(q), _lines(k), _lines(v)
-        log_decay, state, lengths = (None if t is None else t.contiguous() for t in (log_decay, state, lengths))
+        log_decay, state, lengths, kept = (None if t is None else t.contiguous()
+                                           for t in (log_decay, state, lengths, kept))
         batch, length, heads, key_dim = q.shape
         value_dim, device, dtype = v.shape[3], q.device, q.dtype
         sizes, need = (batch, length, heads, key_dim, value_dim), ctx.needs_input_grad
@@ -89,8 +90,8 @@ class _LinearAttentionFunction(Function):
         ws = hip.workspace(nbytes, device) if nbytes else None
         hip.check(lib.vh_linear_attention_backward(
             *_heads_of(dout), *_heads_of(q), *_heads_of(k), *_heads_of(v), code, address(log_decay), ctx.scale,
-            address(state), address(lengths), address(dnew_state), address(dq), address(dk), address(dv),
-            address(dstate), address(ddecay), *sizes, address(ws), nbytes, hip.stream_of(q)),
+            address(state), address(lengths), address(kept), address(dnew_state), address(dq), address(dk),
+            address(dv), address(dstate), address(ddecay), *sizes, address(ws), nbytes, hip.stream_of(q)),
             "vh_linear_attention_backward")
         return dq, dk, dv, None if ddecay is None else ddecay.to(ctx.decay_dtype), dstate, None, None, None
 
@@ -140,7 +141,7 @@ def visionhope_linear_attention(q, k, v, log_decay, *, scale=None, state=None, l
 
 @on_tensor_device
 def _no_grad_forward(q, k, v, log_decay, state, scale, lengths, return_state):
-    out, new_state = _forward(q, k, v, fp32_param(log_decay), scale, state, lengths, return_state)
+    out, new_state, _ = _forward(q, k, v, fp32_param(log_decay), scale, state, lengths, return_state)
     return (out, new_state) if return_state else out
 
 
