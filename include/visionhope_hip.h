@@ -679,7 +679,8 @@ int vh_linear_attention_step(
  * 1024 channels, then an activation (0: none, 1: SiLU, 2: exact GELU): mean and biased variance over
  * a group's channels and all pixels of an image; weight and bias [C] fp32.  stats [3, B, groups]
  * fp32 (or NULL) receives mean, the rest that rounding left of it, and rstd for the backward.
- * Workspaces from the queries, 16-byte aligned.  No counterpart in the reference's native code (its
+ * Workspaces from the queries, 16-byte aligned (NULL where a query says 0).  No counterpart in the
+ * reference's native code (its
  * models/layers.py offers nn.GroupNorm). */
 size_t vh_group_norm_workspace_bytes(int64_t B, int64_t pixels, int64_t channels, int64_t groups, int32_t io_dtype);
 int vh_group_norm_forward(const void* x, int32_t io_dtype, const float* weight, const float* bias, int32_t activation,

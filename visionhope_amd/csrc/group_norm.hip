@@ -7,21 +7,26 @@
 //   db = sum dz,  dw = sum dz xhat  (over images and pixels),
 //   dx = rstd (w dz - (s1 + xhat s2) / n),  s1 = sum w dz,  s2 = sum w dz xhat  over the group
 //
-// Both directions are two passes over the map: partial sums of slabs of pixels, then the outputs,
+// Where a workgroup's registers hold a bundle of an image's groups, one launch reads the map once
+// (both directions).  Larger maps take two passes: partial sums of slabs of pixels, then the outputs,
 // whose workgroups join their image's slabs first.  Bound by the bytes of the map.
 //
-// Statistics: a thread sums its values and their squares about its own first value, so that what
-// cancels is bounded by its own share of the variance; threads and slabs are joined by their means
-// and centred squares with the means in FP64, and the mean is kept as a sum of two floats (an offset
-// large beside the spread loses nothing).
+// Statistics of slabs: a thread sums its values and their squares about its own first value, so that
+// what cancels is bounded by its own share of the variance; threads and slabs are joined by their
+// means and centred squares with the means in FP64.  Values in registers are centred about their
+// rounded mean, whose rest is summed beside the squares.  Either way the mean is kept as a sum of two
+// floats: an offset large beside the spread loses nothing.
+#include <algorithm>
+
 #include "param_sum.h"
 
 namespace vh {
 namespace {
 
 constexpr int GN_NONE = 0, GN_SILU = 1, GN_GELU = 2;
-constexpr int64_t GN_MAX_SLABS = 64;      // one lane of a wave each
+constexpr int64_t GN_MAX_SLABS = 128;
 constexpr int64_t GN_MAX_GROUP = 1024;    // channels of a group: a workgroup's threads
+constexpr int GN_RESIDENT = 512;          // threads, at most, that hold a map in registers
 
 struct GNArgs {
     const void *x, *dy;
@@ -34,6 +39,7 @@ struct GNArgs {
     int32_t pixels, channels, groups, per;           // per: channels of a group
     int32_t bundle, bundles;                         // groups of a workgroup; workgroups for all groups
     int32_t slabs, slab;                             // slab: its pixels
+    int32_t lg, slabs_lg;                            // 2^lg lanes join a group's threads (or its slabs)
     int32_t activation;
     float eps;
 };
@@ -89,16 +95,20 @@ __device__ __forceinline__ float gn_tail(float a, float& bell) {
     p = fmaf(p, t, 0.11170406639575958f);
     return p * t * bell;
 }
-__device__ __forceinline__ float gn_activate(float z, int32_t activation) {
-    if (activation == GN_NONE) return z;
-    if (activation == GN_SILU) return z * sigmoid_fast(z);
+// Outputs of 16 bits take gelu_fast, whose 1e-5 is far below their rounding.
+template <typename T, int ACT>
+__device__ __forceinline__ float gn_activate(float z) {
+    if constexpr (ACT == GN_NONE) return z;
+    if constexpr (ACT == GN_SILU) return z * sigmoid_fast(z);
+    if constexpr (sizeof(T) == 2) return gelu_fast(z);
     float bell;
     const float a = fabsf(z), tail = gn_tail(a, bell);
     return fmaf(-a, tail, fmaxf(z, 0.f));
 }
-__device__ __forceinline__ float gn_slope(float z, int32_t activation) {
-    if (activation == GN_NONE) return 1.f;
-    if (activation == GN_SILU) {
+template <int ACT>
+__device__ __forceinline__ float gn_slope(float z) {
+    if constexpr (ACT == GN_NONE) return 1.f;
+    if constexpr (ACT == GN_SILU) {
         const float s = sigmoid_fast(z);
         return s * fmaf(z, 1.f - s, 1.f);
     }
@@ -106,12 +116,26 @@ __device__ __forceinline__ float gn_slope(float z, int32_t activation) {
     const float tail = gn_tail(fabsf(z), bell);
     return fmaf(z * 0.398942280401432678f, bell, z < 0.f ? tail : 1.f - tail);
 }
+// Runs a loop over values with the activation a compiled choice.
+template <typename F>
+__device__ __forceinline__ void gn_with(int32_t activation, F&& loop) {
+    if (activation == GN_NONE) loop(std::integral_constant<int, GN_NONE>{});
+    else if (activation == GN_SILU) loop(std::integral_constant<int, GN_SILU>{});
+    else loop(std::integral_constant<int, GN_GELU>{});
+}
 
-__device__ __forceinline__ double gn_wave_sum(double v) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
+__device__ __forceinline__ double gn_lane_sum(double v, int32_t lg) {
+    for (int32_t m = 1; m < (1 << lg); m <<= 1) v += __shfl_xor(v, m);
     return v;
 }
+
+// (x - mean) rstd: centred first, so that a constant map far from zero comes out as zeros, then scaled
+// and rid of the mean's rest at once.
+struct GNCentre {
+    float mean, rstd, rest;
+    __device__ __forceinline__ GNCentre(float mean_, float rest_, float rstd_) : mean(mean_), rstd(rstd_), rest(-rest_ * rstd_) {}
+    __device__ __forceinline__ float operator()(float v) const { return fmaf(v - mean, rstd, rest); }
+};
 
 // A thread's place: `vector` of the bundle's vectors in a pixel, pixels `row`, row + rows, ... of
 // a slab; threads behind the last full row are idle.
@@ -119,6 +143,7 @@ struct GNPlace {
     int32_t vectors, rows, vector, row, channel, group;   // channel: its first; group: within the bundle
     int32_t groups;                                       // of this bundle
     int32_t first_pixel, pixels;                          // of the slab
+    int32_t entry, entries;                               // of its group's threads, which stand side by side in LDS
     bool live;
 };
 template <int VEC>
@@ -135,6 +160,9 @@ __device__ __forceinline__ GNPlace gn_place(const GNArgs& a, int32_t bundle, int
     p.group = p.vector * VEC / a.per;
     p.first_pixel = slab * a.slab;
     p.pixels = a.pixels - p.first_pixel < a.slab ? a.pixels - p.first_pixel : a.slab;
+    const int32_t each = a.per / VEC, rows = p.pixels < p.rows ? p.pixels : p.rows;
+    p.entries = each * rows;
+    p.entry = p.group * p.entries + p.row * each + (p.vector - p.group * each);
     return p;
 }
 
@@ -142,14 +170,14 @@ __device__ __forceinline__ GNPlace gn_place(const GNArgs& a, int32_t bundle, int
 template <typename T, int VEC>
 __global__ __launch_bounds__(1024) void group_norm_stats_kernel(const GNArgs a) {
     __shared__ double means[1024];
-    __shared__ float squares[1024];
+    __shared__ float squares[1024], counts[1024];
     const int32_t slab = static_cast<int32_t>(blockIdx.x), bundle = static_cast<int32_t>(blockIdx.y);
     const int64_t image = blockIdx.z;
     const GNPlace p = gn_place<VEC>(a, bundle, slab);
-    float pivot = 0.f, sum = 0.f, square = 0.f;
     if (p.live && p.row < p.pixels) {
+        float sum = 0.f, square = 0.f;
         const T* at = static_cast<const T*>(a.x) + (image * a.pixels + p.first_pixel) * a.channels + p.channel;
-        pivot = to_f32(at[static_cast<int64_t>(p.row) * a.channels]);
+        const float pivot = to_f32(at[static_cast<int64_t>(p.row) * a.channels]);
 #pragma unroll 4
         for (int32_t i = p.row; i < p.pixels; i += p.rows) {
             float v[VEC];
@@ -162,27 +190,23 @@ __global__ __launch_bounds__(1024) void group_norm_stats_kernel(const GNArgs a) 
             }
         }
         const float n = static_cast<float>((p.pixels - p.row + p.rows - 1) / p.rows * VEC), off = sum / n;
-        means[threadIdx.x] = static_cast<double>(pivot) + static_cast<double>(off);
-        squares[threadIdx.x] = fmaxf(fmaf(-sum, off, square), 0.f);
+        means[p.entry] = static_cast<double>(pivot) + static_cast<double>(off);
+        squares[p.entry] = fmaxf(fmaf(-sum, off, square), 0.f);
+        counts[p.entry] = n;
     }
     __syncthreads();
-    const int32_t lane = threadIdx.x & 63, each = a.per / VEC, waves = static_cast<int32_t>(blockDim.x) >> 6;
-    const int32_t rows = p.pixels < p.rows ? p.pixels : p.rows;
-    const double n_all = static_cast<double>(p.pixels) * a.per;
-    for (int32_t g = static_cast<int32_t>(threadIdx.x) >> 6; g < p.groups; g += waves) {
+    const int32_t lanes = 1 << a.lg, sub = static_cast<int32_t>(threadIdx.x) & (lanes - 1);
+    const double inv = 1.0 / (static_cast<double>(p.pixels) * a.per);
+    for (int32_t g = static_cast<int32_t>(threadIdx.x) >> a.lg; g < p.groups; g += static_cast<int32_t>(blockDim.x) >> a.lg) {
         double total = 0.0, centred = 0.0;
-        for (int32_t e = lane; e < each * rows; e += 64) {
-            const int32_t row = e / each, t = row * p.vectors + g * each + (e - row * each);
-            total += means[t] * ((p.pixels - row + p.rows - 1) / p.rows * VEC);
+        for (int32_t e = g * p.entries + sub; e < (g + 1) * p.entries; e += lanes) total = fma(means[e], static_cast<double>(counts[e]), total);
+        const double mean = gn_lane_sum(total, a.lg) * inv;
+        for (int32_t e = g * p.entries + sub; e < (g + 1) * p.entries; e += lanes) {
+            const double d = means[e] - mean;
+            centred += fma(d * d, static_cast<double>(counts[e]), static_cast<double>(squares[e]));
         }
-        const double mean = gn_wave_sum(total) / n_all;
-        for (int32_t e = lane; e < each * rows; e += 64) {
-            const int32_t row = e / each, t = row * p.vectors + g * each + (e - row * each);
-            const double d = means[t] - mean;
-            centred += d * d * ((p.pixels - row + p.rows - 1) / p.rows * VEC) + static_cast<double>(squares[t]);
-        }
-        centred = gn_wave_sum(centred);
-        if (lane == 0) {
+        centred = gn_lane_sum(centred, a.lg);
+        if (sub == 0) {
             double* to = a.partial + ((image * a.slabs + slab) * a.groups + bundle * a.bundle + g) * 2;
             to[0] = mean;
             to[1] = centred;
@@ -190,23 +214,26 @@ __global__ __launch_bounds__(1024) void group_norm_stats_kernel(const GNArgs a) 
     }
 }
 
-// Mean (two floats) and rstd of the bundle's groups from the slabs, in LDS [3][bundle].
+// Mean (two floats) and rstd of the bundle's groups from the slabs, in LDS [3][1024].
 __device__ __forceinline__ void gn_join(const GNArgs& a, const GNPlace& p, int32_t bundle, int64_t image, float* out) {
-    const int32_t lane = threadIdx.x & 63, waves = static_cast<int32_t>(blockDim.x) >> 6;
-    for (int32_t g = static_cast<int32_t>(threadIdx.x) >> 6; g < p.groups; g += waves) {
-        double mean = 0.0, square = 0.0, n = 0.0;
-        if (lane < a.slabs) {
-            const double* from = a.partial + ((image * a.slabs + lane) * a.groups + bundle * a.bundle + g) * 2;
-            mean = from[0];
-            square = from[1];
-            const int32_t left = a.pixels - lane * a.slab;
-            n = static_cast<double>(left < a.slab ? left : a.slab) * a.per;
+    const int32_t lanes = 1 << a.slabs_lg, slab = static_cast<int32_t>(threadIdx.x) & (lanes - 1);
+    const double inv = 1.0 / (static_cast<double>(a.pixels) * a.per);
+    for (int32_t g = static_cast<int32_t>(threadIdx.x) >> a.slabs_lg; g < p.groups; g += static_cast<int32_t>(blockDim.x) >> a.slabs_lg) {
+        const double* from = a.partial + (image * a.slabs * a.groups + bundle * a.bundle + g) * 2;
+        const int64_t step = static_cast<int64_t>(a.groups) * 2;
+        auto count = [&](int32_t i) {
+            const int32_t left = a.pixels - i * a.slab;
+            return static_cast<double>(left < a.slab ? left : a.slab) * a.per;
+        };
+        double total = 0.0, var = 0.0;
+        for (int32_t i = slab; i < a.slabs; i += lanes) total = fma(from[i * step], count(i), total);
+        const double all = gn_lane_sum(total, a.slabs_lg) * inv;
+        for (int32_t i = slab; i < a.slabs; i += lanes) {
+            const double d = from[i * step] - all;
+            var += fma(d * d, count(i), from[i * step + 1]);
         }
-        const double n_all = static_cast<double>(a.pixels) * a.per;
-        const double all = gn_wave_sum(mean * n) / n_all;
-        const double d = mean - all;
-        const double var = gn_wave_sum(d * d * n + square) / n_all;
-        if (lane == 0) {
+        var = gn_lane_sum(var, a.slabs_lg) * inv;
+        if (slab == 0) {
             const float high = static_cast<float>(all);
             out[g] = high;
             out[1024 + g] = static_cast<float>(all - static_cast<double>(high));
@@ -230,23 +257,43 @@ __global__ __launch_bounds__(1024) void group_norm_apply_kernel(const GNArgs a) 
             for (int q = 0; q < 3; ++q) a.stats[q * all + at + g] = stats[q * 1024 + g];
     }
     if (!p.live) return;
-    const float mean = stats[p.group], rest = stats[1024 + p.group], rstd = stats[2048 + p.group];
+    const GNCentre centre(stats[p.group], stats[1024 + p.group], stats[2048 + p.group]);
     float w[VEC], b[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-        w[j] = rstd * a.weight[p.channel + j];
+        w[j] = a.weight[p.channel + j];
         b[j] = a.bias[p.channel + j];
     }
     const int64_t base = (image * a.pixels + p.first_pixel) * a.channels + p.channel;
     const T* x = static_cast<const T*>(a.x) + base;
     T* y = static_cast<T*>(a.y) + base;
+    gn_with(a.activation, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
 #pragma unroll 2
-    for (int32_t i = p.row; i < p.pixels; i += p.rows) {
-        float v[VEC];
-        gn_load<T, VEC>(x + static_cast<int64_t>(i) * a.channels, v);
+        for (int32_t i = p.row; i < p.pixels; i += p.rows) {
+            float v[VEC];
+            gn_load<T, VEC>(x + static_cast<int64_t>(i) * a.channels, v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = gn_activate(fmaf((v[j] - mean) - rest, w[j], b[j]), a.activation);
-        gn_store<T, VEC>(y + static_cast<int64_t>(i) * a.channels, v);
+            for (int j = 0; j < VEC; ++j) v[j] = gn_activate<T, ACT>(fmaf(centre(v[j]), w[j], b[j]));
+            gn_store<T, VEC>(y + static_cast<int64_t>(i) * a.channels, v);
+        }
+    });
+}
+
+// Sums over the rows of threads of each channel, in `parts` [rows][channels]: to `out`, and times the
+// weight to `weighted`.
+__device__ __forceinline__ void gn_channel_sums(const float* parts, const GNPlace& p, int32_t channels, float* out,
+                                                float* weighted, const float* weight) {
+    for (int32_t c = static_cast<int32_t>(threadIdx.x); c < channels; c += static_cast<int32_t>(blockDim.x)) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        int32_t r = 0;
+        for (; r + 3 < p.rows; r += 4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] += parts[(r + i) * channels + c];
+        for (; r < p.rows; ++r) sum[0] += parts[r * channels + c];
+        const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        out[c] = total;
+        weighted[c] = total * weight[c];
     }
 }
 
@@ -262,7 +309,7 @@ __global__ __launch_bounds__(1024) void group_norm_sums_kernel(const GNArgs a) {
     for (int j = 0; j < VEC; ++j) dw[j] = db[j] = 0.f;
     if (p.live) {
         const int64_t all = static_cast<int64_t>(gridDim.z) * a.groups, g = image * a.groups + bundle * a.bundle + p.group;
-        const float mean = a.stats[g], rest = a.stats[all + g], rstd = a.stats[2 * all + g];
+        const GNCentre centre(a.stats[g], a.stats[all + g], a.stats[2 * all + g]);
         float w[VEC], b[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
@@ -271,19 +318,22 @@ __global__ __launch_bounds__(1024) void group_norm_sums_kernel(const GNArgs a) {
         }
         const int64_t base = (image * a.pixels + p.first_pixel) * a.channels + p.channel;
         const T *x = static_cast<const T*>(a.x) + base, *dy = static_cast<const T*>(a.dy) + base;
+        gn_with(a.activation, [&](auto act) {
+            constexpr int ACT = decltype(act)::value;
 #pragma unroll 2
-        for (int32_t i = p.row; i < p.pixels; i += p.rows) {
-            float v[VEC], d[VEC];
-            gn_load<T, VEC>(x + static_cast<int64_t>(i) * a.channels, v);
-            gn_load<T, VEC>(dy + static_cast<int64_t>(i) * a.channels, d);
+            for (int32_t i = p.row; i < p.pixels; i += p.rows) {
+                float v[VEC], d[VEC];
+                gn_load<T, VEC>(x + static_cast<int64_t>(i) * a.channels, v);
+                gn_load<T, VEC>(dy + static_cast<int64_t>(i) * a.channels, d);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float xhat = ((v[j] - mean) - rest) * rstd;
-                const float dz = d[j] * gn_slope(fmaf(xhat, w[j], b[j]), a.activation);
-                dw[j] = fmaf(dz, xhat, dw[j]);
-                db[j] += dz;
+                for (int j = 0; j < VEC; ++j) {
+                    const float xhat = centre(v[j]);
+                    const float dz = d[j] * gn_slope<ACT>(fmaf(xhat, w[j], b[j]));
+                    dw[j] = fmaf(dz, xhat, dw[j]);
+                    db[j] += dz;
+                }
             }
-        }
+        });
     }
     const int32_t channels = p.groups * a.per, first = bundle * a.bundle * a.per, tid = static_cast<int32_t>(threadIdx.x);
     const int32_t threads = static_cast<int32_t>(blockDim.x);
@@ -295,24 +345,19 @@ __global__ __launch_bounds__(1024) void group_norm_sums_kernel(const GNArgs a) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) gn_lds[tid * VEC + j] = q == 0 ? dw[j] : db[j];
         __syncthreads();
-        for (int32_t c = tid; c < channels; c += threads) {
-            float sum = 0.f;
-            for (int32_t r = 0; r < p.rows; ++r) sum += gn_lds[r * channels + c];
-            to[q * a.channels + c] = sum;
-            of_channel[q * channels + c] = sum * a.weight[first + c];
-        }
+        gn_channel_sums(gn_lds, p, channels, to + q * a.channels, of_channel + q * channels, a.weight + first);
     }
     __syncthreads();
-    const int32_t lane = tid & 63, waves = threads >> 6;
-    for (int32_t g = tid >> 6; g < p.groups; g += waves) {
+    const int32_t lanes = 1 << a.lg, sub = tid & (lanes - 1);
+    for (int32_t g = tid >> a.lg; g < p.groups; g += threads >> a.lg) {
         float s1 = 0.f, s2 = 0.f;
-        for (int32_t c = lane; c < a.per; c += 64) {
+        for (int32_t c = sub; c < a.per; c += lanes) {
             s1 += of_channel[channels + g * a.per + c];
             s2 += of_channel[g * a.per + c];
         }
-        s1 = ln_lane_sum(s1, 6);
-        s2 = ln_lane_sum(s2, 6);
-        if (lane == 0) {
+        s1 = ln_lane_sum(s1, a.lg);
+        s2 = ln_lane_sum(s2, a.lg);
+        if (sub == 0) {
             float* out = a.group_sums + ((image * a.slabs + slab) * a.groups + bundle * a.bundle + g) * 2;
             out[0] = s1;
             out[1] = s2;
@@ -326,16 +371,16 @@ __global__ __launch_bounds__(1024) void group_norm_dx_kernel(const GNArgs a) {
     const int32_t slab = static_cast<int32_t>(blockIdx.x), bundle = static_cast<int32_t>(blockIdx.y);
     const int64_t image = blockIdx.z;
     const GNPlace p = gn_place<VEC>(a, bundle, slab);
-    const int32_t lane = threadIdx.x & 63, waves = static_cast<int32_t>(blockDim.x) >> 6;
-    for (int32_t g = static_cast<int32_t>(threadIdx.x) >> 6; g < p.groups; g += waves) {
+    const int32_t lane = static_cast<int32_t>(threadIdx.x) & ((1 << a.slabs_lg) - 1);
+    for (int32_t g = static_cast<int32_t>(threadIdx.x) >> a.slabs_lg; g < p.groups; g += static_cast<int32_t>(blockDim.x) >> a.slabs_lg) {
         float s1 = 0.f, s2 = 0.f;
-        if (lane < a.slabs) {
-            const float* from = a.group_sums + ((image * a.slabs + lane) * a.groups + bundle * a.bundle + g) * 2;
-            s1 = from[0];
-            s2 = from[1];
+        for (int32_t i = lane; i < a.slabs; i += 1 << a.slabs_lg) {
+            const float* from = a.group_sums + ((image * a.slabs + i) * a.groups + bundle * a.bundle + g) * 2;
+            s1 += from[0];
+            s2 += from[1];
         }
-        s1 = ln_lane_sum(s1, 6);
-        s2 = ln_lane_sum(s2, 6);
+        s1 = ln_lane_sum(s1, a.slabs_lg);
+        s2 = ln_lane_sum(s2, a.slabs_lg);
         if (lane == 0) {
             const float n = static_cast<float>(a.pixels) * static_cast<float>(a.per);
             sums[g] = s1 / n;
@@ -345,7 +390,7 @@ __global__ __launch_bounds__(1024) void group_norm_dx_kernel(const GNArgs a) {
     __syncthreads();
     if (!p.live) return;
     const int64_t all = static_cast<int64_t>(gridDim.z) * a.groups, g = image * a.groups + bundle * a.bundle + p.group;
-    const float mean = a.stats[g], rest = a.stats[all + g], rstd = a.stats[2 * all + g];
+    const GNCentre centre(a.stats[g], a.stats[all + g], a.stats[2 * all + g]);
     const float s1 = sums[p.group], s2 = sums[1024 + p.group];
     float w[VEC], b[VEC];
 #pragma unroll
@@ -356,37 +401,316 @@ __global__ __launch_bounds__(1024) void group_norm_dx_kernel(const GNArgs a) {
     const int64_t base = (image * a.pixels + p.first_pixel) * a.channels + p.channel;
     const T *x = static_cast<const T*>(a.x) + base, *dy = static_cast<const T*>(a.dy) + base;
     T* dx = static_cast<T*>(a.dx) + base;
+    gn_with(a.activation, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
 #pragma unroll 2
-    for (int32_t i = p.row; i < p.pixels; i += p.rows) {
-        float v[VEC], d[VEC];
-        gn_load<T, VEC>(x + static_cast<int64_t>(i) * a.channels, v);
-        gn_load<T, VEC>(dy + static_cast<int64_t>(i) * a.channels, d);
+        for (int32_t i = p.row; i < p.pixels; i += p.rows) {
+            float v[VEC], d[VEC];
+            gn_load<T, VEC>(x + static_cast<int64_t>(i) * a.channels, v);
+            gn_load<T, VEC>(dy + static_cast<int64_t>(i) * a.channels, d);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float xhat = centre(v[j]);
+                const float dz = d[j] * gn_slope<ACT>(fmaf(xhat, w[j], b[j]));
+                v[j] = centre.rstd * (fmaf(w[j], dz, -s1) - xhat * s2);
+            }
+            gn_store<T, VEC>(dx + static_cast<int64_t>(i) * a.channels, v);
+        }
+    });
+}
+
+// A vector as loaded, in whole words; unpacked when it is used.
+template <typename T, int VEC>
+struct GNRaw {
+    static constexpr int words = VEC * sizeof(T) < 4 ? 1 : VEC * sizeof(T) / 4;
+    uint32_t w[words];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (words == 4) {
+            const uint4 r = *reinterpret_cast<const uint4*>(p);
+            w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+        } else if constexpr (words == 2) {
+            const uint2 r = *reinterpret_cast<const uint2*>(p);
+            w[0] = r.x; w[1] = r.y;
+        } else if constexpr (VEC * sizeof(T) == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            w[0] = p->bits;
+        }
+    }
+    __device__ __forceinline__ void unpack(float (&v)[VEC]) const {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            const float xhat = ((v[j] - mean) - rest) * rstd;
-            const float dz = d[j] * gn_slope(fmaf(xhat, w[j], b[j]), a.activation);
-            v[j] = rstd * (fmaf(w[j], dz, -s1) - xhat * s2);
+            if constexpr (sizeof(T) == 4) v[j] = __uint_as_float(w[j]);
+            else v[j] = to_f32(T{static_cast<uint16_t>(j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu)});
         }
-        gn_store<T, VEC>(dx + static_cast<int64_t>(i) * a.channels, v);
     }
+    // From here on nothing that was computed from the vector is kept for its sake: the words are what
+    // the registers hold.
+    __device__ __forceinline__ void forget() {
+#pragma unroll
+        for (int i = 0; i < words; ++i) asm("" : "+v"(w[i]));
+    }
+};
+
+// The whole of a bundle's map in one workgroup's registers, K vectors a thread.
+template <typename T, int VEC, int K>
+__global__ __launch_bounds__(GN_RESIDENT) void group_norm_resident_kernel(const GNArgs a) {
+    __shared__ float first[GN_RESIDENT], second[GN_RESIDENT], stats[3 * GN_RESIDENT];
+    const int32_t bundle = static_cast<int32_t>(blockIdx.x), tid = static_cast<int32_t>(threadIdx.x);
+    const int64_t image = blockIdx.y;
+    const GNPlace p = gn_place<VEC>(a, bundle, 0);
+    const int64_t base = image * a.pixels * a.channels + p.channel;
+    const T* x = static_cast<const T*>(a.x) + base;
+    GNRaw<T, VEC> raw[K];
+    float sum = 0.f;
+    const bool mine = p.live && p.row < p.pixels;
+    if (mine) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int32_t i = p.row + k * p.rows;
+            if (i < p.pixels) raw[k].load(x + static_cast<int64_t>(i) * a.channels);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (p.row + k * p.rows < p.pixels) {
+                float v[VEC];
+                raw[k].unpack(v);
+                raw[k].forget();
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) sum += v[j];
+            }
+        first[p.entry] = sum;
+    }
+    __syncthreads();
+    const int32_t lanes = 1 << a.lg, sub = tid & (lanes - 1);
+    const float inv = 1.f / (static_cast<float>(p.pixels) * static_cast<float>(a.per));
+    for (int32_t g = tid >> a.lg; g < p.groups; g += static_cast<int32_t>(blockDim.x) >> a.lg) {
+        float total = 0.f;
+        for (int32_t e = g * p.entries + sub; e < (g + 1) * p.entries; e += lanes) total += first[e];
+        total = ln_lane_sum(total, a.lg);
+        if (sub == 0) stats[g] = total * inv;
+    }
+    __syncthreads();
+    if (mine) {
+        const float mean = stats[p.group];
+        float off = 0.f, square = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (p.row + k * p.rows < p.pixels) {
+                float v[VEC];
+                raw[k].unpack(v);
+                raw[k].forget();
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float d = v[j] - mean;
+                    off += d;
+                    square = fmaf(d, d, square);
+                }
+            }
+        first[p.entry] = off;
+        second[p.entry] = square;
+    }
+    __syncthreads();
+    const int64_t all = static_cast<int64_t>(gridDim.y) * a.groups, at = image * a.groups + bundle * a.bundle;
+    for (int32_t g = tid >> a.lg; g < p.groups; g += static_cast<int32_t>(blockDim.x) >> a.lg) {
+        float off = 0.f, square = 0.f;
+        for (int32_t e = g * p.entries + sub; e < (g + 1) * p.entries; e += lanes) {
+            off += first[e];
+            square += second[e];
+        }
+        off = ln_lane_sum(off, a.lg) * inv;
+        const float var = fmaxf(ln_lane_sum(square, a.lg) * inv - off * off, 0.f);
+        if (sub == 0) {
+            const float mean = stats[g], rstd = 1.f / sqrtf(var + a.eps);
+            stats[GN_RESIDENT + g] = off;
+            stats[2 * GN_RESIDENT + g] = rstd;
+            if (a.stats != nullptr) {
+                a.stats[at + g] = mean;
+                a.stats[all + at + g] = off;
+                a.stats[2 * all + at + g] = rstd;
+            }
+        }
+    }
+    __syncthreads();
+    if (!mine) return;
+    const GNCentre centre(stats[p.group], stats[GN_RESIDENT + p.group], stats[2 * GN_RESIDENT + p.group]);
+    float w[VEC], b[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        w[j] = a.weight[p.channel + j];
+        b[j] = a.bias[p.channel + j];
+    }
+    T* y = static_cast<T*>(a.y) + base;
+    gn_with(a.activation, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int32_t i = p.row + k * p.rows;
+            if (i < p.pixels) {
+                float v[VEC];
+                raw[k].unpack(v);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] = gn_activate<T, ACT>(fmaf(centre(v[j]), w[j], b[j]));
+                gn_store<T, VEC>(y + static_cast<int64_t>(i) * a.channels, v);
+            }
+        }
+    });
+}
+
+// The same for the backward: x and dy in registers, K vectors of each; a row of parameter sums an image.
+template <typename T, int VEC, int K>
+__global__ __launch_bounds__(GN_RESIDENT, sizeof(T) == 2 ? 4 : 2) void group_norm_resident_backward_kernel(const GNArgs a) {
+    extern __shared__ __align__(16) float gn_lds[];   // [threads * VEC], then [2][bundle channels]
+    __shared__ float sums[2 * GN_RESIDENT];
+    const int32_t bundle = static_cast<int32_t>(blockIdx.x), tid = static_cast<int32_t>(threadIdx.x);
+    const int32_t threads = static_cast<int32_t>(blockDim.x);
+    const int64_t image = blockIdx.y;
+    const GNPlace p = gn_place<VEC>(a, bundle, 0);
+    const int64_t base = image * a.pixels * a.channels + p.channel;
+    const bool mine = p.live && p.row < p.pixels;
+    GNRaw<T, VEC> rx[K], rd[K];
+    float dw[VEC], db[VEC], w[VEC], b[VEC];
+    const int64_t all = static_cast<int64_t>(gridDim.y) * a.groups, group = image * a.groups + bundle * a.bundle + p.group;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) dw[j] = db[j] = w[j] = b[j] = 0.f;
+    GNCentre centre(0.f, 0.f, 0.f);
+    if (mine) {
+        const T *x = static_cast<const T*>(a.x) + base, *dy = static_cast<const T*>(a.dy) + base;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int32_t i = p.row + k * p.rows;
+            if (i < p.pixels) {
+                rx[k].load(x + static_cast<int64_t>(i) * a.channels);
+                rd[k].load(dy + static_cast<int64_t>(i) * a.channels);
+            }
+        }
+        centre = GNCentre(a.stats[group], a.stats[all + group], a.stats[2 * all + group]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            w[j] = a.weight[p.channel + j];
+            b[j] = a.bias[p.channel + j];
+        }
+        gn_with(a.activation, [&](auto act) {
+            constexpr int ACT = decltype(act)::value;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (p.row + k * p.rows < p.pixels) {
+                    float v[VEC], d[VEC];
+                    rx[k].unpack(v);
+                    rd[k].unpack(d);
+                    rx[k].forget();
+                    rd[k].forget();
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        const float xhat = centre(v[j]);
+                        const float dz = d[j] * gn_slope<ACT>(fmaf(xhat, w[j], b[j]));
+                        dw[j] = fmaf(dz, xhat, dw[j]);
+                        db[j] += dz;
+                    }
+                }
+        });
+    }
+    const int32_t channels = p.groups * a.per, first = bundle * a.bundle * a.per;
+    float* of_channel = gn_lds + threads * VEC;
+    float* to = a.sums + image * 2 * a.channels + first;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) gn_lds[tid * VEC + j] = q == 0 ? dw[j] : db[j];
+        __syncthreads();
+        gn_channel_sums(gn_lds, p, channels, to + q * a.channels, of_channel + q * channels, a.weight + first);
+    }
+    __syncthreads();
+    const int32_t lanes = 1 << a.lg, sub = tid & (lanes - 1);
+    const float inv = 1.f / (static_cast<float>(p.pixels) * static_cast<float>(a.per));
+    for (int32_t g = tid >> a.lg; g < p.groups; g += threads >> a.lg) {
+        float s1 = 0.f, s2 = 0.f;
+        for (int32_t c = sub; c < a.per; c += lanes) {
+            s1 += of_channel[channels + g * a.per + c];
+            s2 += of_channel[g * a.per + c];
+        }
+        s1 = ln_lane_sum(s1, a.lg);
+        s2 = ln_lane_sum(s2, a.lg);
+        if (sub == 0) {
+            sums[g] = s1 * inv;
+            sums[GN_RESIDENT + g] = s2 * inv;
+        }
+    }
+    __syncthreads();
+    if (!mine) return;
+    const float s1 = sums[p.group], s2 = sums[GN_RESIDENT + p.group];
+    T* dx = static_cast<T*>(a.dx) + base;
+    gn_with(a.activation, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int32_t i = p.row + k * p.rows;
+            if (i < p.pixels) {
+                float v[VEC], d[VEC];
+                rx[k].unpack(v);
+                rd[k].unpack(d);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float xhat = centre(v[j]);
+                    const float dz = d[j] * gn_slope<ACT>(fmaf(xhat, w[j], b[j]));
+                    v[j] = centre.rstd * (fmaf(w[j], dz, -s1) - xhat * s2);
+                }
+                gn_store<T, VEC>(dx + static_cast<int64_t>(i) * a.channels, v);
+            }
+        }
+    });
 }
 
 // ---- host side -------------------------------------------------------------------------
 
 struct GNPlan {
-    int32_t vec, threads, bundle, bundles, slabs, slab;
+    int32_t vec, threads, bundle, bundles, slabs, slab, lg, slabs_lg;
+    int32_t vectors;   // a thread of the resident kernels, 0: slabs
 };
 
-// Vectors lie within a group, so that a thread's values share their statistics; a workgroup takes as
-// many groups as its threads have vectors for (long runs of a pixel's channels), and slabs are cut so
-// that about eight workgroups a CU share the map.
-GNPlan make_plan(int64_t B, int64_t pixels, int64_t channels, int64_t groups, int widest) {
+// 2^result lanes for a group's sum of n values: four values each, and all of the workgroup's groups at
+// once where that takes no more lanes than there are.
+int32_t lanes_lg(int64_t n, int64_t groups, int32_t threads) {
+    int32_t lg = 0;
+    while (lg < 6 && (static_cast<int64_t>(4) << lg) < n && (groups << (lg + 1)) <= threads) ++lg;
+    return lg;
+}
+
+// A bundle in one workgroup's registers, with runs of 128 bytes of a pixel (or all channels): four
+// vectors a thread of 256, or eight of 512.  32 x 14 x 14 x 448 bf16 take 7 us (slabs: 12), 128 of them
+// 13 (21), with the backward 42 (57).  Shorter runs waste the lines that they share (25 us with 32
+// bytes), larger workgroups leave a CU waiting for one (128 x 28 x 28 x 192 in 64-byte runs by 512
+// threads, forward and backward: 91 us, slabs 69).
+bool plan_resident(GNPlan& p, int64_t pixels, int64_t per, int64_t groups, int e) {
+    const int64_t each = per / p.vec, bundle = std::min(groups, (127 + per * e) / (per * e));
+    for (int threads : {256, GN_RESIDENT}) {
+        if (bundle * each > threads) continue;
+        const int64_t rows = threads / (bundle * each), vectors = (pixels + rows - 1) / rows;
+        if (vectors > (threads == 256 ? 4 : 8)) continue;
+        p.threads = threads;
+        p.bundle = static_cast<int32_t>(bundle);
+        p.bundles = static_cast<int32_t>((groups + bundle - 1) / bundle);
+        p.vectors = vectors <= 2 ? static_cast<int32_t>(vectors) : vectors <= 4 ? 4 : 8;
+        p.slabs = 1;
+        p.slab = static_cast<int32_t>(pixels);
+        p.lg = lanes_lg(each * std::min(rows, pixels), bundle, threads);
+        return true;
+    }
+    return false;
+}
+
+// Vectors lie within a group, so that a thread's values share their statistics.  Maps that no
+// workgroup holds are cut into slabs so that about eight workgroups a CU share them; a workgroup then
+// takes as many groups as its threads have vectors for (long runs of a pixel's channels).
+GNPlan make_plan(int64_t B, int64_t pixels, int64_t channels, int64_t groups, int widest, int e) {
     const int64_t per = channels / groups;
     int vec = widest;
     while (per % vec) vec /= 2;
     const int64_t each = per / vec;
-    GNPlan p;
+    GNPlan p{};
     p.vec = vec;
+    if (plan_resident(p, pixels, per, groups, e)) return p;
     p.threads = each <= 256 ? 256 : static_cast<int32_t>((each + 63) / 64 * 64);
     int64_t bundle = p.threads / each;
     bundle = bundle < groups ? bundle : groups;
@@ -401,6 +725,8 @@ GNPlan make_plan(int64_t B, int64_t pixels, int64_t channels, int64_t groups, in
     slabs = slabs < GN_MAX_SLABS ? slabs : GN_MAX_SLABS;
     p.slab = static_cast<int32_t>((pixels + slabs - 1) / slabs);
     p.slabs = static_cast<int32_t>((pixels + p.slab - 1) / p.slab);
+    p.lg = lanes_lg(each * std::min<int64_t>(rows, p.slab), bundle, p.threads);
+    p.slabs_lg = lanes_lg(static_cast<int64_t>(p.slabs) * 4, bundle, p.threads);
     return p;
 }
 
@@ -431,7 +757,7 @@ int widest_of(int64_t channels, int e, std::initializer_list<const void*> pointe
 }
 
 size_t forward_bytes(int64_t B, int64_t groups, const GNPlan& p) {
-    return static_cast<size_t>(B) * p.slabs * groups * 2 * sizeof(double);
+    return p.vectors > 0 ? 0 : static_cast<size_t>(B) * p.slabs * groups * 2 * sizeof(double);
 }
 size_t backward_bytes(int64_t B, int64_t channels, int64_t groups, const GNPlan& p) {
     const int64_t rows = B * p.slabs;
@@ -453,6 +779,8 @@ GNArgs make_args(const GNPlan& p, const void* x, const float* weight, const floa
     a.bundles = p.bundles;
     a.slabs = p.slabs;
     a.slab = p.slab;
+    a.lg = p.lg;
+    a.slabs_lg = p.slabs_lg;
     a.activation = activation;
     return a;
 }
@@ -472,6 +800,14 @@ int by_type(int32_t io, int vec, F&& go) {
     return io == VH_DTYPE_BF16 ? by_vec(bf16_t{}) : by_vec(f16_t{});
 }
 
+template <typename F>
+int by_vectors(int32_t vectors, F&& go) {
+    if (vectors == 1) return go(std::integral_constant<int, 1>{});
+    if (vectors == 2) return go(std::integral_constant<int, 2>{});
+    if (vectors == 4) return go(std::integral_constant<int, 4>{});
+    return go(std::integral_constant<int, 8>{});
+}
+
 }  // namespace
 }  // namespace vh
 
@@ -482,7 +818,7 @@ size_t vh_group_norm_workspace_bytes(int64_t B, int64_t pixels, int64_t channels
     if (check_sizes(io_dtype, B, pixels, channels, groups, 0) != VH_OK) return 0;
     size_t most = 0;   // of the vectors that a call may take
     for (int vec = 16 / dtype_bytes(io_dtype); vec >= 1; vec /= 2) {
-        const size_t one = forward_bytes(B, groups, make_plan(B, pixels, channels, groups, vec));
+        const size_t one = forward_bytes(B, groups, make_plan(B, pixels, channels, groups, vec, dtype_bytes(io_dtype)));
         most = one > most ? one : most;
     }
     return most;
@@ -495,9 +831,9 @@ int vh_group_norm_forward(const void* x, int32_t io_dtype, const float* weight, 
     if (int rc = check_sizes(io_dtype, B, pixels, channels, groups, activation)) return rc;
     VH_REQUIRE(x != nullptr && weight != nullptr && bias != nullptr && y != nullptr, VH_ERR_ARG,
                "x, weight, bias and y must not be null");
-    const GNPlan p = make_plan(B, pixels, channels, groups, widest_of(channels, dtype_bytes(io_dtype), {x, y}));
+    const GNPlan p = make_plan(B, pixels, channels, groups, widest_of(channels, dtype_bytes(io_dtype), {x, y}), dtype_bytes(io_dtype));
     const size_t need = forward_bytes(B, groups, p);
-    VH_REQUIRE(workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+    VH_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                VH_ERR_WORKSPACE, "group norm needs an aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
     GNArgs a = make_args(p, x, weight, bias, stats, pixels, channels, groups, activation);
     a.y = y;
@@ -506,6 +842,12 @@ int vh_group_norm_forward(const void* x, int32_t io_dtype, const float* weight, 
     hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid(static_cast<uint32_t>(p.slabs), static_cast<uint32_t>(p.bundles), static_cast<uint32_t>(B));
     return by_type(io_dtype, p.vec, [&](auto t, auto v) -> int {
+        if (p.vectors > 0)
+            return by_vectors(p.vectors, [&](auto k) -> int {
+                group_norm_resident_kernel<decltype(t), decltype(v)::value, decltype(k)::value>
+                    <<<dim3(static_cast<uint32_t>(p.bundles), static_cast<uint32_t>(B)), p.threads, 0, s>>>(a);
+                return check_launch("group_norm");
+            });
         group_norm_stats_kernel<decltype(t), decltype(v)::value><<<grid, p.threads, 0, s>>>(a);
         if (int rc = check_launch("group_norm statistics")) return rc;
         group_norm_apply_kernel<decltype(t), decltype(v)::value><<<grid, p.threads, 0, s>>>(a);
@@ -518,7 +860,7 @@ size_t vh_group_norm_backward_workspace_bytes(int64_t B, int64_t pixels, int64_t
     if (check_sizes(io_dtype, B, pixels, channels, groups, 0) != VH_OK) return 0;
     size_t most = 0;
     for (int vec = 16 / dtype_bytes(io_dtype); vec >= 1; vec /= 2) {
-        const size_t one = backward_bytes(B, channels, groups, make_plan(B, pixels, channels, groups, vec));
+        const size_t one = backward_bytes(B, channels, groups, make_plan(B, pixels, channels, groups, vec, dtype_bytes(io_dtype)));
         most = one > most ? one : most;
     }
     return most;
@@ -532,7 +874,8 @@ int vh_group_norm_backward(const void* dy, const void* x, int32_t io_dtype, cons
     if (int rc = check_sizes(io_dtype, B, pixels, channels, groups, activation)) return rc;
     VH_REQUIRE(dy != nullptr && x != nullptr && weight != nullptr && bias != nullptr && stats != nullptr && dx != nullptr,
                VH_ERR_ARG, "dy, x, weight, bias, stats and dx must not be null");
-    const GNPlan p = make_plan(B, pixels, channels, groups, widest_of(channels, dtype_bytes(io_dtype), {dy, x, dx}));
+    const GNPlan p = make_plan(B, pixels, channels, groups, widest_of(channels, dtype_bytes(io_dtype), {dy, x, dx}),
+                               dtype_bytes(io_dtype));
     const size_t need = backward_bytes(B, channels, groups, p);
     VH_REQUIRE(workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
                VH_ERR_WORKSPACE, "group norm's backward needs an aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
@@ -547,6 +890,12 @@ int vh_group_norm_backward(const void* dy, const void* x, int32_t io_dtype, cons
     const int rc = by_type(io_dtype, p.vec, [&](auto t, auto v) -> int {
         constexpr int VEC = decltype(v)::value;
         const size_t lds = (static_cast<size_t>(p.threads) * VEC + 2 * static_cast<size_t>(p.bundle) * a.per) * sizeof(float);
+        if (p.vectors > 0)
+            return by_vectors(p.vectors, [&](auto k) -> int {
+                group_norm_resident_backward_kernel<decltype(t), VEC, decltype(k)::value>
+                    <<<dim3(static_cast<uint32_t>(p.bundles), static_cast<uint32_t>(B)), p.threads, lds, s>>>(a);
+                return check_launch("group_norm gradient");
+            });
         group_norm_sums_kernel<decltype(t), VEC><<<grid, p.threads, lds, s>>>(a);
         if (int rc = check_launch("group_norm sums")) return rc;
         group_norm_dx_kernel<decltype(t), VEC><<<grid, p.threads, 0, s>>>(a);

@@ -29,7 +29,7 @@ __device__ __forceinline__ void la_triangle(int32_t tile, int32_t& it, int32_t& 
 
 // Walks a segment's chunks.  OUT: writes outputs; otherwise the segment's last state only.
 template <typename T, int D, bool OUT>
-__global__ __launch_bounds__(4 * D, D == 128 ? 4 : 3) void linear_attention_kernel(const LAPass a) {
+__global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kernel(const LAPass a) {
     using P = LAShape<T, D>;
     constexpr int R = P::R, F = P::F, C = P::C, ORDER = LAType<T>::order;
     constexpr int TILES = C / 16, STEPS_C = C / 32, STEPS_D = D / 32, UNITS = P::units;
@@ -358,7 +358,7 @@ int la_states(LAPass& a, int32_t io_dtype, hipStream_t stream) { return run(a, i
 LACut la_cut(int64_t heads, int64_t N, int32_t padded, int32_t io_dtype) {
     // Workgroups that the card holds at once, by registers and LDS: one round of them, since a
     // segment more than that waits for the end of another.
-    const int64_t held = padded == 32 ? 1024 : padded == 64 ? 768 : io_dtype == VH_DTYPE_F32 ? 256 : 512;
+    const int64_t held = padded == 32 ? 1024 : padded == 64 ? 768 : 256;
     const int64_t chunks = la_ceil(N, la_chunk(io_dtype));
     int64_t segments = held / heads;
     segments = segments < 1 ? 1 : segments < chunks ? segments : chunks;

@@ -31,10 +31,10 @@ def _forward(x, groups, weight, bias, eps, activation, keep):
     y = torch.empty_like(x, memory_format=torch.channels_last)
     stats = torch.empty((3, sizes[0], groups), device=x.device, dtype=torch.float32) if keep else None
     nbytes = lib.vh_group_norm_workspace_bytes(*sizes, code)
-    ws = hip.workspace(nbytes, x.device)
+    ws = hip.workspace(nbytes, x.device) if nbytes else None
     hip.check(lib.vh_group_norm_forward(
         x.data_ptr(), code, weight.data_ptr(), bias.data_ptr(), activation, y.data_ptr(), address(stats), *sizes, eps,
-        ws.data_ptr(), nbytes, hip.stream_of(x)), "vh_group_norm_forward")
+        address(ws), nbytes, hip.stream_of(x)), "vh_group_norm_forward")
     return y, stats
 
 
