@@ -1,0 +1,105 @@
+"""GroupNorm2d in the backbone: stem, downsamples, blocks and head without batch statistics."""
+
+import copy
+
+import pytest
+import torch
+from torch import nn
+from torch.nn import functional as F
+
+from tests.helpers import randn
+from tests.token_lines import compare, half_step, tolerance
+
+
+def _stem(conv_norm):
+    from visionhope_amd.models.layers import PatchEmbedding
+
+    torch.manual_seed(0)
+    return PatchEmbedding(3, 32, conv_norm=conv_norm)
+
+
+def _plain(module):
+    """The same module with torch's GroupNorm and activations, in float64 on the CPU."""
+    layers = []
+    for m in copy.deepcopy(module):
+        if type(m).__name__ != "GroupNorm2d":
+            layers.append(m)
+            continue
+        norm = nn.GroupNorm(m.groups, m.weight.numel(), m.eps)
+        norm.load_state_dict(m.state_dict())
+        layers += [norm] + ([nn.GELU()] if m.activation == "gelu" else [])
+    return nn.Sequential(*layers).double().cpu()
+
+
+def test_surface_and_cpu():
+    from visionhope_amd.models.layers import Downsample, GroupNorm2d, build_norm
+
+    assert GroupNorm2d(96).groups == 6 and GroupNorm2d(30).groups == 1 and GroupNorm2d(32, 4).groups == 4
+    assert isinstance(build_norm(32, "groupnorm2d"), GroupNorm2d) and isinstance(build_norm(32, "group"), nn.GroupNorm)
+    for bad in (lambda: GroupNorm2d(30, 4), lambda: GroupNorm2d(32, activation="relu"), lambda: _stem("none"),
+                lambda: Downsample(8, 16, "none"), lambda: build_norm(8, "none")):
+        with pytest.raises(ValueError):
+            bad()
+    x = randn(2, 32, 5, 7, seed=1)
+    for activation, f in ((None, lambda t: t), ("silu", F.silu), ("gelu", F.gelu)):
+        norm = GroupNorm2d(32, 2, activation=activation)
+        y = norm(x)
+        assert y.is_contiguous(memory_format=torch.channels_last)
+        assert torch.allclose(y, f(F.group_norm(x, 2, norm.weight, norm.bias, 1e-5)))
+    stem = _stem("group")
+    image = randn(2, 3, 32, 32, seed=2)
+    assert torch.allclose(stem(image), _plain(stem.proj)(image.double()).float(), atol=1e-5)
+    assert set(_stem("batch").state_dict()) == {f"proj.{i}.{n}" for i in (0, 3, 6, 9) for n in ("weight", "bias")} | {
+        f"proj.{i}.{n}" for i in (1, 4, 7, 10) for n in ("weight", "bias", "running_mean", "running_var", "num_batches_tracked")}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("channels_last", [True, False])
+def test_stem_and_gradients(device, channels_last):
+    stem = _stem("group")
+    plain = _plain(stem.proj)
+    image = randn(2, 3, 40, 24, seed=3)
+    dout = randn(2, 32, 10, 6, seed=4)
+    want = plain(image.double())
+    (want * dout.double()).sum().backward()
+    stem = stem.to(device)
+    image = image.to(device)
+    if channels_last:
+        stem, image = stem.to(memory_format=torch.channels_last), image.contiguous(memory_format=torch.channels_last)
+    out = stem(image)
+    # the library's FP32 convolutions of up to 288 terms, four norms between them
+    tol = 4 * tolerance(torch.float32, 4 * 288)
+    compare(out, want.detach(), tol, "stem")
+    (out * dout.to(device)).sum().backward()
+    grads = [p.grad for p in plain.parameters()]
+    for a, (name, p) in zip(grads, stem.named_parameters()):
+        if name in ("proj.0.bias", "proj.2.bias", "proj.4.bias", "proj.6.bias"):
+            continue   # what a bias adds to a group of channels the norm takes off: only the spread within one is left
+        compare(p.grad, a, 16 * tol, f"d{name}")
+
+
+@pytest.mark.gpu
+def test_backbone_trains_without_batch_statistics(device):
+    """An image's logits do not depend on the images beside it, and every parameter has a gradient."""
+    from visionhope_amd.models import HierarchicalVisionHOPE
+    from visionhope_amd.models.layers import GroupNorm2d
+
+    torch.manual_seed(1)
+    model = HierarchicalVisionHOPE(num_classes=10, embed_dims=(32, 32, 64, 64), mixer_dims=(16, 16, 32, 32), depths=(1, 1, 1, 1),
+                                   norm_layer="groupnorm2d", conv_norm="group", drop_path_rate=0.0, projection_dim=64,
+                                   layer_scale_init_value=0.1)
+    assert not any(isinstance(m, nn.BatchNorm2d) for m in model.modules())
+    assert sum(isinstance(m, GroupNorm2d) for m in model.modules()) == 4 + 3 + 8 + 2
+    model = model.to(device).to(memory_format=torch.channels_last)
+    images = randn(3, 3, 64, 64, seed=5).to(device).contiguous(memory_format=torch.channels_last)
+    logits = model(images)
+    logits.square().sum().backward()
+    for name, p in model.named_parameters():
+        assert p.grad is not None and torch.isfinite(p.grad).all(), name
+    with torch.no_grad():
+        alone = model(images[:1])
+        # the library picks other products for one image; the network is some 40 layers deep
+        compare(alone, logits[:1].double().cpu(), 40 * tolerance(torch.float32, 4 * 288), "alone")
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            half = model(images)
+        compare(half.float(), logits.double().cpu(), 40 * half_step(torch.bfloat16), "autocast")

@@ -230,6 +230,8 @@ int vh_linear_attention_backward(
     VH_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                VH_ERR_WORKSPACE, "linear attention's backward needs an aligned workspace of %zu bytes, got %zu", need,
                workspace_bytes);
+    VH_REQUIRE(decay || cut.segments == 1 || (kept != nullptr && reinterpret_cast<uintptr_t>(kept) % 16 == 0), VH_ERR_ARG,
+               "linear attention's backward needs the states that the forward left in its workspace");
     const LATokens tq{q, q_batch, q_token, q_head}, tk{k, k_batch, k_token, k_head}, tv{v, v_batch, v_token, v_head};
     const LATokens tdo{dout, dout_batch, dout_token, dout_head};
     LAPass base{};

@@ -11,7 +11,7 @@ from torch import nn
 
 from .block import VisionHOPEBlock
 from .common import ClassificationModel, initialize_weights
-from .layers import Downsample, LayerNorm2d, PatchEmbedding, build_norm
+from .layers import Downsample, GroupNorm2d, LayerNorm2d, PatchEmbedding, build_norm
 
 
 def _four(values):
@@ -28,7 +28,9 @@ class HierarchicalVisionHOPE(ClassificationModel):
     ``mixer_dims[i]`` channels in heads of ``head_dim``.  ``chunk_sizes=None`` scans in
     chunks of the row and column lengths of whatever map arrives (rectangular maps
     included); four explicit values fix each stage's chunk length.  Stochastic depth
-    rises linearly from 0 to ``drop_path_rate`` over all blocks.
+    rises linearly from 0 to ``drop_path_rate`` over all blocks.  ``conv_norm="group"``
+    normalises the convolutions of stem, downsamples and head by groups of an image's
+    channels instead of by the batch (small batches of large images).
     """
 
     def __init__(self, in_chans=3, num_classes=1000, embed_dims=(64, 128, 256, 512),
@@ -37,7 +39,7 @@ class HierarchicalVisionHOPE(ClassificationModel):
                  drop_path_rate=0.1, local_mode="gated_dwconv7", norm_layer="layernorm2d",
                  layer_scale_init_value=1e-6, use_grn=True, use_mlp_dwconv=True,
                  use_direction_scale=True, direction_merge="sum", use_block_cpe=True,
-                 use_output_lepe=True, projection_dim=1024, share_direction_skip=True):
+                 use_output_lepe=True, projection_dim=1024, share_direction_skip=True, conv_norm="batch"):
         super().__init__()
         if isinstance(mlp_ratios, (int, float)):
             mlp_ratios = (float(mlp_ratios),) * 4
@@ -55,7 +57,8 @@ class HierarchicalVisionHOPE(ClassificationModel):
 
         widths = self.embed_dims
         self.downsample_layers = nn.ModuleList(
-            [PatchEmbedding(in_chans, widths[0])] + [Downsample(widths[i - 1], widths[i]) for i in range(1, 4)])
+            [PatchEmbedding(in_chans, widths[0], conv_norm=conv_norm)]
+            + [Downsample(widths[i - 1], widths[i], conv_norm) for i in range(1, 4)])
         drop_rates = torch.linspace(0, drop_path_rate, sum(self.depths)).tolist()
         block_options = dict(head_dim=head_dim, local_mode=local_mode, norm_layer=norm_layer,
                              layer_scale_init_value=layer_scale_init_value, use_grn=use_grn,
@@ -73,8 +76,9 @@ class HierarchicalVisionHOPE(ClassificationModel):
             first += depth
         self.norm = build_norm(widths[-1], norm_layer)
         self.head_pre_logits = nn.Conv2d(widths[-1], projection_dim, 1)
-        self.head_norm = nn.BatchNorm2d(projection_dim)
-        self.head_act = nn.SiLU()
+        group = conv_norm == "group"
+        self.head_norm = GroupNorm2d(projection_dim, activation="silu") if group else nn.BatchNorm2d(projection_dim)
+        self.head_act = nn.Identity() if group else nn.SiLU()
         self.num_features = int(projection_dim)
         self.head = nn.Linear(self.num_features, num_classes)
         self.grad_checkpointing = False

@@ -6,6 +6,7 @@ from torch import nn
 from torch.nn import functional as F
 
 from ..utils.grn import GlobalResponseNorm
+from ..utils.group_norm import ACTIVATIONS, visionhope_group_norm
 from ..utils.layer_norm_cuda import can_fuse_layernorm2d, visionhope_layernorm2d
 
 
@@ -54,11 +55,42 @@ class LayerNorm2d(nn.Module):
         return y.contiguous(memory_format=torch.channels_last) if channels_last else y.contiguous()
 
 
+class GroupNorm2d(nn.Module):
+    """Group norm of an NCHW map, then ``activation`` (None, "silu" or "gelu") in the same pass.
+
+    ``groups`` defaults to one for every 16 channels, or to a single one where they do not divide.
+    GPU tensors run the native kernel and come out channels-last, in the input's dtype.
+    """
+
+    def __init__(self, dim, groups=None, eps=1e-5, activation=None):
+        super().__init__()
+        self.groups = (dim // 16 if dim % 16 == 0 else 1) if groups is None else int(groups)
+        if dim <= 0 or self.groups < 1 or dim % self.groups:
+            raise ValueError(f"{dim} channels do not divide into {self.groups} groups")
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}")
+        self.weight = nn.Parameter(torch.ones(dim))
+        self.bias = nn.Parameter(torch.zeros(dim))
+        self.eps, self.activation = eps, activation
+
+    def forward(self, x):
+        if x.is_cuda:
+            return visionhope_group_norm(x, self.groups, self.weight, self.bias, self.eps, activation=self.activation)
+        y = F.group_norm(x, self.groups, self.weight.to(x.dtype), self.bias.to(x.dtype), self.eps)
+        y = {None: lambda t: t, "silu": F.silu, "gelu": F.gelu}[self.activation](y)
+        return y.contiguous(memory_format=torch.channels_last)
+
+    def extra_repr(self):
+        return f"{self.weight.numel()}, groups={self.groups}, eps={self.eps}, activation={self.activation}"
+
+
 def build_norm(dim, norm_layer="group"):
     if norm_layer == "group":
         return nn.GroupNorm(1, dim)
     if norm_layer == "layernorm2d":
         return LayerNorm2d(dim)
+    if norm_layer == "groupnorm2d":
+        return GroupNorm2d(dim)
     raise ValueError(f"Unsupported norm_layer={norm_layer!r}.")
 
 
@@ -95,6 +127,15 @@ class FeedForwardNetwork(nn.Module):
         return self.drop(self.fc2(self.drop(self.grn(h))))
 
 
+def _conv_norm(conv_norm, width, activation=None):
+    """The modules between a convolution and the next: its norm and activation."""
+    if conv_norm == "group":
+        return [GroupNorm2d(width, activation=activation)]
+    if conv_norm != "batch":
+        raise ValueError(f"Unsupported conv_norm={conv_norm!r}.")
+    return [nn.BatchNorm2d(width)] + ([nn.GELU()] if activation == "gelu" else [])
+
+
 # Stem stages: (fraction of embed_dim as width divisor, stride, GELU after the BatchNorm).
 _STEM = ((2, 2, True), (2, 1, True), (1, 2, True), (1, 1, False))
 
@@ -103,9 +144,10 @@ class PatchEmbedding(nn.Module):
     """Stride-4 convolutional stem (reference ``models/layers.py:85-107``): four 3x3
     convolutions of widths embed_dim/2, embed_dim/2, embed_dim, embed_dim and strides 2,
     1, 2, 1, each followed by BatchNorm and, except the last, GELU (``proj``, a
-    Sequential whose indices are the checkpoint keys)."""
+    Sequential whose indices are the checkpoint keys).  ``conv_norm="group"`` puts a
+    ``GroupNorm2d`` with that activation in their place (no statistics of the batch)."""
 
-    def __init__(self, in_chans, embed_dim, patch_size=4):
+    def __init__(self, in_chans, embed_dim, patch_size=4, conv_norm="batch"):
         super().__init__()
         if patch_size != 4:
             raise ValueError("The VisionHOPE stem requires patch_size=4")
@@ -114,9 +156,8 @@ class PatchEmbedding(nn.Module):
         modules, channels = [], in_chans
         for divisor, stride, gelu in _STEM:
             width = embed_dim // divisor
-            modules += [nn.Conv2d(channels, width, 3, stride=stride, padding=1), nn.BatchNorm2d(width)]
-            if gelu:
-                modules.append(nn.GELU())
+            modules.append(nn.Conv2d(channels, width, 3, stride=stride, padding=1))
+            modules += _conv_norm(conv_norm, width, "gelu" if gelu else None)
             channels = width
         self.proj = nn.Sequential(*modules)
         self.norm = nn.Identity()
@@ -169,12 +210,12 @@ class PatchEmbedding(nn.Module):
 
 class Downsample(nn.Module):
     """Stage transition (reference ``models/layers.py:110-119``): a 3x3, stride-2 convolution
-    without bias, then BatchNorm."""
+    without bias, then BatchNorm (or a ``GroupNorm2d``, ``conv_norm="group"``)."""
 
-    def __init__(self, in_dim, out_dim):
+    def __init__(self, in_dim, out_dim, conv_norm="batch"):
         super().__init__()
         self.proj = nn.Conv2d(in_dim, out_dim, 3, stride=2, padding=1, bias=False)
-        self.norm = nn.BatchNorm2d(out_dim)
+        self.norm = _conv_norm(conv_norm, out_dim)[0]
 
     def forward(self, x):
         if (getattr(self, "_vh_fold_bn", False) and not self.training and x.is_cuda
