@@ -27,7 +27,7 @@ template <> struct LAType<bf16_t> { static constexpr int raw = 1, tokens = 64, f
 template <> struct LAType<f16_t> { static constexpr int raw = 2, tokens = 32, formed = 2, order = 1; };
 template <> struct LAType<float> { static constexpr int raw = 3, tokens = 32, formed = 3, order = 2; };
 
-// Limbs of what enters a state, an FP32 result: 24 bits.
+// Limbs of what enters a state that is an FP32 result: 24 bits.
 constexpr int LA_STATE_LIMBS = 3;
 
 struct LATokens {   // an activation [B, N, heads, dim]: element strides of sequence, token and head
@@ -116,12 +116,12 @@ template <typename T> struct LAOct { uint4 u; };
 template <> struct LAOct<float> { float4 a, b; };
 
 // Values col .. col + 7 of a row of `dim`, zeros behind it.  `vec`: elements that one load may take
-// (8, 4 or 1), by dim, strides and addresses.
-template <typename T>
+// (8, 4 or 1), by dim, strides and addresses; WIDE: 8.
+template <typename T, bool WIDE>
 __device__ __forceinline__ LAOct<T> la_load(const T* row, int32_t col, int32_t dim, int32_t vec) {
     LAOct<T> r{};
     if (col >= dim) return r;
-    if (vec == 8) {
+    if (WIDE || vec == 8) {
         if constexpr (sizeof(T) == 4) {
             r.a = *reinterpret_cast<const float4*>(row);
             r.b = *reinterpret_cast<const float4*>(row + 4);
@@ -216,44 +216,37 @@ struct LAShape {
     static constexpr int lds = head + (3 * R * tile + F * weights) * 2;
 };
 
-// Where value d of a row stands that a product with the state contracts over: d = 32 x + 16 h + 4 y + r
-// at 32 x + 8 y + 4 h + r, the order in which two tiles of accumulators have it.
-__device__ __forceinline__ int32_t la_place(int32_t d) {
-    return (d & ~31) + ((d & 15) >> 2) * 8 + ((d >> 4) & 1) * 4 + (d & 3);
+// Key index of row 4 g + r of tile m of a state: two tiles together hold, for a lane, eight neighbours
+// in a row, which are at once a lane's share of an operand that is contracted over the key index.
+__device__ __forceinline__ int32_t la_state_row(int32_t m, int32_t g, int32_t r) {
+    return 32 * (m >> 1) + 8 * g + 4 * (m & 1) + r;
 }
 
-// Eight values col .. col + 7 of token i into a tile; PLACED: in the order above.
-template <typename T, int D, bool PLACED>
+// Eight values col .. col + 7 of token i into a tile.
+template <typename T, int D>
 __device__ __forceinline__ void la_stage(const LAOct<T>& raw, uint16_t* tile, int32_t col, int32_t i) {
     using P = LAShape<T, D>;
     uint4 limbs[P::R];
     la_limbs<T>(raw, limbs);
 #pragma unroll
-    for (int l = 0; l < P::R; ++l) {
-        uint16_t* row = tile + l * P::tile + i * P::row_d;
-        if constexpr (PLACED) {
-            *reinterpret_cast<uint2*>(row + la_place(col)) = make_uint2(limbs[l].x, limbs[l].y);
-            *reinterpret_cast<uint2*>(row + la_place(col + 4)) = make_uint2(limbs[l].z, limbs[l].w);
-        } else {
-            *reinterpret_cast<uint4*>(row + col) = limbs[l];
-        }
-    }
+    for (int l = 0; l < P::R; ++l) *reinterpret_cast<uint4*>(tile + l * P::tile + i * P::row_d + col) = limbs[l];
 }
 
 typedef short la_i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) la_i16x4 la_lds_i16x4;
 
-// A column of a tile over eight tokens, of every limb: lane l gets column 16 m + l % 16 at tokens
-// 32 x + 8 (l / 16) .. + 7.  The transposing read takes four tokens' rows from the four quarters of
-// a 16-lane group and gives each lane one column of them.  `at`: la_column<PLACED>.
-template <bool PLACED>
+// A column of a tile over eight tokens, of every limb: lane l gets column 16 m + l % 16 (ROWS: the key
+// index of that row of a state's tile m) at tokens 32 x + 8 (l / 16) .. + 7.  The transposing read takes
+// four columns of four tokens from the quarters of a 16-lane group and gives each lane one column of
+// them.  `at`: la_column<ROWS>.
+template <bool ROWS>
 __device__ __forceinline__ int32_t la_column(int32_t lane, int32_t row_d) {
-    return (8 * (lane >> 4) + ((lane & 15) >> 2)) * row_d + (lane & 3) * (PLACED ? 8 : 4);
+    return (8 * (lane >> 4) + ((lane & 15) >> 2)) * row_d + (lane & 3) * (ROWS ? 8 : 4);
 }
-template <typename T, int D, bool PLACED>
+template <typename T, int D, bool ROWS>
 __device__ __forceinline__ void la_turned(const uint16_t* tile, int32_t at, int32_t x, int32_t m, uint4 (&out)[LAShape<T, D>::R]) {
     using P = LAShape<T, D>;
-    const int32_t of_tile = PLACED ? 32 * (m >> 1) + 4 * (m & 1) : 16 * m;
+    const int32_t of_tile = ROWS ? 32 * (m >> 1) + 4 * (m & 1) : 16 * m;
 #pragma unroll
     for (int l = 0; l < P::R; ++l) {
         const uint16_t* from = tile + l * P::tile + at + 32 * x * P::row_d + of_tile;
@@ -261,6 +254,27 @@ __device__ __forceinline__ void la_turned(const uint16_t* tile, int32_t at, int3
         const la_i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_i16x4*)(from + 4 * P::row_d));
         const uint2 ua = __builtin_bit_cast(uint2, a), ub = __builtin_bit_cast(uint2, b);
         out[l] = make_uint4(ua.x, ua.y, ub.x, ub.y);
+    }
+}
+
+// s += tiles of k^T v over a chunk: v's columns (weighted, FP32) as limbs, three where an FP32 result comes
+// of it and two where only values rounded to 16 bits do.
+template <typename T, int D>
+__device__ __forceinline__ void la_enter(const uint16_t* ks, int32_t at, int32_t x, const float (&v)[8], bool fine,
+                                         la_f32x4 (&s)[D / 16]) {
+    constexpr int R = LAType<T>::raw;
+    uint4 vw[LA_STATE_LIMBS];
+    la_split8<LA_STATE_LIMBS>(v, vw);
+    const uint4 coarse[2] = {vw[0], vw[1]}, rest[1] = {vw[2]};
+#pragma unroll
+    for (int m = 0; m < D / 16; ++m) {
+        uint4 ka[R];
+        la_turned<T, D, true>(ks, at, x, m, ka);
+        if (sizeof(T) == 4 || fine) {
+            const uint4 first[1] = {ka[0]};
+            s[m] = la_mm<0>(first, rest, s[m]);
+        }
+        s[m] = la_mm<2>(ka, coarse, s[m]);
     }
 }
 
@@ -287,6 +301,7 @@ struct LAPass {
     int32_t batches, tokens, heads, kdim, vdim, segments, chunks_per_segment, chunk, reversed;
     int32_t vec_q, vec_k, vec_v;   // elements of one load
     bool wide_out;
+    bool fine;               // an FP32 result comes of the states
 };
 
 // Tokens of a sequence.

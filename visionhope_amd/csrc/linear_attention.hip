@@ -27,17 +27,18 @@ __device__ __forceinline__ void la_triangle(int32_t tile, int32_t& it, int32_t& 
     jt = tile - it * (it + 1) / 2;
 }
 
-// Walks a segment's chunks.  OUT: writes outputs; otherwise the segment's last state only.
-template <typename T, int D, bool OUT>
+// Walks a segment's chunks.  OUT: writes outputs; otherwise the segment's last state only.  WIDE: all
+// loads take eight values, without the choice at each of them (5 % of a pass).
+template <typename T, int D, bool OUT, bool WIDE>
 __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kernel(const LAPass a) {
     using P = LAShape<T, D>;
     constexpr int R = P::R, F = P::F, C = P::C, ORDER = LAType<T>::order;
     constexpr int TILES = C / 16, STEPS_C = C / 32, STEPS_D = D / 32, UNITS = P::units;
     extern __shared__ __align__(16) unsigned char la_lds[];
     float* entering = reinterpret_cast<float*>(la_lds);                     // [C]: weights of what enters the state
-    uint16_t* ks = reinterpret_cast<uint16_t*>(la_lds + P::head);           // [R][C][D], placed
+    uint16_t* ks = reinterpret_cast<uint16_t*>(la_lds + P::head);           // [R][C][D]
     uint16_t* vs = ks + R * P::tile;                                        // [R][C][D]
-    uint16_t* qs = vs + R * P::tile;                                        // [R][C][D], placed
+    uint16_t* qs = vs + R * P::tile;                                        // [R][C][D]
     uint16_t* ws = qs + R * P::tile;                                        // [F][C][C]: weights of pairs
 
     const int32_t tid = static_cast<int32_t>(threadIdx.x), lane = tid & 63;
@@ -79,9 +80,9 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
             if (OUT) rq[u] = LAOct<T>{};
             rk[u] = rv[u] = LAOct<T>{};
             if (i < nt) {
-                if constexpr (OUT) rq[u] = la_load(q + (t * qt + col), col, a.kdim, a.vec_q);
-                rk[u] = la_load(k + (t * kt + col), col, a.kdim, a.vec_k);
-                rv[u] = la_load(v + (t * vt + col), col, a.vdim, a.vec_v);
+                if constexpr (OUT) rq[u] = la_load<T, WIDE>(q + (t * qt + col), col, a.kdim, a.vec_q);
+                rk[u] = la_load<T, WIDE>(k + (t * kt + col), col, a.kdim, a.vec_k);
+                rv[u] = la_load<T, WIDE>(v + (t * vt + col), col, a.vdim, a.vec_v);
             }
         }
     };
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
         for (int32_t i = tid; i < F * P::weights / 2; i += P::threads) reinterpret_cast<uint32_t*>(ws)[i] = 0;
     }
 
-    // the state: key rows 16 m + 4 g .. + 3, value column 16 wave + n16
+    // the state: key rows la_state_row(m, g, 0 .. 3), value column 16 wave + n16
     la_f32x4 s[D / 16];
 #pragma unroll
     for (int m = 0; m < D / 16; ++m) s[m] = la_f32x4{0.f, 0.f, 0.f, 0.f};
@@ -116,17 +117,20 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
             for (int m = 0; m < D / 16; ++m)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (16 * m + 4 * g + r < a.kdim) s[m][r] = at[(16 * m + 4 * g + r) * a.state_row];
+                    if (la_state_row(m, g, r) < a.kdim) s[m][r] = at[la_state_row(m, g, r) * a.state_row];
         }
     } else if (OUT && (a.reversed ? segment < last : true)) {
         const int32_t slot = a.reversed ? segment : segment - 1;
         const float* at = a.slots + (bh * (a.segments - 1) + slot) * D * D;
-        if (a.turned) {   // row 16 m + 4 g + r of this state is the column of that lane there
+        if (a.turned) {   // this state's column is a row there: of tile m2, group g2, its last two bits
+            const int32_t m2 = 2 * (column >> 5) + ((column >> 2) & 1), g2 = (column >> 3) & 3;
 #pragma unroll
             for (int m = 0; m < D / 16; ++m)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    s[m][r] = at[((m * (D / 16) + wave) * 64 + (n16 >> 2) * 16 + 4 * g + r) * 4 + (n16 & 3)];
+                for (int r = 0; r < 4; ++r) {
+                    const int32_t c = la_state_row(m, g, r);
+                    s[m][r] = at[(((c >> 4) * (D / 16) + m2) * 64 + 16 * g2 + (c & 15)) * 4 + (column & 3)];
+                }
         } else {
 #pragma unroll
             for (int m = 0; m < D / 16; ++m)
@@ -147,9 +151,9 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
         }
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-            if constexpr (OUT) la_stage<T, D, true>(rq[u], qs, col, row + 32 * u);
-            la_stage<T, D, true>(rk[u], ks, col, row + 32 * u);
-            la_stage<T, D, false>(rv[u], vs, col, row + 32 * u);
+            if constexpr (OUT) la_stage<T, D>(rq[u], qs, col, row + 32 * u);
+            la_stage<T, D>(rk[u], ks, col, row + 32 * u);
+            la_stage<T, D>(rv[u], vs, col, row + 32 * u);
         }
         if (step + 1 < chunks) fetch(a.reversed ? chunk - 1 : chunk + 1);
         __syncthreads();
@@ -224,14 +228,7 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
             const float4 e1 = *reinterpret_cast<const float4*>(entering + 32 * x + 8 * g + 4);
             v[0] *= e0.x; v[1] *= e0.y; v[2] *= e0.z; v[3] *= e0.w;
             v[4] *= e1.x; v[5] *= e1.y; v[6] *= e1.z; v[7] *= e1.w;
-            uint4 vw[LA_STATE_LIMBS];
-            la_split8<LA_STATE_LIMBS>(v, vw);
-#pragma unroll
-            for (int m = 0; m < D / 16; ++m) {
-                uint4 ka[R];
-                la_turned<T, D, true>(ks, k_column, x, m, ka);
-                s[m] = la_mm<2>(ka, vw, s[m]);
-            }
+            la_enter<T, D>(ks, k_column, x, v, a.fine, s);
         }
         if constexpr (OUT) {
             __syncthreads();   // all weights are there
@@ -275,7 +272,7 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
             for (int m = 0; m < D / 16; ++m)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (16 * m + 4 * g + r < a.kdim) at[(16 * m + 4 * g + r) * a.state_row] = s[m][r];
+                    if (la_state_row(m, g, r) < a.kdim) at[la_state_row(m, g, r) * a.state_row] = s[m][r];
         }
     }
 }
@@ -315,28 +312,33 @@ __global__ __launch_bounds__(256) void linear_attention_join_kernel(const LAPass
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool WIDE>
 int launch_pass(const LAPass& a, bool states, hipStream_t stream) {
     using P = LAShape<T, D>;
     const int64_t heads = static_cast<int64_t>(a.batches) * a.heads;
     if (a.segments > 1 && !a.ready) {
-        linear_attention_kernel<T, D, false><<<static_cast<uint32_t>(heads * (a.segments - 1)), P::threads, P::state_lds, stream>>>(a);
+        linear_attention_kernel<T, D, false, WIDE><<<static_cast<uint32_t>(heads * (a.segments - 1)), P::threads, P::state_lds, stream>>>(a);
         if (int rc = check_launch("linear_attention states")) return rc;
         const int32_t quads = D * D / 4;
         linear_attention_join_kernel<<<static_cast<uint32_t>(la_ceil(heads * quads, 256)), 256, 0, stream>>>(a, quads);
         if (int rc = check_launch("linear_attention join")) return rc;
     }
     if (states) return VH_OK;
-    linear_attention_kernel<T, D, true><<<static_cast<uint32_t>(heads * a.segments), P::threads, P::lds, stream>>>(a);
+    linear_attention_kernel<T, D, true, WIDE><<<static_cast<uint32_t>(heads * a.segments), P::threads, P::lds, stream>>>(a);
     return check_launch("linear_attention");
 }
 
 template <typename T>
 int launch_typed(const LAPass& a, bool states, hipStream_t stream) {
     const int32_t d = la_padded(a.kdim, a.vdim);
-    if (d == 32) return launch_pass<T, 32>(a, states, stream);
-    if (d == 64) return launch_pass<T, 64>(a, states, stream);
-    return launch_pass<T, 128>(a, states, stream);
+    auto go = [&](auto wide) -> int {
+        constexpr bool WIDE = decltype(wide)::value;
+        if (d == 32) return launch_pass<T, 32, WIDE>(a, states, stream);
+        if (d == 64) return launch_pass<T, 64, WIDE>(a, states, stream);
+        return launch_pass<T, 128, WIDE>(a, states, stream);
+    };
+    if (a.vec_q == 8 && a.vec_k == 8 && a.vec_v == 8) return go(std::true_type{});
+    return go(std::false_type{});
 }
 
 int run(LAPass& a, int32_t io_dtype, bool states, hipStream_t stream) {
@@ -518,6 +520,7 @@ int vh_linear_attention_forward(
     a.scale_in = 1.f;
     a.state = state;
     a.new_state = new_state;
+    a.fine = new_state != nullptr;
     a.state_row = value_dim;
     a.state_col = 1;
     a.lengths = lengths;

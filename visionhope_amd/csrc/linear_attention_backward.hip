@@ -59,8 +59,8 @@ __global__ __launch_bounds__(4 * D, 2) void linear_attention_decay_kernel(const 
         for (int u = 0; u < P::units; ++u) {
             const int32_t i = row + 32 * u;
             LAOct<T> raw{};
-            if (i < nt) raw = la_load(p + (t0 + i) * from[x].ts + col, col, x < 2 ? a.kdim : a.vdim, vec[x]);
-            la_stage<T, D, false>(raw, tiles + x * TILE, col, i);
+            if (i < nt) raw = la_load<T, false>(p + (t0 + i) * from[x].ts + col, col, x < 2 ? a.kdim : a.vdim, vec[x]);
+            la_stage<T, D>(raw, tiles + x * TILE, col, i);
         }
     }
     __syncthreads();
@@ -87,8 +87,8 @@ __global__ __launch_bounds__(4 * D, 2) void linear_attention_decay_kernel(const 
         for (int r = 0; r < 4; ++r)
             if (d - r > 0) sum = fmaf(w[r] * e[r], powers[d - r] * (static_cast<float>(d - r) * a.scale), sum);
     }
-    // the chunk's sums over tokens in the states' layout: key rows 16 m + 4 g .. + 3, a value column
-    const int32_t column = 16 * wave + n16, at_column = la_column<false>(lane, P::row_d);
+    // the chunk's sums over tokens in the states' layout
+    const int32_t column = 16 * wave + n16, k_column = la_column<true>(lane, P::row_d), v_column = la_column<false>(lane, P::row_d);
     la_f32x4 before[D / 16], behind[D / 16];
     const int64_t all = a.chunks - 1;
     const int32_t last = (end - 1) / C;
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(4 * D, 2) void linear_attention_decay_kernel(const 
         if (chunk < last) behind[m] = reinterpret_cast<const la_f32x4*>(a.adjoints + (bh * all + chunk) * D * D)[at];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int32_t row = 16 * m + 4 * g + r;
+            const int32_t row = la_state_row(m, g, r);
             const int64_t given = bh * a.kdim * a.vdim + row * a.vdim + column;
             if (row >= a.kdim || column >= a.vdim) continue;
             if (chunk == 0 && a.state != nullptr) before[m][r] = a.state[given];
@@ -117,8 +117,8 @@ __global__ __launch_bounds__(4 * D, 2) void linear_attention_decay_kernel(const 
         }
 #pragma unroll
         for (int x = 0; x < STEPS_C; ++x) {
-            uint4 va[R], vw[LA_STATE_LIMBS];
-            la_turned<T, D, false>(tiles + (2 + part) * TILE, at_column, x, wave, va);
+            uint4 va[R];
+            la_turned<T, D, false>(tiles + (2 + part) * TILE, v_column, x, wave, va);
             float v[8];
             la_join8<R>(va, v);
 #pragma unroll
@@ -126,13 +126,7 @@ __global__ __launch_bounds__(4 * D, 2) void linear_attention_decay_kernel(const 
                 const int32_t t = 32 * x + 8 * g + i, m = part == 0 ? t + 1 : nt - 1 - t;
                 v[i] *= m > 0 ? powers[m] * (static_cast<float>(m) * (part == 0 ? a.scale : 1.f)) : 0.f;
             }
-            la_split8<LA_STATE_LIMBS>(v, vw);
-#pragma unroll
-            for (int m = 0; m < D / 16; ++m) {
-                uint4 ka[R];
-                la_turned<T, D, false>(tiles + part * TILE, at_column, x, m, ka);
-                acc[m] = la_mm<2>(ka, vw, acc[m]);
-            }
+            la_enter<T, D>(tiles + part * TILE, k_column, x, v, true, acc);
         }
 #pragma unroll
         for (int m = 0; m < D / 16; ++m)
@@ -254,6 +248,7 @@ int vh_linear_attention_backward(
         a.kdim = dk_;
         a.vdim = dv_;
         a.scale_in = 1.f;
+        a.fine = true;
         a.state = state;
         a.state_row = value_dim;
         a.state_col = 1;
@@ -291,6 +286,7 @@ int vh_linear_attention_backward(
     a.state_row = value_dim;
     a.state_col = 1;
     a.new_state = dstate;
+    a.fine = dstate != nullptr || decay;
     if (int rc = la_run(a, io_dtype, s)) return rc;
     a = base;
     a.q = tv;
