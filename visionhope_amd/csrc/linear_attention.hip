@@ -16,6 +16,8 @@
 // The gradients are the same form with other operands (linear_attention_backward.hip): `reversed`
 // walks the tokens from the last one, where the state is the gradient of S behind a chunk and
 // enters with one power of g less.
+#include <algorithm>
+
 #include "linear_attention.h"
 
 namespace vh {
@@ -358,14 +360,30 @@ int la_run(LAPass& a, int32_t io_dtype, hipStream_t stream) { return run(a, io_d
 int la_states(LAPass& a, int32_t io_dtype, hipStream_t stream) { return run(a, io_dtype, true, stream); }
 
 LACut la_cut(int64_t heads, int64_t N, int32_t padded, int32_t io_dtype) {
-    // Workgroups that the card holds at once, by registers and LDS: one round of them, since a
-    // segment more than that waits for the end of another.
-    const int64_t held = padded == 32 ? 1024 : padded == 64 ? 768 : 256;
+    // The time of a cut, in chunks of a workgroup that has its CU to itself: a second and a third one there
+    // cost a third each; segments cost a pass for their states, 45 % of the outputs', a launch, and the
+    // states' way to memory and back twice, beside chunks that take 0.57 of that time for their own bytes.
+    // (bf16 heads of 64: 3.2, 4.2 and 5.4 us a chunk.  96 heads of 49 chunks take 61 us in 7 segments and
+    // 67 in 5; 304 of 13 take 53 us whole, 59 in 2 segments and 67 in 5.)  `held`: workgroups that the
+    // card holds at once, by registers and LDS; more of them wait for the end of others.
+    const int64_t held = padded == 32 ? 1024 : padded == 64 ? 768 : 256, cus = 256;
     const int64_t chunks = la_ceil(N, la_chunk(io_dtype));
-    int64_t segments = held / heads;
-    segments = segments < 1 ? 1 : segments < chunks ? segments : chunks;
-    const int64_t each = la_ceil(chunks, segments);
-    return {static_cast<int32_t>(la_ceil(chunks, each)), static_cast<int32_t>(each)};
+    const double state = 4.0 * padded / (la_chunk(io_dtype) * dtype_bytes(io_dtype)) * 0.57 / cus;
+    LACut best{1, static_cast<int32_t>(chunks)};
+    double least = 0.0;
+    // candidates: one to three segments, and as many as k workgroups on every CU are
+    for (int64_t k = -2; k <= 2 * held / cus; ++k) {
+        const int64_t wanted = std::min(chunks, std::max<int64_t>(1, k <= 0 ? k + 3 : k * cus / heads));
+        const int64_t each = la_ceil(chunks, wanted), segments = la_ceil(chunks, each), groups = heads * segments;
+        const int64_t rounds = la_ceil(groups, held), together = rounds > 1 ? held / cus : la_ceil(groups, cus);
+        double cost = static_cast<double>(rounds * each) * (1.0 + (together - 1) / 3.0);
+        if (segments > 1) cost = cost * 1.45 + 1.0 + state * static_cast<double>(heads * (segments - 1));
+        if (k == -2 || cost < least) {
+            least = cost;
+            best = {static_cast<int32_t>(segments), static_cast<int32_t>(each)};
+        }
+    }
+    return best;
 }
 
 size_t la_slots_bytes(int64_t heads, const LACut& cut, int32_t padded) {
