@@ -203,14 +203,27 @@ __device__ __forceinline__ void la_store(T* row, int32_t col, int32_t dim, bool 
         if (col + i < dim) row[i] = from_f32<T>(v[i]);
 }
 
-// Tiles of a chunk in LDS, for heads padded to D: rows of tokens, eight values longer than they
-// need, so that the 16-byte reads of 16 rows spread over all banks.
+// LDS tiles have rows of W values (32, 64 or 128) whose blocks of eight are permuted by the row: block b of
+// row r stands at b ^ la_fold(r).  Sixteen rows' blocks of one index then lie in sixteen different places
+// of the 256 bytes that the banks are wide, and so do the blocks that a transposing read takes from
+// four rows (rows eight values longer, without it: half of the LDS cycles were conflicts).
+template <int W>
+__device__ __forceinline__ int32_t la_fold(int32_t row) {
+    const int32_t low = (row >> 2) & 3;
+    return W == 128 ? (row & 3) << 2 | low : W == 64 ? ((row >> 1) & 1) << 2 | low : low;
+}
+// Where block b of a row starts.  Another block x of the same row is at this place ^ 8 (b ^ x).
+template <int W>
+__device__ __forceinline__ int32_t la_block(int32_t row, int32_t b) {
+    return row * W + 8 * (b ^ la_fold<W>(row));
+}
+
+// Tiles of a chunk, for heads padded to D.
 template <typename T, int D>
 struct LAShape {
     static constexpr int R = LAType<T>::raw, F = LAType<T>::formed, C = LAType<T>::tokens;
     static constexpr int waves = D / 16, threads = 64 * waves, units = C / 32;   // units: of eight values a thread
-    static constexpr int row_d = D + 8, row_c = C + 8;
-    static constexpr int tile = C * row_d, weights = C * row_c;   // one limb
+    static constexpr int tile = C * D, weights = C * C;   // one limb
     static constexpr int head = 512;                              // bytes of small tables
     static constexpr int state_lds = head + 2 * R * tile * 2;
     static constexpr int lds = head + (3 * R * tile + F * weights) * 2;
@@ -229,7 +242,7 @@ __device__ __forceinline__ void la_stage(const LAOct<T>& raw, uint16_t* tile, in
     uint4 limbs[P::R];
     la_limbs<T>(raw, limbs);
 #pragma unroll
-    for (int l = 0; l < P::R; ++l) *reinterpret_cast<uint4*>(tile + l * P::tile + i * P::row_d + col) = limbs[l];
+    for (int l = 0; l < P::R; ++l) *reinterpret_cast<uint4*>(tile + l * P::tile + la_block<D>(i, col / 8)) = limbs[l];
 }
 
 typedef short la_i16x4 __attribute__((ext_vector_type(4)));
@@ -238,20 +251,21 @@ typedef __attribute__((address_space(3))) la_i16x4 la_lds_i16x4;
 // A column of a tile over eight tokens, of every limb: lane l gets column 16 m + l % 16 (ROWS: the key
 // index of that row of a state's tile m) at tokens 32 x + 8 (l / 16) .. + 7.  The transposing read takes
 // four columns of four tokens from the quarters of a 16-lane group and gives each lane one column of
-// them.  `at`: la_column<ROWS>.
-template <bool ROWS>
-__device__ __forceinline__ int32_t la_column(int32_t lane, int32_t row_d) {
-    return (8 * (lane >> 4) + ((lane & 15) >> 2)) * row_d + (lane & 3) * (ROWS ? 8 : 4);
+// them.  `at`: la_column<D, ROWS>.
+template <int D, bool ROWS>
+__device__ __forceinline__ int32_t la_column(int32_t lane) {
+    const int32_t row = 8 * (lane >> 4) + ((lane & 15) >> 2), c = lane & 3;
+    return ROWS ? la_block<D>(row, c) : la_block<D>(row, c >> 1) + 4 * (c & 1);
 }
 template <typename T, int D, bool ROWS>
 __device__ __forceinline__ void la_turned(const uint16_t* tile, int32_t at, int32_t x, int32_t m, uint4 (&out)[LAShape<T, D>::R]) {
     using P = LAShape<T, D>;
-    const int32_t of_tile = ROWS ? 32 * (m >> 1) + 4 * (m & 1) : 16 * m;
+    const int32_t first = ROWS ? (at ^ (32 * (m >> 1))) + 4 * (m & 1) : at ^ (16 * m);
 #pragma unroll
     for (int l = 0; l < P::R; ++l) {
-        const uint16_t* from = tile + l * P::tile + at + 32 * x * P::row_d + of_tile;
-        const la_i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_i16x4*)from);
-        const la_i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_i16x4*)(from + 4 * P::row_d));
+        const uint16_t* from = tile + l * P::tile + 32 * x * D;
+        const la_i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_i16x4*)(from + first));
+        const la_i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((la_lds_i16x4*)(from + (first ^ 8) + 4 * D));   // four rows on
         const uint2 ua = __builtin_bit_cast(uint2, a), ub = __builtin_bit_cast(uint2, b);
         out[l] = make_uint4(ua.x, ua.y, ub.x, ub.y);
     }

@@ -140,8 +140,8 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
         }
     }
 
-    const int32_t at_row = n16 * P::row_d + 8 * g, at_weights = n16 * P::row_c + 8 * g;
-    const int32_t k_column = la_column<true>(lane, P::row_d), v_column = la_column<false>(lane, P::row_d);
+    const int32_t at_row = la_block<D>(n16, g), at_weights = la_block<C>(n16, g), to_weights = la_block<C>(n16, g >> 1) + 4 * (g & 1);
+    const int32_t k_column = la_column<D, true>(lane), v_column = la_column<D, false>(lane);
     int32_t entered = 0;   // the chunk length that `entering` stands for
     for (int32_t step = 0; step < chunks; ++step) {
         const int32_t chunk = a.reversed ? chunks - 1 - step : step;
@@ -173,8 +173,8 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
 #pragma unroll
                 for (int x = 0; x < STEPS_D; ++x) {
                     uint4 ka[R], qa[R];
-                    la_read(ks, P::tile, 16 * jt * P::row_d + at_row + 32 * x, ka);
-                    la_read(qs, P::tile, 16 * it * P::row_d + at_row + 32 * x, qa);
+                    la_read(ks, P::tile, 16 * jt * D + (at_row ^ (32 * x)), ka);
+                    la_read(qs, P::tile, 16 * it * D + (at_row ^ (32 * x)), qa);
                     w = la_mm<(R == 1 ? 0 : 2)>(ka, qa, w);
                 }
                 if (it == jt) {
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
                 la_split<F>(w[2], w[3], hi);
 #pragma unroll
                 for (int l = 0; l < F; ++l)
-                    *reinterpret_cast<uint2*>(ws + l * P::weights + (16 * it + n16) * P::row_c + 16 * jt + 4 * g) = make_uint2(lo[l], hi[l]);
+                    *reinterpret_cast<uint2*>(ws + l * P::weights + 16 * it * C + (to_weights ^ (16 * jt))) = make_uint2(lo[l], hi[l]);
             }
             // what comes from the state: value rows, token columns
 #pragma unroll
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
 #pragma unroll
                 for (int it = 0; it < TILES; ++it) {
                     uint4 qa[R];
-                    la_read(qs, P::tile, 16 * it * P::row_d + at_row + 32 * x, qa);
+                    la_read(qs, P::tile, 16 * it * D + (at_row ^ (32 * x)), qa);
                     o[it] = la_mm<ORDER>(sa, qa, o[it]);
                 }
             }
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
                 for (int x = 0; x < STEPS_C; ++x)
                     if (32 * x < 16 * (it + 1)) {
                         uint4 wa[F];
-                        la_read(ws, P::weights, 16 * it * P::row_c + at_weights + 32 * x, wa);
+                        la_read(ws, P::weights, 16 * it * C + (at_weights ^ (32 * x)), wa);
                         o[it] = la_mm<ORDER>(va[x], wa, o[it]);
                     }
             T* out = static_cast<T*>(a.out) + ((batch * static_cast<int64_t>(a.tokens) + t0) * a.heads + head) * a.vdim;

@@ -74,7 +74,7 @@ __global__ __launch_bounds__(4 * D, 2) void linear_attention_decay_kernel(const 
 #pragma unroll
         for (int x = 0; x < STEPS_D; ++x) {
             uint4 m[R], n[R];
-            const int32_t of_j = (16 * jt + n16) * P::row_d + 32 * x + 8 * g, of_i = (16 * it + n16) * P::row_d + 32 * x + 8 * g;
+            const int32_t at = la_block<D>(n16, g) ^ (32 * x), of_j = 16 * jt * D + at, of_i = 16 * it * D + at;
             la_read(tiles + TILE, P::tile, of_j, m);
             la_read(tiles, P::tile, of_i, n);
             w = la_mm<(R == 1 ? 0 : 2)>(m, n, w);
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(4 * D, 2) void linear_attention_decay_kernel(const 
             if (d - r > 0) sum = fmaf(w[r] * e[r], powers[d - r] * (static_cast<float>(d - r) * a.scale), sum);
     }
     // the chunk's sums over tokens in the states' layout
-    const int32_t column = 16 * wave + n16, k_column = la_column<true>(lane, P::row_d), v_column = la_column<false>(lane, P::row_d);
+    const int32_t column = 16 * wave + n16, k_column = la_column<D, true>(lane), v_column = la_column<D, false>(lane);
     la_f32x4 before[D / 16], behind[D / 16];
     const int64_t all = a.chunks - 1;
     const int32_t last = (end - 1) / C;
