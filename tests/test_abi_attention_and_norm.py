@@ -66,7 +66,7 @@ REFUSED = [
     ("vh_group_norm_forward", NORM, dict(G=3), hip.VH_ERR_SHAPE, "groups"),
     ("vh_group_norm_forward", NORM, dict(G=0), hip.VH_ERR_SHAPE, "groups"),
     ("vh_group_norm_forward", NORM, dict(C=2050, G=2), hip.VH_ERR_SHAPE, "1024"),
-    ("vh_group_norm_forward", NORM, dict(B=1 << 16), hip.VH_ERR_SHAPE, "range"),
+    ("vh_group_norm_forward", NORM, dict(B=1 << 21), hip.VH_ERR_SHAPE, "range"),
     ("vh_group_norm_forward", NORM, dict(act=3), hip.VH_ERR_ARG, "activation"),
     ("vh_group_norm_forward", NORM, dict(y=None), hip.VH_ERR_ARG, "null"),
     ("vh_group_norm_forward", NORM, dict(pixels=100000, wsn=16), hip.VH_ERR_WORKSPACE, "workspace"),

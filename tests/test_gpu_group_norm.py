@@ -137,6 +137,11 @@ def test_layouts_and_odd_addresses(device, dtype):
         assert torch.equal(a, b)
 
 
+def test_many_images(device):
+    """More images than a grid's second and third dimension count."""
+    _check(device, (70000, 16, 1, 2), 2, torch.bfloat16, "silu", "many images")
+
+
 def test_parameters_of_other_types_and_unwanted_gradients(device):
     from visionhope_amd.utils.group_norm import visionhope_group_norm
 
