@@ -10,8 +10,8 @@
 // Where a workgroup's registers hold a bundle of an image's groups, one launch reads the map once
 // (both directions).  Larger maps take two passes: partial sums of slabs of pixels, then the outputs,
 // whose workgroups join their image's slabs first.  128 x 56 x 56 x 96 bf16 with GELU: 15 + 29 us forward
-// (231 MB at 5.3 TB/s), 40 + 41 + 9 us backward, bound by the vector unit (33 instructions a value and
-// pass: the activation's slope is formed twice).  32 x 14 x 14 x 448: 6.5 and 9 + 3 us.
+// (231 MB at 5.3 TB/s), 39 + 40 + 9 us backward, bound by the vector unit (33 instructions a value and
+// pass: the activation's slope is formed twice).  32 x 14 x 14 x 448: 6.5 and 8 + 3 us.
 //
 // Statistics of slabs: a thread sums its values and their squares about its own first value, so that
 // what cancels is bounded by its own share of the variance; threads and slabs are joined by their
@@ -688,10 +688,10 @@ int32_t lanes_lg(int64_t n, int64_t groups, int32_t threads) {
 }
 
 // A bundle in one workgroup's registers, with runs of 128 bytes of a pixel (or all channels): four
-// vectors a thread of 256, or eight of 512.  32 x 14 x 14 x 448 bf16 take 7 us (slabs: 12), 128 of them
-// 13 (21), with the backward 42 (57).  Shorter runs waste the lines that they share (25 us with 32
-// bytes), larger workgroups leave a CU waiting for one (128 x 28 x 28 x 192 in 64-byte runs by 512
-// threads, forward and backward: 91 us, slabs 69).
+// vectors a thread of 256, or eight of 512.  32 x 14 x 14 x 448 bf16 take 6 us (slabs: 10), 128 of them
+// 13 (19), with the backward 42 (52).  Shorter runs waste the lines that they share (128 of them 25 us
+// with 32 bytes).  Runs of 64 bytes would hold 28 x 28 x 192 too: 32 of them forward 10 us (slabs 12), but
+// 128 forward and backward 79 (slabs 67).
 bool plan_resident(GNPlan& p, int64_t pixels, int64_t per, int64_t groups, int e) {
     const int64_t each = per / p.vec, bundle = std::min(groups, (127 + per * e) / (per * e));
     for (int threads : {256, GN_RESIDENT}) {

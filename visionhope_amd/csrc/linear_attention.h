@@ -206,8 +206,8 @@ __device__ __forceinline__ void la_store(T* row, int32_t col, int32_t dim, bool 
 // LDS tiles have rows of W values (32, 64 or 128) whose blocks of eight are permuted by the row: block b of
 // row r stands at b ^ la_fold(r).  Sixteen rows' blocks of one index then lie in sixteen different places
 // of the 256 bytes that the banks are wide, and so do the blocks that a transposing read takes from
-// four rows.  (Rows that were eight values longer instead: LDS cycles of the output pass at 8 x 784 x 8
-// heads of 128 4.7 M, 2.6 M of them conflicts, now 3.5 M and 1.5 M.)
+// four rows.  (Rows eight values longer instead: 203 against 197 us a training pass of 32 x 3136 x 3
+// heads of 64.)
 template <int W>
 __device__ __forceinline__ int32_t la_fold(int32_t row) {
     const int32_t low = (row >> 2) & 3;

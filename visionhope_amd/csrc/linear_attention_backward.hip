@@ -7,9 +7,9 @@
 //
 // with S the state before a chunk of n tokens and G the gradient of the state behind it.  dq starts from
 // the states that the forward left between its segments; G's are formed once, for dv, and read
-// transposed for dk.  32 x 3136 x 3 heads of 64 in bf16: 40 (dq) + 17 + 6 + 38 (dv) + 38 us (dk).  dk and
-// dv in one walk read a third less, but hold two workgroups a CU: 73 us for both at heads of 64, and
-// 30 % more at heads of 32.
+// transposed for dk.  32 x 3136 x 3 heads of 64 in bf16: 39 (dq) + 17 + 6 + 38 (dv) + 38 us (dk).  dk and
+// dv in one walk read a third less, but hold two workgroups a CU: 73 us instead of 77 for both there, and
+// 141 us instead of 118 for a whole training pass of 16 x 3136 x 6 heads of 32.
 //
 // A decay that is trained takes the states of both walks at every chunk, and one more pass:
 //   dlog_decay = sum over chunks of  sum_{i > j} (i-j) g^(i-j) scale (q[i] . k[j]) (do[i] . v[j])
