@@ -108,3 +108,13 @@ def test_cpu_tensors_are_refused():
                  lambda: visionhope_group_norm(torch.zeros(1, 8, 2, 2), 2, torch.ones(8), torch.zeros(8))):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+@pytest.mark.parametrize("change", [dict(B=1 << 15, H=32, N=65, K=128, V=128),   # 2^20 heads of 128 x 128 / 4 threads
+                                    dict(B=1 << 17, H=16, N=257, K=128, V=8),
+                                    dict(B=1 << 10, H=16, N=1 << 14, K=128, V=8)])   # 2^14 heads in 2^9 segments of 512 threads
+def test_launches_of_too_many_threads_are_refused(lib, change):
+    """A trained decay takes the states of every chunk: their passes may exceed the 2^32 threads of a launch."""
+    strides = {f"{n}{part}": 0 for n in ("do", "q", "k", "v") for part in "bth"}
+    assert _call(lib, "vh_linear_attention_backward", BACK, ddecay=P, ws=None, wsn=0, **strides, **change) == hip.VH_ERR_SHAPE
+    assert "range" in lib.vh_last_error().decode()

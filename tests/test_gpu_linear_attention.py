@@ -401,3 +401,19 @@ def test_only_the_state_has_a_gradient(device):
     assert got[0].abs().max() == 0 and grads[0] is None   # the oracle's last state does not read q
     for name, a, b in list(zip(NAMES, got, grads))[1:]:
         compare(a, b, tolerance(torch.float32, 2 * 50 * 130 if name == "log_decay" else 66), f"d{name}")
+
+
+@pytest.mark.parametrize("learned", [False, True])
+def test_a_graph_that_is_kept_gives_the_same_gradients_again(device, learned):
+    """The backward starts from the states that the forward left, and leaves them as they were."""
+    from visionhope_amd.utils.linear_attention import visionhope_linear_attention
+
+    shape = (1, 4096, 2, 32)   # cut into segments
+    q, k, v = (randn(*shape, seed=s).to(device).requires_grad_() for s in (1, 2, 3))
+    decay = torch.full((2,), -0.01, device=device, requires_grad=learned)
+    o = visionhope_linear_attention(q, k, v, decay)
+    do = randn(*shape, seed=4).to(device)
+    leaves = [q, k, v] + ([decay] if learned else [])
+    first = torch.autograd.grad(o, leaves, do, retain_graph=True)
+    again = torch.autograd.grad(o, leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))

@@ -334,6 +334,7 @@ struct LACut {   // segments of a line, and chunks of each (the last may have fe
 LACut la_cut(int64_t heads, int64_t N, int32_t padded, int32_t io_dtype);
 size_t la_slots_bytes(int64_t heads, const LACut& cut, int32_t padded);
 int la_check_sizes(int32_t io_dtype, int64_t B, int64_t N, int64_t heads, int64_t key_dim, int64_t value_dim);
+int la_check_cut(int64_t heads, const LACut& cut, int32_t padded);   // a launch has 2^32 threads at most
 int la_check_strides(std::initializer_list<int64_t> token_strides);   // below 2^24 elements
 // Runs a pass (sets its widths and its chunk itself); la_states: only as far as the states between
 // the segments.

@@ -411,6 +411,14 @@ int la_check_sizes(int32_t io_dtype, int64_t B, int64_t N, int64_t heads, int64_
     return VH_OK;
 }
 
+int la_check_cut(int64_t heads, const LACut& cut, int32_t padded) {
+    // 4 padded threads a workgroup of a pass; the join has one for every four values of a head's state
+    VH_REQUIRE(heads * cut.segments * 4 * padded < (1ll << 32) &&
+                   (cut.segments == 1 || heads * padded * padded / 4 <= (1ll << 32) - 256), VH_ERR_SHAPE,
+               "linear attention: %lld heads in %lld segments are out of range", (long long)heads, (long long)cut.segments);
+    return VH_OK;
+}
+
 int la_check_strides(std::initializer_list<int64_t> token_strides) {
     for (int64_t t : token_strides)
         VH_REQUIRE(t >= 0 && t < (1ll << 24), VH_ERR_SHAPE, "linear attention: a token stride of %lld is out of range", (long long)t);
@@ -530,6 +538,7 @@ int vh_linear_attention_forward(
                "state and new_state must not overlap");
     const int32_t padded = la_padded(key_dim, value_dim);
     const LACut cut = la_cut(B * heads, N, padded, io_dtype);
+    if (int rc = la_check_cut(B * heads, cut, padded)) return rc;
     const size_t need = la_slots_bytes(B * heads, cut, padded);
     VH_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                VH_ERR_WORKSPACE, "linear attention needs an aligned workspace of %zu bytes, got %zu", need, workspace_bytes);

@@ -223,8 +223,7 @@ int vh_linear_attention_backward(
     const bool decay = dlog_decay != nullptr;
     const LACut cut = backward_cut(B * heads, N, padded, io_dtype, decay);
     const size_t need = backward_bytes(B * heads, cut, padded, decay);
-    VH_REQUIRE(B * heads * cut.segments < (1ll << 23), VH_ERR_SHAPE,
-               "linear attention's backward: %lld heads of %lld tokens are out of range", (long long)(B * heads), (long long)N);
+    if (int rc = la_check_cut(B * heads, cut, padded)) return rc;
     VH_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                VH_ERR_WORKSPACE, "linear attention's backward needs an aligned workspace of %zu bytes, got %zu", need,
                workspace_bytes);
