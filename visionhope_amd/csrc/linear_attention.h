@@ -20,15 +20,16 @@ typedef __bf16 la_bf16x8 __attribute__((ext_vector_type(8)));
 typedef float la_f32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T> struct LAType;
-// raw: limbs of a tensor's values; tokens: of a chunk; formed: limbs of weights and states as
-// operands of a product that is rounded to T (2: 16 bits of them, so that the sum's one rounding
-// to T is the only one that counts)
-template <> struct LAType<bf16_t> { static constexpr int raw = 1, tokens = 64, formed = 2, order = 1; };
-template <> struct LAType<f16_t> { static constexpr int raw = 2, tokens = 32, formed = 2, order = 1; };
-template <> struct LAType<float> { static constexpr int raw = 3, tokens = 32, formed = 3, order = 2; };
+// raw: limbs of a tensor's values; tokens: of a chunk
+template <> struct LAType<bf16_t> { static constexpr int raw = 1, tokens = 64; };
+template <> struct LAType<f16_t> { static constexpr int raw = 2, tokens = 32; };
+template <> struct LAType<float> { static constexpr int raw = 3, tokens = 32; };
 
-// Limbs of what enters a state that is an FP32 result: 24 bits.
-constexpr int LA_STATE_LIMBS = 3;
+// Limbs of what is formed in FP32 (weights of pairs, states, what enters a state) and the order of
+// its products: 24 bits for every type, so that results do not depend on what else a call returns.
+// (Two limbs turn the rounding of 0.25 % of bf16 and of 2 % of FP16 results, three of 0.02 and 0.1 %:
+// 197 against 210 us a bf16 training pass of 32 x 3136 x 3 heads of 64.)
+constexpr int LA_FORMED = 3, LA_ORDER = 2;
 
 struct LATokens {   // an activation [B, N, heads, dim]: element strides of sequence, token and head
     const void* data;
@@ -42,10 +43,10 @@ __device__ __forceinline__ la_f32x4 la_mfma(const uint4& a, const uint4& b, la_f
 // c += a b over 32 values: lane l holds row (column) l % 16 of a (b), and of the contracted index
 // the eight values that group l / 16 has (any order, the same for both); of the result, rows
 // 4 (l / 16) .. + 3 in column l % 16.  Smallest products first.
-template <int ORDER, int NA, int NB>
+template <int NA, int NB>
 __device__ __forceinline__ la_f32x4 la_mm(const uint4 (&a)[NA], const uint4 (&b)[NB], la_f32x4 c) {
 #pragma unroll
-    for (int o = ORDER; o >= 0; --o)
+    for (int o = LA_ORDER; o >= 0; --o)
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
             const int j = o - i;
@@ -222,7 +223,7 @@ __device__ __forceinline__ int32_t la_block(int32_t row, int32_t b) {
 // Tiles of a chunk, for heads padded to D.
 template <typename T, int D>
 struct LAShape {
-    static constexpr int R = LAType<T>::raw, F = LAType<T>::formed, C = LAType<T>::tokens;
+    static constexpr int R = LAType<T>::raw, F = LA_FORMED, C = LAType<T>::tokens;
     static constexpr int waves = D / 16, threads = 64 * waves, units = C / 32;   // units: of eight values a thread
     static constexpr int tile = C * D, weights = C * C;   // one limb
     static constexpr int head = 512;                              // bytes of small tables
@@ -272,24 +273,16 @@ __device__ __forceinline__ void la_turned(const uint16_t* tile, int32_t at, int3
     }
 }
 
-// s += tiles of k^T v over a chunk: v's columns (weighted, FP32) as limbs, three where an FP32 result comes
-// of it and two where only values rounded to 16 bits do.
+// s += tiles of k^T v over a chunk: v's columns (weighted, FP32) as limbs.
 template <typename T, int D>
-__device__ __forceinline__ void la_enter(const uint16_t* ks, int32_t at, int32_t x, const float (&v)[8], bool fine,
-                                         la_f32x4 (&s)[D / 16]) {
-    constexpr int R = LAType<T>::raw;
-    uint4 vw[LA_STATE_LIMBS];
-    la_split8<LA_STATE_LIMBS>(v, vw);
-    const uint4 coarse[2] = {vw[0], vw[1]}, rest[1] = {vw[2]};
+__device__ __forceinline__ void la_enter(const uint16_t* ks, int32_t at, int32_t x, const float (&v)[8], la_f32x4 (&s)[D / 16]) {
+    uint4 vw[LA_FORMED];
+    la_split8<LA_FORMED>(v, vw);
 #pragma unroll
     for (int m = 0; m < D / 16; ++m) {
-        uint4 ka[R];
+        uint4 ka[LAType<T>::raw];
         la_turned<T, D, true>(ks, at, x, m, ka);
-        if (sizeof(T) == 4 || fine) {
-            const uint4 first[1] = {ka[0]};
-            s[m] = la_mm<0>(first, rest, s[m]);
-        }
-        s[m] = la_mm<2>(ka, coarse, s[m]);
+        s[m] = la_mm(ka, vw, s[m]);
     }
 }
 
@@ -316,7 +309,6 @@ struct LAPass {
     int32_t batches, tokens, heads, kdim, vdim, segments, chunks_per_segment, chunk, reversed;
     int32_t vec_q, vec_k, vec_v;   // elements of one load
     bool wide_out;
-    bool fine;               // an FP32 result comes of the states
 };
 
 // Tokens of a sequence.

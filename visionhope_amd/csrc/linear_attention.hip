@@ -38,7 +38,7 @@ __device__ __forceinline__ void la_triangle(int32_t tile, int32_t& it, int32_t& 
 template <typename T, int D, bool OUT, bool WIDE>
 __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kernel(const LAPass a) {
     using P = LAShape<T, D>;
-    constexpr int R = P::R, F = P::F, C = P::C, ORDER = LAType<T>::order;
+    constexpr int R = P::R, F = P::F, C = P::C;
     constexpr int TILES = C / 16, STEPS_C = C / 32, STEPS_D = D / 32, UNITS = P::units;
     extern __shared__ __align__(16) unsigned char la_lds[];
     float* entering = reinterpret_cast<float*>(la_lds);                     // [C]: weights of what enters the state
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
                     uint4 ka[R], qa[R];
                     la_read(ks, P::tile, 16 * jt * D + (at_row ^ (32 * x)), ka);
                     la_read(qs, P::tile, 16 * it * D + (at_row ^ (32 * x)), qa);
-                    w = la_mm<(R == 1 ? 0 : 2)>(ka, qa, w);
+                    w = la_mm(ka, qa, w);
                 }
                 if (it == jt) {
 #pragma unroll
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
                 for (int it = 0; it < TILES; ++it) {
                     uint4 qa[R];
                     la_read(qs, P::tile, 16 * it * D + (at_row ^ (32 * x)), qa);
-                    o[it] = la_mm<ORDER>(sa, qa, o[it]);
+                    o[it] = la_mm(sa, qa, o[it]);
                 }
             }
 #pragma unroll
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
             const float4 e1 = *reinterpret_cast<const float4*>(entering + 32 * x + 8 * g + 4);
             v[0] *= e0.x; v[1] *= e0.y; v[2] *= e0.z; v[3] *= e0.w;
             v[4] *= e1.x; v[5] *= e1.y; v[6] *= e1.z; v[7] *= e1.w;
-            la_enter<T, D>(ks, k_column, x, v, a.fine, s);
+            la_enter<T, D>(ks, k_column, x, v, s);
         }
         if constexpr (OUT) {
             __syncthreads();   // all weights are there
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(4 * D, D == 128 ? 2 : 3) void linear_attention_kern
                     if (32 * x < 16 * (it + 1)) {
                         uint4 wa[F];
                         la_read(ws, P::weights, 16 * it * C + (at_weights ^ (32 * x)), wa);
-                        o[it] = la_mm<ORDER>(va[x], wa, o[it]);
+                        o[it] = la_mm(va[x], wa, o[it]);
                     }
             T* out = static_cast<T*>(a.out) + ((batch * static_cast<int64_t>(a.tokens) + t0) * a.heads + head) * a.vdim;
 #pragma unroll
@@ -552,7 +552,6 @@ int vh_linear_attention_forward(
     a.scale_in = 1.f;
     a.state = state;
     a.new_state = new_state;
-    a.fine = new_state != nullptr;
     a.state_row = value_dim;
     a.state_col = 1;
     a.lengths = lengths;

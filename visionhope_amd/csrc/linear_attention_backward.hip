@@ -81,10 +81,10 @@ __global__ __launch_bounds__(4 * D, 2) void linear_attention_decay_kernel(const 
             const int32_t at = la_block<D>(n16, g) ^ (32 * x), of_j = 16 * jt * D + at, of_i = 16 * it * D + at;
             la_read(tiles + TILE, P::tile, of_j, m);
             la_read(tiles, P::tile, of_i, n);
-            w = la_mm<(R == 1 ? 0 : 2)>(m, n, w);
+            w = la_mm(m, n, w);
             la_read(tiles + 3 * TILE, P::tile, of_j, m);
             la_read(tiles + 2 * TILE, P::tile, of_i, n);
-            e = la_mm<(R == 1 ? 0 : 2)>(m, n, e);
+            e = la_mm(m, n, e);
         }
         const int32_t d = 16 * it + n16 - (16 * jt + 4 * g);
 #pragma unroll
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(4 * D, 2) void linear_attention_decay_kernel(const 
                 const int32_t t = 32 * x + 8 * g + i, m = part == 0 ? t + 1 : nt - 1 - t;
                 v[i] *= m > 0 ? powers[m] * (static_cast<float>(m) * (part == 0 ? a.scale : 1.f)) : 0.f;
             }
-            la_enter<T, D>(tiles + part * TILE, k_column, x, v, true, acc);
+            la_enter<T, D>(tiles + part * TILE, k_column, x, v, acc);
         }
 #pragma unroll
         for (int m = 0; m < D / 16; ++m)
@@ -251,7 +251,6 @@ int vh_linear_attention_backward(
         a.kdim = dk_;
         a.vdim = dv_;
         a.scale_in = 1.f;
-        a.fine = true;
         a.state = state;
         a.state_row = value_dim;
         a.state_col = 1;
@@ -289,7 +288,6 @@ int vh_linear_attention_backward(
     a.state_row = value_dim;
     a.state_col = 1;
     a.new_state = dstate;
-    a.fine = dstate != nullptr || decay;
     if (int rc = la_run(a, io_dtype, s)) return rc;
     a = base;
     a.q = tv;
