@@ -9,15 +9,17 @@
 //
 // Where a workgroup's registers hold a bundle of an image's groups, one launch reads the map once
 // (both directions).  Larger maps take two passes: partial sums of slabs of pixels, then the outputs,
-// whose workgroups join their image's slabs first.  128 x 56 x 56 x 96 bf16 with GELU: 15 + 33 us forward
-// (231 MB at 4.8 TB/s), 41 + 40 + 9 us backward, bound by the vector unit (33 instructions a value and
+// whose workgroups join their image's slabs first.  128 x 56 x 56 x 96 bf16 with GELU: 17 + 32 us forward
+// (231 MB at 4.7 TB/s), 41 + 40 + 9 us backward, bound by the vector unit (33 instructions a value and
 // pass: the activation's slope is formed twice).  32 x 14 x 14 x 448: 6.5 and 8 + 3 us.
 //
-// Statistics of slabs: a thread sums its values and their squares about its own first value, so that
-// what cancels is bounded by its own share of the variance; threads and slabs are joined by their
-// means and centred squares with the means in FP64.  Values in registers are centred about their
-// rounded mean, whose rest is summed beside the squares.  Either way the mean is kept as a sum of two
-// floats: an offset large beside the spread loses nothing.
+// Statistics of slabs: a thread takes its values in runs of about 32 from registers, each run's squares
+// centred about the run's own rounded mean, whose rest is summed beside them; runs, threads and slabs are
+// joined by their means and centred squares in FP64.  No long sum is of squares about a value that may
+// stand far from the others (sums about a thread's first value were 15 us there, and at 10^4 beside a
+// spread of one, 2048 x 96 x 96 x 16, rstd was off by 2.5e-4).  Values of a map in registers are centred about their rounded mean in
+// the same way.  Either way the mean is kept as a sum of two floats: an offset large beside the spread
+// loses nothing.
 #include <algorithm>
 
 #include "param_sum.h"
@@ -172,6 +174,39 @@ __device__ __forceinline__ GNPlace gn_place(const GNArgs& a) {
     return p;
 }
 
+// A vector as loaded, in whole words; unpacked when it is used.
+template <typename T, int VEC>
+struct GNRaw {
+    static constexpr int words = VEC * sizeof(T) < 4 ? 1 : VEC * sizeof(T) / 4;
+    uint32_t w[words];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (words == 4) {
+            const uint4 r = *reinterpret_cast<const uint4*>(p);
+            w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+        } else if constexpr (words == 2) {
+            const uint2 r = *reinterpret_cast<const uint2*>(p);
+            w[0] = r.x; w[1] = r.y;
+        } else if constexpr (VEC * sizeof(T) == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            w[0] = p->bits;
+        }
+    }
+    __device__ __forceinline__ void unpack(float (&v)[VEC]) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            if constexpr (sizeof(T) == 4) v[j] = __uint_as_float(w[j]);
+            else v[j] = to_f32(T{static_cast<uint16_t>(j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu)});
+        }
+    }
+    // What follows is computed from the words again: values of other places in the code are not carried
+    // here in registers.
+    __device__ __forceinline__ void forget() {
+#pragma unroll
+        for (int i = 0; i < words; ++i) asm volatile("" : "+v"(w[i]));
+    }
+};
+
 // Sums of one slab of one image: a group's mean and centred squares.
 template <typename T, int VEC>
 __global__ __launch_bounds__(1024) void group_norm_stats_kernel(const GNArgs a) {
@@ -181,23 +216,47 @@ __global__ __launch_bounds__(1024) void group_norm_stats_kernel(const GNArgs a) 
     const int32_t bundle = p.bundle, slab = p.slab;
     const int64_t image = p.image;
     if (p.live && p.row < p.pixels) {
-        float sum = 0.f, square = 0.f;
+        constexpr int RUN = VEC >= 4 ? 32 / VEC : 8;   // vectors
         const T* at = static_cast<const T*>(a.x) + (image * a.pixels + p.first_pixel) * a.channels + p.channel;
-        const float pivot = to_f32(at[static_cast<int64_t>(p.row) * a.channels]);
-#pragma unroll 4
-        for (int32_t i = p.row; i < p.pixels; i += p.rows) {
-            float v[VEC];
-            gn_load<T, VEC>(at + static_cast<int64_t>(i) * a.channels, v);
+        double mean = 0.0, centred = 0.0;
+        float n = 0.f;
+        for (int32_t i = p.row; i < p.pixels; i += RUN * p.rows) {
+            GNRaw<T, VEC> raw[RUN];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float d = v[j] - pivot;
-                sum += d;
-                square = fmaf(d, d, square);
-            }
+            for (int k = 0; k < RUN; ++k)
+                if (i + k * p.rows < p.pixels) raw[k].load(at + static_cast<int64_t>(i + k * p.rows) * a.channels);
+            float sum = 0.f, count = 0.f;
+#pragma unroll
+            for (int k = 0; k < RUN; ++k)
+                if (i + k * p.rows < p.pixels) {
+                    float v[VEC];
+                    raw[k].unpack(v);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) sum += v[j];
+                    count += VEC;
+                }
+            const float about = sum / count;
+            float off = 0.f, square = 0.f;
+#pragma unroll
+            for (int k = 0; k < RUN; ++k)
+                if (i + k * p.rows < p.pixels) {
+                    float v[VEC];
+                    raw[k].unpack(v);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        const float d = v[j] - about;
+                        off += d;
+                        square = fmaf(d, d, square);
+                    }
+                }
+            const float rest = off / count, share = count / (n + count);
+            const double d = static_cast<double>(about) + static_cast<double>(rest) - mean;
+            mean = fma(d, static_cast<double>(share), mean);
+            centred += fma(d * d, static_cast<double>(n * share), static_cast<double>(fmaxf(fmaf(-off, rest, square), 0.f)));
+            n += count;
         }
-        const float n = static_cast<float>((p.pixels - p.row + p.rows - 1) / p.rows * VEC), off = sum / n;
-        means[p.entry] = static_cast<double>(pivot) + static_cast<double>(off);
-        squares[p.entry] = fmaxf(fmaf(-sum, off, square), 0.f);
+        means[p.entry] = mean;
+        squares[p.entry] = static_cast<float>(centred);
         counts[p.entry] = n;
     }
     __syncthreads();
@@ -424,39 +483,6 @@ __global__ __launch_bounds__(1024) void group_norm_dx_kernel(const GNArgs a) {
         }
     });
 }
-
-// A vector as loaded, in whole words; unpacked when it is used.
-template <typename T, int VEC>
-struct GNRaw {
-    static constexpr int words = VEC * sizeof(T) < 4 ? 1 : VEC * sizeof(T) / 4;
-    uint32_t w[words];
-    __device__ __forceinline__ void load(const T* p) {
-        if constexpr (words == 4) {
-            const uint4 r = *reinterpret_cast<const uint4*>(p);
-            w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
-        } else if constexpr (words == 2) {
-            const uint2 r = *reinterpret_cast<const uint2*>(p);
-            w[0] = r.x; w[1] = r.y;
-        } else if constexpr (VEC * sizeof(T) == 4) {
-            w[0] = *reinterpret_cast<const uint32_t*>(p);
-        } else {
-            w[0] = p->bits;
-        }
-    }
-    __device__ __forceinline__ void unpack(float (&v)[VEC]) const {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            if constexpr (sizeof(T) == 4) v[j] = __uint_as_float(w[j]);
-            else v[j] = to_f32(T{static_cast<uint16_t>(j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu)});
-        }
-    }
-    // What follows is computed from the words again: values of other places in the code are not carried
-    // here in registers.
-    __device__ __forceinline__ void forget() {
-#pragma unroll
-        for (int i = 0; i < words; ++i) asm volatile("" : "+v"(w[i]));
-    }
-};
 
 // The whole of a bundle's map in one workgroup's registers, K vectors a thread.
 template <typename T, int VEC, int K>
