@@ -6,7 +6,7 @@ from torch import nn
 from torch.nn import functional as F
 
 from ..utils.grn import GlobalResponseNorm
-from ..utils.group_norm import ACTIVATIONS, visionhope_group_norm
+from ..utils.group_norm import ACTIVATIONS, MAX_GROUP_CHANNELS, visionhope_group_norm
 from ..utils.layer_norm_cuda import can_fuse_layernorm2d, visionhope_layernorm2d
 
 
@@ -58,8 +58,8 @@ class LayerNorm2d(nn.Module):
 class GroupNorm2d(nn.Module):
     """Group norm of an NCHW map, then ``activation`` (None, "silu" or "gelu") in the same pass.
 
-    ``groups`` defaults to one for every 16 channels, or to a single one where they do not divide.
-    GPU tensors run the native kernel and come out channels-last, in the input's dtype.
+    ``groups`` defaults to one for every 16 channels, or to a single one where they do not divide; a
+    group has at most 1024 channels.  GPU tensors run the native kernel and come out channels-last, in the input's dtype.
     """
 
     def __init__(self, dim, groups=None, eps=1e-5, activation=None):
@@ -67,6 +67,8 @@ class GroupNorm2d(nn.Module):
         self.groups = (dim // 16 if dim % 16 == 0 else 1) if groups is None else int(groups)
         if dim <= 0 or self.groups < 1 or dim % self.groups:
             raise ValueError(f"{dim} channels do not divide into {self.groups} groups")
+        if dim // self.groups > MAX_GROUP_CHANNELS:
+            raise ValueError(f"groups have at most {MAX_GROUP_CHANNELS} channels, got {dim // self.groups}; give groups")
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}")
         self.weight = nn.Parameter(torch.ones(dim))
