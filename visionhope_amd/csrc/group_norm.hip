@@ -11,15 +11,15 @@
 // (both directions).  Larger maps take two passes: partial sums of slabs of pixels, then the outputs,
 // whose workgroups join their image's slabs first.  128 x 56 x 56 x 96 bf16 with GELU: 17 + 32 us forward
 // (231 MB at 4.7 TB/s), 41 + 40 + 9 us backward, bound by the vector unit (33 instructions a value and
-// pass: the activation's slope is formed twice).  32 x 14 x 14 x 448: 6.5 and 8 + 3 us.
+// pass: the activation's slope is formed twice).  32 x 14 x 14 x 448: 6.7 and 9 + 4 us.
 //
 // Statistics of slabs: a thread takes its values in runs of about 32 from registers, each run's squares
 // centred about the run's own rounded mean, whose rest is summed beside them; runs, threads and slabs are
 // joined by their means and centred squares in FP64.  No long sum is of squares about a value that may
-// stand far from the others (sums about a thread's first value were 15 us there, and at 10^4 beside a
-// spread of one, 2048 x 96 x 96 x 16, rstd was off by 2.5e-4).  Values of a map in registers are centred about their rounded mean in
-// the same way.  Either way the mean is kept as a sum of two floats: an offset large beside the spread
-// loses nothing.
+// stand far from the others: about a thread's first value instead, 10^4 beside a spread of one, rstd was
+// off by 2.5e-4 at 2048 x 96 x 96 x 16 (and the statistics took 15 us where they take 17).  Values of a
+// map in registers are centred about their rounded mean in the same way.  Either way the mean is kept as a
+// sum of two floats: an offset large beside the spread loses nothing.
 #include <algorithm>
 
 #include "param_sum.h"
@@ -28,6 +28,9 @@ namespace vh {
 namespace {
 
 constexpr int GN_NONE = 0, GN_SILU = 1, GN_GELU = 2;
+// Slabs of an image, each a workgroup for every bundle; a workgroup of the second pass joins them all.  8 x
+// 128 x 128 x 96 bf16 takes 23.7 us forward (64 slabs: 24.4, 256: 25.1); one or two large maps would be
+// faster with more (1 x 512 x 512 x 96: 93 us, with 512 slabs 43).
 constexpr int64_t GN_MAX_SLABS = 128;
 constexpr int64_t GN_MAX_GROUP = 1024;    // channels of a group: a workgroup's threads
 constexpr int GN_RESIDENT = 512;          // threads, at most, that hold a map in registers
@@ -716,7 +719,7 @@ int32_t lanes_lg(int64_t n, int64_t groups, int32_t threads) {
 // vectors a thread of 256, or eight of 512.  32 x 14 x 14 x 448 bf16 take 6 us (slabs: 10), 128 of them
 // 13 (19), with the backward 42 (52).  Shorter runs waste the lines that they share (128 of them 25 us
 // with 32 bytes).  Runs of 64 bytes would hold 28 x 28 x 192 too: 32 of them forward 10 us (slabs 12), but
-// 128 forward and backward 79 (slabs 67).
+// 128 forward and backward 79 (slabs 69).
 bool plan_resident(GNPlan& p, int64_t pixels, int64_t per, int64_t groups, int e) {
     const int64_t each = per / p.vec, bundle = std::min(groups, (127 + per * e) / (per * e));
     for (int threads : {256, GN_RESIDENT}) {

@@ -208,7 +208,7 @@ __device__ __forceinline__ void la_store(T* row, int32_t col, int32_t dim, bool 
 // row r stands at b ^ la_fold(r).  Sixteen rows' blocks of one index then lie in sixteen different places
 // of the 256 bytes that the banks are wide, and so do the blocks that a transposing read takes from
 // four rows.  (Rows eight values longer instead: 203 against 197 us a training pass of 32 x 3136 x 3
-// heads of 64.)
+// heads of 64, with what is formed as two limbs.)
 template <int W>
 __device__ __forceinline__ int32_t la_fold(int32_t row) {
     const int32_t low = (row >> 2) & 3;

@@ -12,10 +12,10 @@
 // the reads, and the next chunk's values are on their way to registers meanwhile.
 //
 // Few heads and sequences are cut into segments: a pass for each segment's own last state, a
-// join over the segments, and the output pass (la_cut).  Bound by the bytes of q, k, v and o:
-// 32 x 3136 x 3 heads of 64 in bf16 take 18 + 5 + 38 us, the output pass 154 MB at 4.1 TB/s of a
-// copy's 4.9; 1 x 16384 x 16 heads 18 + 9 + 36.  Heads of 128 hold one workgroup a CU and wait for
-// latency (8 x 784 x 8 heads: 14 + 6 + 25 us, the output pass 51 MB at 2.0 TB/s).
+// join over the segments, and the output pass (la_cut).  Bound by the bytes of q, k, v and o, with vector
+// work beside them: 32 x 3136 x 3 heads of 64 in bf16 take 18 + 5 + 44 us, the output pass 154 MB at
+// 3.5 TB/s of a copy's 4.9; 1 x 16384 x 16 heads 16 + 9 + 40.  Heads of 128 hold one workgroup a CU and
+// wait for latency (8 x 784 x 8 heads: 14 + 6 + 27 us, the output pass 51 MB at 1.9 TB/s).
 //
 // The gradients are the same form with other operands (linear_attention_backward.hip): `reversed`
 // walks the tokens from the last one, where the state is the gradient of S behind a chunk and
@@ -367,8 +367,8 @@ LACut la_cut(int64_t heads, int64_t N, int32_t padded, int32_t io_dtype) {
     // The time of a cut, in chunks of a workgroup that has its CU to itself: a second and a third one there
     // cost a third each; segments cost a pass for their states, 45 % of the outputs', a launch, and the
     // states' way to memory and back twice, beside chunks that take 0.57 of that time for their own bytes.
-    // (bf16 heads of 64: 3.2, 4.2 and 5.4 us a chunk.  96 heads of 49 chunks take 61 us in 7 segments and
-    // 67 in 5; 304 of 13 take 53 us whole, 59 in 2 segments and 67 in 5.)  `held`: workgroups that the
+    // (bf16 heads of 64: 3.1 us a chunk of one workgroup a CU, 4.5 of two.  96 heads of 49 chunks take 151 us
+    // whole, 93 in 3 segments, 71 in 5 and in 7; 304 of 13 take 59 us whole, 60 in 2 segments, 70 in 5.)  `held`: workgroups that the
     // card holds at once, by registers and LDS; more of them wait for the end of others.
     const int64_t held = padded == 32 ? 1024 : padded == 64 ? 768 : 256, cus = 256;
     const int64_t chunks = la_ceil(N, la_chunk(io_dtype));

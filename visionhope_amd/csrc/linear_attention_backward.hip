@@ -7,14 +7,15 @@
 //
 // with S the state before a chunk of n tokens and G the gradient of the state behind it.  dq starts from
 // the states that the forward left between its segments; G's are formed once, for dv, and read
-// transposed for dk.  32 x 3136 x 3 heads of 64 in bf16: 39 (dq) + 17 + 6 + 38 (dv) + 38 us (dk).  dk and
-// dv in one walk read a third less, but hold two workgroups a CU: 73 us instead of 77 for both there, and
-// 141 us instead of 118 for a whole training pass of 16 x 3136 x 6 heads of 32.
+// transposed for dk.  32 x 3136 x 3 heads of 64 in bf16: 45 (dq) + 17 + 6 + 43 (dv) + 43 us (dk).  dk and
+// dv in one walk read a third less, but hold two workgroups a CU: with operands of two bf16 values 73 us
+// instead of 77 for both there, and 141 instead of 118 for a training pass of 16 x 3136 x 6 heads of 32.
 //
 // A decay that is trained takes the states of both walks at every chunk, and one more pass:
 //   dlog_decay = sum over chunks of  sum_{i > j} (i-j) g^(i-j) scale (q[i] . k[j]) (do[i] . v[j])
 //              + <S, sum_i (i+1) g^(i+1) scale q[i] do[i]^T + n g^n G> + <G, sum_j (n-1-j) g^(n-1-j) k[j] v[j]^T>
-// Powers stand beside small steps only, so nothing large cancels.
+// Powers stand beside small steps only, so nothing large cancels.  A training pass of 32 x 3136 x 3 heads of
+// 64 in bf16 takes 464 us with it and 217 without, of 8 x 784 x 8 in FP32 174 and 103.
 #include "linear_attention.h"
 
 namespace vh {

@@ -59,7 +59,8 @@ class GroupNorm2d(nn.Module):
     """Group norm of an NCHW map, then ``activation`` (None, "silu" or "gelu") in the same pass.
 
     ``groups`` defaults to one for every 16 channels, or to a single one where they do not divide; a
-    group has at most 1024 channels.  GPU tensors run the native kernel and come out channels-last, in the input's dtype.
+    group has at most 1024 channels.  GPU tensors run the native kernel and come out channels-last,
+    in the input's dtype.
     """
 
     def __init__(self, dim, groups=None, eps=1e-5, activation=None):

@@ -121,8 +121,8 @@ def visionhope_linear_attention(q, k, v, log_decay, *, scale=None, state=None, l
     a sequence's end are zero, whatever stands there.  Returns o in q's dtype, or
     ``(o, new_state)`` with ``return_state``.  q, k and v may be slices of wider tensors or expanded
     over heads (keys and values that heads share); results are dense.  Differentiable in every
-    tensor but lengths.  Values within a sequence must be finite: one that is not may reach
-    the outputs of the 64 tokens around it.
+    tensor but lengths.  Values within a sequence must be finite: a key or value that is not
+    reaches, in its head, every later output through the state and earlier ones of its chunk of 64.
     """
     name = "visionhope_linear_attention"
     check_io(name, q, 4)
